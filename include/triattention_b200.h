@@ -311,6 +311,42 @@ int tri_qk_accumulators(const int32_t* requests, int num_requests, const void* q
                         const void* k4x, int32_t* acc, int batch, int heads_q, int heads_kv, int tokens,
                         int* device_error, void* stream);
 
+/* ---- INT8 projections: the matrix products around the attention (no counterpart in the reference, whose models run theirs
+ * in bf16 through torch) -----------------------------------------------------------------------------------------------
+ * Rows of codes: int8, symmetric, one f32 scale per row; a row stands for scale * code.  Code rows start on 16-byte
+ * boundaries (base pointer and codes_stride, in bytes).  Element types of the other tensors: */
+enum { TRI_BF16 = 0, TRI_FP16 = 1, TRI_FP32 = 2 };
+/* Strides are in elements, features contiguous; width 1..131071 (128 * 128 * width < 2^31); rows = 0 is a no-op.
+ * scale = max|y| / 127, code = rint(y / scale).  A row whose largest magnitude is below 2^-119 gets scale 0 and codes 0; a row
+ * with a NaN, an infinity or an overflow in it gets scale NaN and codes 0.  Output buffers must not overlap inputs, except
+ * residual_out, which may be residual or x itself (same stride). */
+
+/* y = x. */
+int tri_quantize_rows(const void* x, int type, int64_t rows, int width, int64_t x_stride, void* codes, int64_t codes_stride,
+                      float* scales, void* stream);
+
+/* y = gate / (1 + exp(-gate)) * up, in f32; gate and up may be the halves of one tensor. */
+int tri_silu_mul_rows(const void* gate, const void* up, int type, int64_t rows, int width, int64_t gate_stride,
+                      int64_t up_stride, void* codes, int64_t codes_stride, float* scales, void* stream);
+
+/* h = x + residual rounded to the type (written to residual_out; x itself without a residual: both pointers NULL),
+ * y = h / sqrt(mean h^2 + eps) * weight[width] in f32.  eps 0..1. */
+int tri_rms_norm_rows(const void* x, const void* residual, const void* weight, int type, int64_t rows, int width,
+                      int64_t x_stride, int64_t residual_stride, double eps, void* residual_out, int64_t residual_out_stride,
+                      void* codes, int64_t codes_stride, float* scales, void* stream);
+
+/* out = scale * code, rounded to the type. */
+int tri_dequantize_rows(const void* codes, int64_t codes_stride, const float* scales, int type, int64_t rows, int width,
+                        void* out, int64_t out_stride, void* stream);
+
+/* out[t][n] = (sum_k codes[t][k] weight[n][k]) * weight_scales[n] * scales[t] + bias[n] + residual[t][n]: the sum is an exact
+ * 32-bit integer, the rest f32, rounded once to the type.  codes int8 [tokens,width], weight int8 [outputs,width] (both code
+ * rows), scales f32 [tokens], weight_scales f32 [outputs]; bias [outputs] and residual [tokens,outputs] of the output's type
+ * or NULL.  out must not overlap any input except residual itself (same stride). */
+int tri_int8_linear(const void* codes, int64_t codes_stride, const float* scales, const void* weight, int64_t weight_stride,
+                    const float* weight_scales, const void* bias, const void* residual, int64_t residual_stride, void* out,
+                    int64_t out_stride, int type, int64_t tokens, int outputs, int width, int* device_error, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,123 @@
+"""INT8 projections without a GPU: what the entry points refuse (before any CUDA call) and how rows of codes are held."""
+import pytest
+import torch
+
+from triattention_b200.kernels import extension
+from triattention_b200.kernels.extension import MAX_WIDTH, Module, load_library
+from triattention_b200.kernels.linear import Int8Ops, Int8Rows
+
+P = 4096            # a 16-byte aligned address that a refused call never touches
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return load_library()
+
+
+def refused(lib, status, what):
+    assert status == -1 and what in lib.tri_last_error().decode(), lib.tri_last_error()
+
+
+def test_row_entry_points_refuse_bad_arguments(lib):
+    def quantize(x=P, type=0, rows=4, width=64, stride=64, codes=P, pitch=64, scales=P):
+        return lib.tri_quantize_rows(x, type, rows, width, stride, codes, pitch, scales, None)
+
+    for bad in (dict(width=0), dict(width=MAX_WIDTH + 1), dict(width=-5), dict(type=3), dict(type=-1), dict(rows=-1), dict(rows=1 << 31)):
+        refused(lib, quantize(**bad), "quantize_rows: rows, width")
+    for bad in (dict(x=None), dict(codes=None), dict(scales=None)):
+        refused(lib, quantize(**bad), "null")
+    for bad in (dict(codes=P + 8), dict(pitch=72), dict(pitch=48)):
+        refused(lib, quantize(**bad), "16-byte")
+    for bad in (dict(x=P + 1), dict(x=P + 2, type=2), dict(stride=-64)):
+        refused(lib, quantize(**bad), "input rows")
+    assert quantize(rows=0, x=None, codes=None, scales=None) == 0          # an empty batch is no work
+
+    def gated(gate=P, up=P, type=1, rows=4, width=64, codes=P, pitch=64):
+        return lib.tri_silu_mul_rows(gate, up, type, rows, width, 128, 128, codes, pitch, P, None)
+
+    refused(lib, gated(up=None), "silu_mul_rows: null")
+    refused(lib, gated(up=P + 1), "silu_mul_rows: input rows")
+    refused(lib, gated(pitch=63), "silu_mul_rows: code rows")
+    refused(lib, gated(width=MAX_WIDTH + 1), "silu_mul_rows: rows, width")
+    assert gated(rows=0) == 0
+
+    def norm(x=P, residual=P, weight=P, rows=4, width=64, eps=1e-6, out=P, out_stride=64, codes=P):
+        return lib.tri_rms_norm_rows(x, residual, weight, 0, rows, width, 64, 64, eps, out, out_stride, codes, 64, P, None)
+
+    refused(lib, norm(weight=None), "rms_norm_rows: null")
+    refused(lib, norm(residual=None), "both or none")
+    refused(lib, norm(out=None), "both or none")
+    for eps in (-1e-9, 1.5, float("nan")):
+        refused(lib, norm(eps=eps), "eps")
+    refused(lib, norm(out_stride=63), "overlap")
+    refused(lib, norm(weight=P + 1), "input rows")
+    refused(lib, norm(codes=P + 4), "16-byte")
+    assert norm(rows=0) == 0
+
+    def values(codes=P, pitch=64, type=0, rows=2, width=64, out=P, out_stride=64):
+        return lib.tri_dequantize_rows(codes, pitch, P, type, rows, width, out, out_stride, None)
+
+    refused(lib, values(codes=None), "dequantize_rows: null")
+    refused(lib, values(pitch=65), "16-byte")
+    refused(lib, values(out_stride=60), "output rows")
+    refused(lib, values(out=P + 2, type=2), "output rows")
+    assert values(rows=0) == 0
+
+
+def test_linear_entry_point_refuses_bad_arguments(lib):
+    def linear(codes=P, pitch=64, scales=P, weight=P, weight_pitch=64, weight_scales=P, bias=None, residual=None, residual_stride=0,
+               out=P, out_stride=32, type=0, tokens=4, outputs=32, width=64, error=P):
+        return lib.tri_int8_linear(codes, pitch, scales, weight, weight_pitch, weight_scales, bias, residual, residual_stride, out,
+                                   out_stride, type, tokens, outputs, width, error, None)
+
+    for bad in (dict(width=0), dict(width=MAX_WIDTH + 1), dict(outputs=0), dict(tokens=-1), dict(tokens=1 << 31), dict(type=5)):
+        refused(lib, linear(**bad), "int8_linear: tokens, outputs, width")
+    for name in ("codes", "scales", "weight", "weight_scales", "out", "error"):
+        refused(lib, linear(**{name: None}), "int8_linear: null")
+    for bad in (dict(codes=P + 1), dict(weight=P + 8), dict(pitch=80 + 8), dict(weight_pitch=63), dict(pitch=48), dict(weight_pitch=0)):
+        refused(lib, linear(**bad), "16-byte")
+    for bad in (dict(out=P + 1), dict(bias=P + 1), dict(residual=P + 2, type=2)):
+        refused(lib, linear(**bad), "alignment")
+    for bad in (dict(out_stride=31), dict(residual=P, residual_stride=-1)):
+        refused(lib, linear(**bad), "output and residual rows")
+    assert linear(tokens=0) == 0
+
+
+def test_module_and_ops_refuse_host_tensors_and_shapes(lib):
+    module, ops = Module(lib), Int8Ops(Module(lib))
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="on a GPU"):
+        ops.quantize_rows(x)
+    with pytest.raises(RuntimeError, match="on a GPU"):
+        ops.silu_mul(x, x)
+    with pytest.raises(RuntimeError, match="on a GPU"):
+        ops.rms_norm(x, x[0], 1e-6)
+    with pytest.raises(RuntimeError, match="on a GPU"):
+        ops.linear(Int8Rows(x.to(torch.int8), torch.ones(4)), Int8Rows(x.to(torch.int8), torch.ones(4)))
+    with pytest.raises(RuntimeError, match="on a GPU"):
+        module.dequantize_rows(x.to(torch.int8), torch.ones(4), x)
+    with pytest.raises(RuntimeError, match="one shape"):
+        ops.silu_mul(x, x[:, :32])
+    with pytest.raises(RuntimeError, match="one shape"):
+        ops.rms_norm(x, x[0], 1e-6, residual=x[:1])
+    with pytest.raises(RuntimeError, match="rows of 1"):
+        ops.quantize_rows(torch.zeros(1, MAX_WIDTH + 1))
+    with pytest.raises(RuntimeError, match="rows of 1"):
+        ops.quantize_rows(torch.zeros(3, 0))
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.quantize_rows(x.requires_grad_())
+
+
+def test_rows_of_codes_are_checked():
+    codes = torch.zeros(2, 3, 16, dtype=torch.int8)
+    rows = Int8Rows(codes, torch.ones(2, 3))
+    assert rows.shape == (2, 3, 16) and rows.dtype == torch.bfloat16 and rows.device == codes.device
+    for bad in ((codes.float(), torch.ones(2, 3)), (codes, torch.ones(2, 3).double()), (codes, torch.ones(6)), (codes, torch.ones(2, 3, 1))):
+        with pytest.raises(RuntimeError, match="Int8Rows"):
+            Int8Rows(*bad)
+
+
+def test_a_library_without_an_entry_point_asks_to_be_rebuilt(monkeypatch):
+    monkeypatch.setitem(extension.SIGNATURES, "tri_not_there", [])
+    with pytest.raises(RuntimeError, match="tri_not_there: rebuild"):
+        load_library()

@@ -1,0 +1,369 @@
+"""INT8 projections on the GPU against their definitions in float64.
+
+Tolerances.  A code is rint(y * (127 / max|y|)) with two fp32 roundings before the rint, so it lies within half a step of the
+exact quotient, plus 127 * 2^-23 for those roundings and whatever error y itself has.  A product is an exact integer, converted
+(one rounding), scaled twice, added to up to twice (2^-24 of the operands' magnitude each) and rounded once to the output's type
+(half a step: finfo.eps / 2)."""
+import numpy as np
+import pytest
+import torch
+
+from triattention_b200.kernels.linear import Int8Ops, Int8Rows
+
+pytestmark = pytest.mark.gpu
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = (BF16, FP16, FP32)
+U = 2.0 ** -24          # half a step of fp32, relative
+
+
+@pytest.fixture(scope="module")
+def ops(module):
+    return Int8Ops(module)
+
+
+def randn(*shape, seed=0, dtype=BF16, outliers=False):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    x = torch.randn(*shape, generator=gen, device="cuda")
+    if outliers:
+        x = x * torch.where(torch.rand(shape[-1], generator=gen, device="cuda") < 0.02, 20.0, 1.0)
+    return x.to(dtype)
+
+
+def check_codes(rows, y, slack=0.0):
+    """rows against the exact values y (float64 [T,H]); slack: relative error that y itself may have in fp32."""
+    codes, scales = rows.codes.reshape(y.shape).double(), rows.scales.reshape(-1).double()
+    largest = y.abs().amax(1)
+    assert rows.codes.dtype == torch.int8 and rows.scales.dtype == FP32
+    torch.testing.assert_close(scales, largest / 127, rtol=slack + 4 * U, atol=0)
+    quotient = torch.where(largest[:, None] > 0, y / largest[:, None] * 127, 0.0)
+    assert float((codes - quotient).abs().max()) <= 0.5 + 127 * (2 * U + 2 * slack)
+    assert int(codes.abs().max()) <= 127
+
+
+WIDTHS = [(1, 1), (1, 7), (3, 16), (2, 129), (5, 1000), (4, 1024), (33, 4096), (2, 5001), (3, 8192), (2, 14336), (2, 16384),
+          (2, 32768), (1, 40000), (1, 131071), (700, 128), (1500, 65)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", WIDTHS)
+def test_quantize_rows(ops, rows, width, dtype):
+    x = randn(rows, width, seed=rows + width, dtype=dtype, outliers=True)
+    check_codes(ops.quantize_rows(x), x.double())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", WIDTHS)
+def test_silu_mul(ops, rows, width, dtype):
+    gate, up = 3 * randn(rows, width, seed=1, dtype=dtype), randn(rows, width, seed=2, dtype=dtype, outliers=True)
+    g, u = gate.double(), up.double()
+    # __expf: 2 + 1.173 |x| steps of 2^-23; __fdividef: 2 steps; the sum and the product half a step each
+    slack = (2 + 1.173 * float(g.abs().max()) + 2 + 1) * 2 * U
+    check_codes(ops.silu_mul(gate, up), g * torch.sigmoid(g) * u, slack)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", WIDTHS)
+@pytest.mark.parametrize("residual", (False, True))
+def test_rms_norm(ops, rows, width, dtype, residual):
+    x, w = randn(rows, width, seed=3, dtype=dtype, outliers=True), (1 + 0.2 * randn(width, seed=4, dtype=FP32)).to(dtype)
+    r = 3 * randn(rows, width, seed=5, dtype=dtype) if residual else None
+    got = ops.rms_norm(x, w, 1e-5, residual=r)
+    h = x
+    if residual:
+        got, total = got
+        h = (x.float() + r.float()).to(dtype)
+        assert total.dtype == dtype and torch.equal(total, h)
+    h = h.double()
+    y = h / (h.square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+    # h * w, rsqrt, division, products: half a step each; the sum of squares: at most a few steps (partial sums by thread)
+    check_codes(got, y, slack=(8 + width / 256 + 16) * U)
+
+
+def test_rows_that_hold_nothing_or_too_much(ops):
+    inf, nan = float("inf"), float("nan")
+    for dtype in TYPES:
+        for width in (24, 333, 4096, 40000):
+            x = randn(9, width, seed=6, dtype=dtype)
+            x[1] = 0
+            x[2, width - 1] = nan
+            x[3, 0] = inf
+            x[4, width // 2] = -inf
+            x[5] = -0.0
+            x[6] = torch.finfo(dtype).max
+            x[7], x[7, 3] = 0, -torch.finfo(dtype).max
+            rows = ops.quantize_rows(x)
+            assert rows.scales[[1, 5]].tolist() == [0, 0] and not rows.codes[[1, 2, 3, 4, 5]].any()
+            assert torch.isnan(rows.scales[2:5]).all()
+            ok = [0, 6, 7, 8]
+            check_codes(Int8Rows(rows.codes[ok], rows.scales[ok]), x[ok].double())
+            back = ops.dequantize(rows, FP32)
+            assert torch.isnan(back[2:5]).all() and not back[[1, 5]].any() and torch.isfinite(back[ok]).all()
+            gated = ops.silu_mul(x, torch.ones_like(x))
+            assert gated.scales[[1, 5]].tolist() == [0, 0] and torch.isnan(gated.scales[2:5]).all()
+            assert not gated.codes[[1, 2, 3, 4, 5]].any()
+            for eps in (1e-5, 0.0):
+                normed = ops.rms_norm(x, torch.ones(width, dtype=dtype, device="cuda"), eps)
+                assert normed.scales[[1, 5]].tolist() == [0, 0] and torch.isnan(normed.scales[2:5]).all()
+                assert not normed.codes[[1, 2, 3, 4, 5]].any()
+                h = x[ok].double()
+                check_codes(Int8Rows(normed.codes[ok], normed.scales[ok]), h / (h.square().mean(1, keepdim=True) + eps).sqrt(),
+                            slack=(24 + width / 256) * U)
+
+
+@pytest.mark.parametrize("size", (1e30, 1e19, 1e-15, 1e-25, 1e-30))
+@pytest.mark.parametrize("eps", (0.0, 1e-6))
+@pytest.mark.parametrize("residual", (False, True))
+def test_norm_of_rows_whose_squares_leave_fp32(ops, size, eps, residual):
+    x = (randn(4, 777, seed=7, dtype=FP32) * size).to(BF16)
+    w = torch.full((777,), 0.5, dtype=BF16, device="cuda")
+    r = (randn(4, 777, seed=8, dtype=FP32) * size).to(BF16) if residual else None
+    got = ops.rms_norm(x, w, eps, residual=r)
+    h = (x if r is None else x + r).double()
+    y = h / (h.square().mean(1, keepdim=True) + eps).sqrt() * 0.5
+    check_codes(got if r is None else got[0], y, slack=32 * U)
+    # in place: the new residual over the old one
+    if residual:
+        codes, scales = torch.empty(4, 784, dtype=torch.int8, device="cuda")[:, :777], torch.empty(4, device="cuda")
+        ops.module.rms_norm_rows(x, w, eps, codes, scales, r, r)
+        assert torch.equal(r, got[1]) and torch.equal(codes, got[0].codes) and torch.equal(scales, got[0].scales)
+
+
+def test_rows_strided_offset_and_shaped(ops):
+    """Halves of one tensor, every offset of the first element, a broadcast row, leading dimensions, an empty batch."""
+    wide = randn(40, 3 * 1000 + 8, seed=9)
+    for off in range(9):
+        x = wide[:, off:off + 1000]
+        got, want = ops.quantize_rows(x), ops.quantize_rows(x.contiguous())
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+        up = wide[:, 2000 + off // 2:3000 + off // 2]
+        got, want = ops.silu_mul(x, up), ops.silu_mul(x.contiguous(), up.contiguous())
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+        w = wide[0, 3 + off:1003 + off]
+        (got, total), (want, sums) = ops.rms_norm(x, w, 1e-6, residual=up), ops.rms_norm(x.contiguous(), w.clone(), 1e-6, residual=up.contiguous())
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales) and torch.equal(total, sums)
+    one = randn(1, 96, seed=10)
+    many = ops.quantize_rows(one.expand(5, 96))
+    assert torch.equal(many.codes, ops.quantize_rows(one).codes.expand(5, 96))
+    x = randn(2, 3, 130, seed=11)
+    rows = ops.quantize_rows(x)
+    assert rows.shape == (2, 3, 130) and rows.scales.shape == (2, 3) and rows.dtype == BF16
+    assert torch.equal(rows.codes.reshape(6, 130), ops.quantize_rows(x.reshape(6, 130)).codes)
+    assert ops.dequantize(rows).shape == x.shape and ops.dequantize(rows).dtype == BF16
+    flat = ops.quantize_rows(x[0, 0])
+    assert flat.shape == (130,) and flat.scales.shape == () and torch.equal(flat.codes, rows.codes[0, 0])
+    none = ops.quantize_rows(x[:0])
+    assert none.shape == (0, 3, 130) and ops.dequantize(none).shape == (0, 3, 130)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 129), (17, 4096), (2, 16400), (1000, 65)])
+def test_dequantize(ops, rows, width, dtype):
+    got = ops.quantize_rows(randn(rows, width, seed=12))
+    out = ops.dequantize(got, dtype)
+    assert out.dtype == dtype and torch.equal(out, (got.codes.float() * got.scales[:, None]).to(dtype))
+
+
+# ---- products --------------------------------------------------------------------------------------------------------
+
+def codes_rows(rows, width, seed, low=-127, high=128, extra=0):
+    """Random code rows whose rows lie `extra` more 16-byte units apart than they must."""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    pitch = (-(-width // 16) + extra) * 16
+    codes = torch.randint(low, high, (rows, pitch), generator=gen, device="cuda", dtype=torch.int8)[:, :width]
+    return Int8Rows(codes, torch.rand(rows, generator=gen, device="cuda") * 0.01 + 1e-4)
+
+
+def check_linear(ops, x, w, dtype=BF16, bias=None, residual=None, got=None):
+    if got is None:
+        got = ops.linear(x, w, bias=bias, residual=residual, dtype=dtype)
+    total = x.codes.double() @ w.codes.double().T               # exact: below 2^53
+    y = total * w.scales.double() * x.scales.double()[:, None]
+    size = y.abs() * 3
+    for more in (bias, residual):
+        if more is not None:
+            y = y + more.double()
+            size = size + more.double().abs() + y.abs()
+    far = (got.double() - y).abs() - (U * 2 * size + y.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -25 * (dtype == FP16))
+    assert got.dtype == dtype and got.shape == y.shape
+    assert not far.numel() or float(far.max()) <= 0, (float(far.max()), int((far > 0).sum()))
+    return got
+
+
+SHAPES = [(1, 1, 1), (1, 17, 33), (2, 8, 16), (3, 128, 64), (7, 130, 127), (1, 4096, 4096), (8, 512, 1024), (16, 256, 4096),
+          (16, 1000, 4099), (17, 129, 160), (31, 384, 8192), (32, 4608, 3584), (33, 96, 96), (64, 300, 1000), (65, 127, 2000),
+          (100, 2000, 500), (127, 640, 2048), (128, 128, 128), (129, 257, 2051), (200, 1111, 777), (255, 256, 512), (256, 4096, 1024),
+          (257, 513, 130), (300, 1000, 100), (511, 384, 384), (512, 512, 512), (777, 1003, 1051), (1000, 640, 512), (1500, 2048, 256),
+          (2049, 1025, 129), (4096, 512, 640), (3, 20000, 48), (5000, 3, 48), (700, 5000, 17), (2, 2, 30000), (24, 24, 131071)]
+
+
+@pytest.mark.parametrize("tokens,outputs,width", SHAPES)
+def test_linear(ops, tokens, outputs, width):
+    x, w = codes_rows(tokens, width, 1), codes_rows(outputs, width, 2)
+    check_linear(ops, x, w)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,outputs,width", [(1, 4096, 512), (5, 333, 1000), (48, 640, 4096), (130, 1001, 300), (600, 777, 1024),
+                                                  (2048, 1024, 512)])
+@pytest.mark.parametrize("with_bias,with_residual", [(True, False), (False, True), (True, True)])
+def test_linear_types_bias_residual(ops, tokens, outputs, width, dtype, with_bias, with_residual):
+    x, w = codes_rows(tokens, width, 3, low=-128), codes_rows(outputs, width, 4, low=-128, extra=1)
+    check_linear(ops, x, w, dtype, randn(outputs, seed=5, dtype=dtype) if with_bias else None,
+                 randn(tokens, outputs, seed=6, dtype=dtype) if with_residual else None)
+
+
+@pytest.mark.parametrize("tokens,outputs", [(2, 130), (200, 140)])
+def test_linear_largest_sums(ops, tokens, outputs):
+    """Every product at its largest, at the widest row: 131071 * 128 * 128 = 2^31 - 16384."""
+    x, w = codes_rows(tokens, 131071, 7), codes_rows(outputs, 131071, 8)
+    x.codes.fill_(-128), w.codes.fill_(-128)
+    x.scales.fill_(1), w.scales.fill_(1)
+    assert torch.equal(ops.linear(x, w, dtype=FP32), torch.full((tokens, outputs), 2147467264.0, device="cuda"))
+    w.codes.fill_(127)
+    assert torch.equal(ops.linear(x, w, dtype=FP32), torch.full((tokens, outputs), -128.0 * 127 * 131071, device="cuda"))
+
+
+@pytest.mark.parametrize("tokens", (1, 40, 300, 1100))
+def test_linear_writes_its_rows_only(ops, tokens):
+    """Output, residual and codes inside wider buffers: nothing beside the rows is written, nothing beside them is read."""
+    outputs, width = 333, 250
+    x, w = codes_rows(tokens, width, 9, extra=2), codes_rows(outputs, width, 10, extra=3)
+    for rows in (x.codes, w.codes):      # what lies between the rows changes nothing
+        base = rows.as_strided((rows.shape[0], rows.stride(0)), (rows.stride(0), 1))
+        base[:, width:] = 77
+    room = torch.full((tokens + 2, outputs + 9), 7.0, dtype=BF16, device="cuda")
+    out = room[1:-1, 5:5 + outputs]
+    residual = randn(tokens, outputs + 3, seed=11)[:, 2:-1]
+    ops.module.int8_linear(x.codes, x.scales, w.codes, w.scales, out, residual=residual)
+    check_linear(ops, x, w, residual=residual, got=out)
+    kept = torch.full_like(room, 7.0)
+    kept[1:-1, 5:5 + outputs] = out
+    assert torch.equal(room, kept)
+    want = out.clone()
+    out.copy_(residual)                  # the residual stream updated in place
+    ops.module.int8_linear(x.codes, x.scales, w.codes, w.scales, out, residual=out)
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("tokens", (3, 70, 700))
+def test_linear_keeps_a_bad_row_to_itself(ops, tokens):
+    x, w = codes_rows(tokens, 512, 12), codes_rows(200, 512, 13)
+    x.scales[1] = float("nan")
+    x.codes[2].zero_()
+    x.scales[2] = 0
+    got = ops.linear(x, w, bias=torch.ones(200, dtype=BF16, device="cuda"))
+    assert torch.isnan(got[1]).all() and (got[2] == 1).all()
+    keep = [t for t in range(tokens) if t != 1]
+    check_linear(ops, Int8Rows(x.codes[keep], x.scales[keep]), w, bias=torch.ones(200, dtype=BF16, device="cuda"), got=got[keep])
+
+
+def test_linear_shapes_and_empty_batch(ops):
+    x, w = codes_rows(6, 160, 14), codes_rows(64, 160, 15)
+    flat = ops.linear(x, w)
+    cube = Int8Rows(x.codes.view(2, 3, 160), x.scales.view(2, 3))
+    got = ops.linear(cube, w, residual=torch.zeros(2, 3, 64, dtype=BF16, device="cuda"))
+    assert got.shape == (2, 3, 64) and torch.equal(got.view(6, 64), flat)
+    assert ops.linear(Int8Rows(x.codes[:0], x.scales[:0]), w).shape == (0, 64)
+    one = ops.linear(Int8Rows(x.codes[0], x.scales[0]), w)
+    assert one.shape == (64,) and torch.equal(one, ops.linear(Int8Rows(x.codes[:1], x.scales[:1]), w)[0])
+
+
+def test_same_bits_every_time(ops):
+    """The sums are integers, so no order of the work shows in the result."""
+    for tokens, outputs, width in ((1, 4096, 8192), (40, 1000, 14336), (520, 1000, 4096)):
+        x, w = codes_rows(tokens, width, 16), codes_rows(outputs, width, 17)
+        first = ops.linear(x, w)
+        assert all(torch.equal(ops.linear(x, w), first) for _ in range(5))
+
+
+# ---- together, and as programs use them ------------------------------------------------------------------------------
+
+def layer(ops, state, x, residual):
+    normed, residual = ops.rms_norm(x, state["norm"], 1e-5, residual=residual)
+    both = ops.linear(normed, state["gate_up"])
+    half = both.shape[-1] // 2
+    return ops.linear(ops.silu_mul(both[..., :half], both[..., half:]), state["down"], bias=state["bias"], residual=residual)
+
+
+def layer_state(ops, hidden=384, inner=1000):
+    weight = lambda n, k, seed: ops.quantize_rows(0.05 * randn(n, k, seed=seed, dtype=FP32))
+    return dict(norm=(1 + 0.1 * randn(hidden, seed=20, dtype=FP32)).to(BF16), gate_up=weight(2 * inner, hidden, 21),
+                down=weight(hidden, inner, 22), bias=randn(hidden, seed=23))
+
+
+@pytest.mark.parametrize("tokens", (1, 19, 300))
+def test_a_feed_forward_block(ops, tokens):
+    """Norm, gate and up, gated activation, down with bias and residual in one run: every stage is the exact function (float64) of
+    what the stage before it gave, within that stage's own roundings, and the run's result has the last stage's bits."""
+    state = layer_state(ops)
+    x, residual = randn(tokens, 384, seed=24), randn(tokens, 384, seed=25)
+    got = layer(ops, state, x, residual)
+    normed, total = ops.rms_norm(x, state["norm"], 1e-5, residual=residual)
+    assert torch.equal(total, (x.float() + residual.float()).to(BF16))
+    h = total.double()
+    check_codes(normed, h / (h.square().mean(1, keepdim=True) + 1e-5).sqrt() * state["norm"].double(), slack=32 * U)
+    both = check_linear(ops, normed, state["gate_up"])
+    g, u = both[:, :1000].double(), both[:, 1000:].double()
+    gated = ops.silu_mul(both[:, :1000], both[:, 1000:])
+    check_codes(gated, g * torch.sigmoid(g) * u, (5 + 1.173 * float(g.abs().max())) * 2 * U)
+    check_linear(ops, gated, state["down"], bias=state["bias"], residual=total, got=got)
+
+
+def test_captured_replayed_and_on_other_streams(ops):
+    """Two graphs of one block over inputs of their own, replayed in turn and at the same time on two streams."""
+    state = layer_state(ops)
+    xs = [randn(t, 384, seed=30 + t) for t in (1, 40, 300)]
+    rs = [randn(t, 384, seed=60 + t) for t in (1, 40, 300)]
+    wants = [layer(ops, state, x, r) for x, r in zip(xs, rs)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for x, r in zip(xs, rs):
+            layer(ops, state, x, r)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for x, r in zip(xs, rs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(layer(ops, state, x, r))
+        graphs.append(graph)
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        for i, graph in enumerate(graphs):
+            with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+                graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(o, w) for o, w in zip(outs, wants))
+    xs[1].copy_(xs[1].flip(0)), rs[1].copy_(rs[1].flip(0))
+    graphs[1].replay()
+    assert torch.equal(outs[1], wants[1].flip(0))
+    ops.module.check_device_error()
+
+
+def test_refusals_on_the_gpu(ops):
+    x, w = codes_rows(4, 64, 40), codes_rows(32, 64, 41)
+    y = randn(4, 64, seed=42)
+    with pytest.raises(RuntimeError, match="codes"):
+        ops.linear(x, codes_rows(32, 80, 41))
+    with pytest.raises(RuntimeError, match="16-byte"):
+        ops.module.int8_linear(x.codes[:, 1:], x.scales, w.codes[:, 1:], w.scales, torch.empty(4, 32, dtype=BF16, device="cuda"))
+    with pytest.raises(RuntimeError, match="bias"):
+        ops.linear(x, w, bias=torch.zeros(32, device="cuda"))
+    with pytest.raises(RuntimeError, match="bias"):
+        ops.linear(x, w, bias=torch.zeros(31, dtype=BF16, device="cuda"))
+    with pytest.raises(RuntimeError, match="residual"):
+        ops.linear(x, w, residual=torch.zeros(4, 33, dtype=BF16, device="cuda"))
+    with pytest.raises(RuntimeError, match="contiguous features"):
+        ops.quantize_rows(y.T)
+    with pytest.raises(RuntimeError, match="one shape"):
+        ops.silu_mul(y, y[:3])
+    with pytest.raises(RuntimeError, match="weight"):
+        ops.rms_norm(y, torch.ones(63, dtype=BF16, device="cuda"), 1e-5)
+    with pytest.raises(RuntimeError, match="eps"):
+        ops.rms_norm(y, torch.ones(64, dtype=BF16, device="cuda"), -1.0)
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.quantize_rows(y.clone().requires_grad_())
+    with torch.no_grad():
+        ops.quantize_rows(y.clone().requires_grad_())

@@ -18,7 +18,8 @@ from pathlib import Path
 ROOT = Path(__file__).resolve().parent
 CSRC = ROOT / "csrc"
 LIBRARY = ROOT / "libtriattn_sm100a.so"
-SOURCES = ("abi.cu", "kv_write.cu", "decode.cu", "prefill.cu", "tasks.cu")
+SOURCES = ("abi.cu", "kv_write.cu", "decode.cu", "prefill.cu", "tasks.cu", "rows.cu", "linear.cu")
+IEEE = ("rows.cu",)     # compiled without --use_fast_math: their codes are those of IEEE fp32 arithmetic
 FLAGS = ("-O3", "-std=c++17", "--use_fast_math", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
          "-Xcompiler", "-fPIC")
 
@@ -36,7 +37,7 @@ def _digest() -> str:
         if path.suffix in (".cu", ".cuh", ".h"):
             h.update(path.name.encode())
             h.update(path.read_bytes())
-    h.update(" ".join(FLAGS).encode())
+    h.update(" ".join(FLAGS + SOURCES + IEEE).encode())
     return h.hexdigest()[:16]
 
 
@@ -51,7 +52,8 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     objects, procs = [], []
     for name in SOURCES:
         obj = obj_dir / (Path(name).stem + ".o")
-        cmd = [nvcc(), *FLAGS, "-I", str(CSRC), "-c", str(CSRC / name), "-o", str(obj)]
+        flags = [f for f in FLAGS if f != "--use_fast_math"] if name in IEEE else FLAGS
+        cmd = [nvcc(), *flags, "-I", str(CSRC), "-c", str(CSRC / name), "-o", str(obj)]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         procs.append((name, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

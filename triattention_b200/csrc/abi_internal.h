@@ -9,6 +9,10 @@
 
 enum TriStatus : int { TRI_OK = 0, TRI_ERR_ARGUMENT = -1, TRI_ERR_CUDA = -2, TRI_ERR_DEVICE = -3 };
 
+// Element types of the row and projection entry points, and the widest row of codes (128 * 128 * width < 2^31).
+enum TriType : int { TRI_BF16 = 0, TRI_FP16 = 1, TRI_FP32 = 2 };
+constexpr int TRI_MAX_WIDTH = 131071;
+
 void tri_set_error(const char* what);
 int tri_launch_status(const char* where);
 

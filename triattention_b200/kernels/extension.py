@@ -46,11 +46,18 @@ SIGNATURES = {
     "tri_decode_occupancy": [],
     "tri_decode_tail_hint": [_I],
     "tri_qk_accumulators": [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
+    "tri_quantize_rows": [_P, _I, _L, _I, _L, _P, _L, _P, _P],
+    "tri_silu_mul_rows": [_P, _P, _I, _L, _I, _L, _L, _P, _L, _P, _P],
+    "tri_rms_norm_rows": [_P, _P, _P, _I, _L, _I, _L, _L, _D, _P, _L, _P, _L, _P, _P],
+    "tri_dequantize_rows": [_P, _L, _P, _I, _L, _I, _P, _L, _P],
+    "tri_int8_linear": [_P, _L, _P, _P, _L, _P, _P, _P, _L, _P, _L, _I, _L, _I, _I, _P, _P],
     "tri_abi_version": [],
 }
 
 
 ABI_VERSION = 5         # tri_abi_version() of the library these signatures describe
+ROW_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}    # TRI_BF16, TRI_FP16, TRI_FP32
+MAX_WIDTH = 131071      # widest row of INT8 codes: 128 * 128 * width stays below 2^31
 LONG_TAIL_ROWS = 8      # tri_decode_tail_hint: above this many rows (or without a hint) the unrolled merge kernel runs
 
 
@@ -61,7 +68,9 @@ def load_library() -> ctypes.CDLL:
                            "(there is no CPU or PyTorch fallback)")
     lib = ctypes.CDLL(str(LIBRARY))
     for name, argtypes in SIGNATURES.items():
-        fn = getattr(lib, name)
+        fn = getattr(lib, name, None)
+        if fn is None:      # built before this entry point was added
+            raise RuntimeError(f"{LIBRARY.name} has no {name}: rebuild it with `python -m triattention_b200.build`")
         fn.argtypes, fn.restype = argtypes, ctypes.c_int
     lib.tri_last_error.argtypes, lib.tri_last_error.restype = [], ctypes.c_char_p
     if lib.tri_abi_version() != ABI_VERSION:     # a library built from older sources takes other arguments
@@ -432,6 +441,91 @@ class Module:
 
     def decode_occupancy(self):
         return self._check(self.lib.tri_decode_occupancy())
+
+    # -- INT8 projections ------------------------------------------------------------------------
+    @staticmethod
+    def _rows(x, name, dtype=None, like=None):
+        """2-D rows on a GPU with contiguous features; `like`: a tensor whose shape and device they have."""
+        if not (x.is_cuda and x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1) and
+                (x.dtype in ROW_TYPES if dtype is None else x.dtype == dtype)):
+            raise RuntimeError(f"{name}: rows [T,H] of {dtype or 'bf16, fp16 or fp32'} on a GPU with contiguous features")
+        if like is not None and (x.shape != like.shape or x.device != like.device):
+            raise RuntimeError(f"{name}: shape and device of the other rows")
+        return x
+
+    def _code_rows(self, codes, scales, like, name="codes"):
+        self._rows(codes, name, torch.int8)
+        rows, width = codes.shape
+        if not (1 <= width <= MAX_WIDTH and codes.device == like.device and codes.data_ptr() % 16 == 0 and
+                (rows <= 1 or codes.stride(0) % 16 == 0)):
+            raise RuntimeError(f"{name}: rows [T,1..{MAX_WIDTH}] that start on 16-byte boundaries, on the device of the other tensors")
+        if not (scales.dtype == torch.float32 and scales.shape == (rows,) and scales.device == codes.device and scales.is_contiguous()):
+            raise RuntimeError(f"{name}: float32 scales [{rows}], one a row")
+        return -(-width // 16) * 16 if rows <= 1 else codes.stride(0)
+
+    def quantize_rows(self, x, codes, scales):
+        """codes [T,H] and scales [T] of the rows x [T,H]."""
+        self._rows(x, "x"), self._rows(codes, "codes", torch.int8, like=x)
+        pitch = self._code_rows(codes, scales, x)
+        with torch.cuda.device(x.device):
+            self._check(self.lib.tri_quantize_rows(x.data_ptr(), ROW_TYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0),
+                                                   codes.data_ptr(), pitch, scales.data_ptr(), _stream()))
+
+    def silu_mul_rows(self, gate, up, codes, scales):
+        """codes and scales of silu(gate) * up."""
+        self._rows(gate, "gate"), self._rows(up, "up", gate.dtype, like=gate), self._rows(codes, "codes", torch.int8, like=gate)
+        pitch = self._code_rows(codes, scales, gate)
+        with torch.cuda.device(gate.device):
+            self._check(self.lib.tri_silu_mul_rows(gate.data_ptr(), up.data_ptr(), ROW_TYPES[gate.dtype], gate.shape[0],
+                                                   gate.shape[1], gate.stride(0), up.stride(0), codes.data_ptr(), pitch,
+                                                   scales.data_ptr(), _stream()))
+
+    def rms_norm_rows(self, x, weight, eps, codes, scales, residual=None, residual_out=None):
+        """codes and scales of the normed rows of h = x (+ residual, whose rounded sum goes to residual_out)."""
+        self._rows(x, "x"), self._rows(codes, "codes", torch.int8, like=x)
+        pitch = self._code_rows(codes, scales, x)
+        if not (weight.dtype == x.dtype and weight.shape == x.shape[1:] and weight.device == x.device and weight.is_contiguous()):
+            raise RuntimeError("norm weight [H] of the type and on the device of x")
+        if (residual is None) != (residual_out is None):
+            raise RuntimeError("the residual and where its sum goes (both or none)")
+        strides = (0, 0)
+        if residual is not None:
+            self._rows(residual, "residual", x.dtype, like=x), self._rows(residual_out, "residual_out", x.dtype, like=x)
+            strides = residual.stride(0), residual_out.stride(0) if x.shape[0] > 1 else x.shape[1]
+        with torch.cuda.device(x.device):
+            self._check(self.lib.tri_rms_norm_rows(x.data_ptr(), _ptr(residual), weight.data_ptr(), ROW_TYPES[x.dtype], x.shape[0],
+                                                   x.shape[1], x.stride(0), strides[0], float(eps), _ptr(residual_out), strides[1],
+                                                   codes.data_ptr(), pitch, scales.data_ptr(), _stream()))
+
+    def dequantize_rows(self, codes, scales, out):
+        """out [T,H] = scale * code, rounded to out's type."""
+        self._rows(out, "out"), self._rows(codes, "codes", torch.int8, like=out)
+        pitch = self._code_rows(codes, scales, out)
+        with torch.cuda.device(out.device):
+            self._check(self.lib.tri_dequantize_rows(codes.data_ptr(), pitch, scales.data_ptr(), ROW_TYPES[out.dtype], out.shape[0],
+                                                     out.shape[1], out.data_ptr(), out.stride(0) if out.shape[0] > 1 else out.shape[1],
+                                                     _stream()))
+        return out
+
+    def int8_linear(self, codes, scales, weight, weight_scales, out, bias=None, residual=None):
+        """out [T,N] = (codes [T,K] . weight [N,K]^T) * weight_scales[n] * scales[t] + bias[n] + residual[t,n]."""
+        self._rows(out, "out")
+        pitch, weight_pitch = self._code_rows(codes, scales, out), self._code_rows(weight, weight_scales, out, "weight")
+        tokens, outputs = out.shape
+        if codes.shape[0] != tokens or weight.shape != (outputs, codes.shape[1]) or outputs < 1:
+            raise RuntimeError("codes [T,K], weight [N,K], out [T,N]")
+        if bias is not None and not (bias.dtype == out.dtype and bias.shape == (outputs,) and bias.device == out.device and
+                                     bias.is_contiguous()):
+            raise RuntimeError("bias [N] of the output's type, on its device")
+        if residual is not None:
+            self._rows(residual, "residual", out.dtype, like=out)
+        with torch.cuda.device(out.device):
+            self._check(self.lib.tri_int8_linear(codes.data_ptr(), pitch, scales.data_ptr(), weight.data_ptr(), weight_pitch,
+                                                 weight_scales.data_ptr(), _ptr(bias), _ptr(residual),
+                                                 0 if residual is None else residual.stride(0), out.data_ptr(),
+                                                 out.stride(0) if tokens > 1 else outputs, ROW_TYPES[out.dtype], tokens, outputs,
+                                                 codes.shape[1], self.error_word(out.device).data_ptr(), _stream()))
+        return out
 
     # -- parity helpers --------------------------------------------------------------------------
     def qk_accumulators(self, requests, q8, q4x, k8, k4x, batch, heads_q, heads_kv, tokens):
