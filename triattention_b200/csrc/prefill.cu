@@ -146,22 +146,6 @@ __global__ void __launch_bounds__(ProbeThreads) qk_accum_kernel(const __grid_con
 }
 
 // ---- host side ----------------------------------------------------------------------------------
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_fn() {
-  static EncodeTiled fn = nullptr;
-  if (fn == nullptr) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiled>(p);
-  }
-  return fn;
-}
-
 // int8 rows [units][tokens][128]: box = 128 rows x 128 bytes of one unit, 128-byte swizzle, rows past
 // `tokens` are filled with zeros by the copy engine.
 static int make_q_map(CUtensorMap* map, const void* base, int tokens, int units) {
