@@ -443,89 +443,115 @@ class Module:
         return self._check(self.lib.tri_decode_occupancy())
 
     # -- INT8 projections ------------------------------------------------------------------------
-    @staticmethod
-    def _rows(x, name, dtype=None, like=None):
-        """2-D rows on a GPU with contiguous features; `like`: a tensor whose shape and device they have."""
-        if not (x.is_cuda and x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1) and
-                (x.dtype in ROW_TYPES if dtype is None else x.dtype == dtype)):
-            raise RuntimeError(f"{name}: rows [T,H] of {dtype or 'bf16, fp16 or fp32'} on a GPU with contiguous features")
-        if like is not None and (x.shape != like.shape or x.device != like.device):
-            raise RuntimeError(f"{name}: shape and device of the other rows")
-        return x
+    # (These calls are short against the host's own time per call, so the checks are few and flat.)
+    def _launch(self, fn, index, *args):
+        """fn(*args, stream) on the current stream of GPU `index`."""
+        if index == torch.cuda.current_device():
+            return self._check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+        with torch.cuda.device(index):
+            return self._check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
-    def _code_rows(self, codes, scales, like, name="codes"):
-        self._rows(codes, name, torch.int8)
+    @staticmethod
+    def _rows(x, name):
+        """(type, GPU) of rows [T,H] with contiguous features."""
+        kind, index = ROW_TYPES.get(x.dtype), x.get_device()
+        if kind is None or index < 0 or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] != 1):
+            raise RuntimeError(f"{name}: rows [T,H] of bf16, fp16 or fp32 on a GPU with contiguous features")
+        return kind, index
+
+    @staticmethod
+    def _like(x, other, name):
+        """Rows of the shape, type and GPU of `other`."""
+        if (x.shape != other.shape or x.dtype != other.dtype or x.get_device() != other.get_device() or
+                (x.stride(1) != 1 and x.shape[1] != 1)):
+            raise RuntimeError(f"{name}: shape, type and device of the other rows, with contiguous features")
+
+    @staticmethod
+    def _code_rows(codes, scales, index, name="codes"):
+        """Bytes between the rows of codes int8 [T,H] with scales f32 [T] on GPU `index`."""
+        if codes.dtype != torch.int8 or codes.dim() != 2 or codes.get_device() != index or index < 0:
+            raise RuntimeError(f"{name}: int8 rows [T,H] on a GPU, the one of the other tensors")
         rows, width = codes.shape
-        if not (1 <= width <= MAX_WIDTH and codes.device == like.device and codes.data_ptr() % 16 == 0 and
-                (rows <= 1 or codes.stride(0) % 16 == 0)):
-            raise RuntimeError(f"{name}: rows [T,1..{MAX_WIDTH}] that start on 16-byte boundaries, on the device of the other tensors")
-        if not (scales.dtype == torch.float32 and scales.shape == (rows,) and scales.device == codes.device and scales.is_contiguous()):
-            raise RuntimeError(f"{name}: float32 scales [{rows}], one a row")
-        return -(-width // 16) * 16 if rows <= 1 else codes.stride(0)
+        pitch = codes.stride(0) if rows > 1 else -(-width // 16) * 16
+        if not 1 <= width <= MAX_WIDTH or codes.data_ptr() % 16 or pitch % 16 or (codes.stride(1) != 1 and width != 1):
+            raise RuntimeError(f"{name}: rows [T,1..{MAX_WIDTH}] that start on 16-byte boundaries, contiguous features")
+        if scales.dtype != torch.float32 or scales.shape != (rows,) or scales.get_device() != index or not scales.is_contiguous():
+            raise RuntimeError(f"{name}: float32 scales [{rows}], one a row, on the same GPU")
+        return pitch
 
     def quantize_rows(self, x, codes, scales):
         """codes [T,H] and scales [T] of the rows x [T,H]."""
-        self._rows(x, "x"), self._rows(codes, "codes", torch.int8, like=x)
-        pitch = self._code_rows(codes, scales, x)
-        with torch.cuda.device(x.device):
-            self._check(self.lib.tri_quantize_rows(x.data_ptr(), ROW_TYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0),
-                                                   codes.data_ptr(), pitch, scales.data_ptr(), _stream()))
+        kind, index = self._rows(x, "x")
+        pitch = self._code_rows(codes, scales, index)
+        if codes.shape != x.shape:
+            raise RuntimeError("codes have the shape of x")
+        self._launch(self.lib.tri_quantize_rows, index, x.data_ptr(), kind, *x.shape, x.stride(0), codes.data_ptr(), pitch,
+                     scales.data_ptr())
 
     def silu_mul_rows(self, gate, up, codes, scales):
         """codes and scales of silu(gate) * up."""
-        self._rows(gate, "gate"), self._rows(up, "up", gate.dtype, like=gate), self._rows(codes, "codes", torch.int8, like=gate)
-        pitch = self._code_rows(codes, scales, gate)
-        with torch.cuda.device(gate.device):
-            self._check(self.lib.tri_silu_mul_rows(gate.data_ptr(), up.data_ptr(), ROW_TYPES[gate.dtype], gate.shape[0],
-                                                   gate.shape[1], gate.stride(0), up.stride(0), codes.data_ptr(), pitch,
-                                                   scales.data_ptr(), _stream()))
+        kind, index = self._rows(gate, "gate")
+        self._like(up, gate, "up")
+        pitch = self._code_rows(codes, scales, index)
+        if codes.shape != gate.shape:
+            raise RuntimeError("codes have the shape of gate and up")
+        self._launch(self.lib.tri_silu_mul_rows, index, gate.data_ptr(), up.data_ptr(), kind, *gate.shape, gate.stride(0),
+                     up.stride(0), codes.data_ptr(), pitch, scales.data_ptr())
 
     def rms_norm_rows(self, x, weight, eps, codes, scales, residual=None, residual_out=None):
         """codes and scales of the normed rows of h = x (+ residual, whose rounded sum goes to residual_out)."""
-        self._rows(x, "x"), self._rows(codes, "codes", torch.int8, like=x)
-        pitch = self._code_rows(codes, scales, x)
-        if not (weight.dtype == x.dtype and weight.shape == x.shape[1:] and weight.device == x.device and weight.is_contiguous()):
+        kind, index = self._rows(x, "x")
+        pitch = self._code_rows(codes, scales, index)
+        rows, width = x.shape
+        if codes.shape != x.shape:
+            raise RuntimeError("codes have the shape of x")
+        if weight.dtype != x.dtype or weight.shape != (width,) or weight.get_device() != index or (weight.stride(0) != 1 and width != 1):
             raise RuntimeError("norm weight [H] of the type and on the device of x")
-        if (residual is None) != (residual_out is None):
+        if residual is None and residual_out is None:
+            self._launch(self.lib.tri_rms_norm_rows, index, x.data_ptr(), None, weight.data_ptr(), kind, rows, width, x.stride(0), 0,
+                         eps, None, 0, codes.data_ptr(), pitch, scales.data_ptr())
+            return
+        if residual is None or residual_out is None:
             raise RuntimeError("the residual and where its sum goes (both or none)")
-        strides = (0, 0)
-        if residual is not None:
-            self._rows(residual, "residual", x.dtype, like=x), self._rows(residual_out, "residual_out", x.dtype, like=x)
-            strides = residual.stride(0), residual_out.stride(0) if x.shape[0] > 1 else x.shape[1]
-        with torch.cuda.device(x.device):
-            self._check(self.lib.tri_rms_norm_rows(x.data_ptr(), _ptr(residual), weight.data_ptr(), ROW_TYPES[x.dtype], x.shape[0],
-                                                   x.shape[1], x.stride(0), strides[0], float(eps), _ptr(residual_out), strides[1],
-                                                   codes.data_ptr(), pitch, scales.data_ptr(), _stream()))
+        self._like(residual, x, "residual"), self._like(residual_out, x, "residual_out")
+        self._launch(self.lib.tri_rms_norm_rows, index, x.data_ptr(), residual.data_ptr(), weight.data_ptr(), kind, rows, width,
+                     x.stride(0), residual.stride(0), eps, residual_out.data_ptr(), residual_out.stride(0) if rows > 1 else width,
+                     codes.data_ptr(), pitch, scales.data_ptr())
 
     def dequantize_rows(self, codes, scales, out):
         """out [T,H] = scale * code, rounded to out's type."""
-        self._rows(out, "out"), self._rows(codes, "codes", torch.int8, like=out)
-        pitch = self._code_rows(codes, scales, out)
-        with torch.cuda.device(out.device):
-            self._check(self.lib.tri_dequantize_rows(codes.data_ptr(), pitch, scales.data_ptr(), ROW_TYPES[out.dtype], out.shape[0],
-                                                     out.shape[1], out.data_ptr(), out.stride(0) if out.shape[0] > 1 else out.shape[1],
-                                                     _stream()))
+        kind, index = self._rows(out, "out")
+        pitch = self._code_rows(codes, scales, index)
+        rows, width = out.shape
+        if codes.shape != out.shape:
+            raise RuntimeError("codes have the shape of out")
+        self._launch(self.lib.tri_dequantize_rows, index, codes.data_ptr(), pitch, scales.data_ptr(), kind, rows, width,
+                     out.data_ptr(), out.stride(0) if rows > 1 else width)
         return out
 
     def int8_linear(self, codes, scales, weight, weight_scales, out, bias=None, residual=None):
         """out [T,N] = (codes [T,K] . weight [N,K]^T) * weight_scales[n] * scales[t] + bias[n] + residual[t,n]."""
-        self._rows(out, "out")
-        pitch, weight_pitch = self._code_rows(codes, scales, out), self._code_rows(weight, weight_scales, out, "weight")
+        kind, index = self._rows(out, "out")
+        pitch, weight_pitch = self._code_rows(codes, scales, index), self._code_rows(weight, weight_scales, index, "weight")
         tokens, outputs = out.shape
-        if codes.shape[0] != tokens or weight.shape != (outputs, codes.shape[1]) or outputs < 1:
+        width = codes.shape[1]
+        if codes.shape[0] != tokens or weight.shape != (outputs, width) or outputs < 1:
             raise RuntimeError("codes [T,K], weight [N,K], out [T,N]")
-        if bias is not None and not (bias.dtype == out.dtype and bias.shape == (outputs,) and bias.device == out.device and
-                                     bias.is_contiguous()):
+        if bias is not None and (bias.dtype != out.dtype or bias.shape != (outputs,) or bias.get_device() != index or
+                                 (bias.stride(0) != 1 and outputs != 1)):
             raise RuntimeError("bias [N] of the output's type, on its device")
+        residual_stride = 0
         if residual is not None:
-            self._rows(residual, "residual", out.dtype, like=out)
-        with torch.cuda.device(out.device):
-            self._check(self.lib.tri_int8_linear(codes.data_ptr(), pitch, scales.data_ptr(), weight.data_ptr(), weight_pitch,
-                                                 weight_scales.data_ptr(), _ptr(bias), _ptr(residual),
-                                                 0 if residual is None else residual.stride(0), out.data_ptr(),
-                                                 out.stride(0) if tokens > 1 else outputs, ROW_TYPES[out.dtype], tokens, outputs,
-                                                 codes.shape[1], self.error_word(out.device).data_ptr(), _stream()))
+            self._like(residual, out, "residual")
+            residual_stride = residual.stride(0)
+        self._launch(self.lib.tri_int8_linear, index, codes.data_ptr(), pitch, scales.data_ptr(), weight.data_ptr(), weight_pitch,
+                     weight_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                     None if residual is None else residual.data_ptr(), residual_stride, out.data_ptr(),
+                     out.stride(0) if tokens > 1 else outputs, kind, tokens, outputs, width, self._error_pointer(index))
         return out
+
+    def _error_pointer(self, index):
+        return (self._errors[index] if index in self._errors else self.error_word(index)).data_ptr()
 
     # -- parity helpers --------------------------------------------------------------------------
     def qk_accumulators(self, requests, q8, q4x, k8, k4x, batch, heads_q, heads_kv, tokens):

@@ -29,6 +29,18 @@ class Int8Rows:
             raise RuntimeError("Int8Rows: int8 codes [..., H] and float32 scales [...]")
         self.codes, self.scales, self.dtype = codes, scales, dtype
 
+    @classmethod
+    def _of(cls, codes, scales, dtype):
+        self = cls.__new__(cls)     # made by a call of this file: nothing to check
+        self.codes, self.scales, self.dtype = codes, scales, dtype
+        return self
+
+    def _flat(self):
+        """codes [T, H] and scales [T]."""
+        if self.codes.dim() == 2:
+            return self.codes, self.scales
+        return self.codes.reshape(-1, self.codes.shape[-1]), self.scales.reshape(-1)
+
     @property
     def shape(self):
         return self.codes.shape
@@ -53,12 +65,15 @@ class Int8Ops:
 
     @staticmethod
     def _inference(*tensors):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-            raise RuntimeError("the INT8 projections have no backward pass: call them under torch.no_grad() or inference_mode()")
+        if torch.is_grad_enabled():
+            for t in tensors:
+                if t is not None and t.requires_grad:
+                    raise RuntimeError("the INT8 projections have no backward pass: call them under torch.no_grad() or "
+                                       "inference_mode()")
 
     @staticmethod
     def _empty_codes(x):
-        """Uninitialised codes [T, H], rows a multiple of 16 bytes apart, and scales [T]."""
+        """Uninitialised codes [T,H], rows a multiple of 16 bytes apart, and scales [T], for the rows x [T,H]."""
         rows, width = x.shape
         if not 1 <= width <= MAX_WIDTH:
             raise RuntimeError(f"rows of 1..{MAX_WIDTH} features")
@@ -70,7 +85,7 @@ class Int8Ops:
     def _shaped(codes, scales, like):
         if like.dim() != 2:
             codes, scales = codes.view(like.shape), scales.view(like.shape[:-1])
-        return Int8Rows(codes, scales, like.dtype)
+        return Int8Rows._of(codes, scales, like.dtype)
 
     def quantize_rows(self, x):
         """x [..., H] (bf16, fp16 or fp32) -> Int8Rows."""
@@ -94,32 +109,37 @@ class Int8Ops:
         """h = x + residual (rounded to x's type); h / sqrt(mean h^2 + eps) * weight -> Int8Rows, or (Int8Rows, h) with a
         residual."""
         self._inference(x, weight, residual)
-        if residual is not None and residual.shape != x.shape:
-            raise RuntimeError("x and residual have one shape")
         flat = _flat(x)
-        codes, scales = self._empty_codes(flat)
         if residual is None:
+            codes, scales = self._empty_codes(flat)
             self.module.rms_norm_rows(flat, weight, eps, codes, scales)
             return self._shaped(codes, scales, x)
-        total = torch.empty(flat.shape, dtype=x.dtype, device=x.device)
+        if residual.shape != x.shape:
+            raise RuntimeError("x and residual have one shape")
+        codes, scales = self._empty_codes(flat)
+        total = flat.new_empty(flat.shape)
         self.module.rms_norm_rows(flat, weight, eps, codes, scales, _flat(residual), total)
-        return self._shaped(codes, scales, x), total.view(x.shape)
+        return self._shaped(codes, scales, x), total if x.dim() == 2 else total.view(x.shape)
 
     def dequantize(self, rows, dtype=None):
         """The values that rows of codes stand for, in `dtype` (default: the type they were made from)."""
-        flat = _flat(rows.codes)
-        out = torch.empty(flat.shape, dtype=dtype or rows.dtype, device=flat.device)
-        return self.module.dequantize_rows(flat, rows.scales.reshape(-1), out).view(rows.shape)
+        codes, scales = rows._flat()
+        out = torch.empty(codes.shape, dtype=dtype or rows.dtype, device=codes.device)
+        self.module.dequantize_rows(codes, scales, out)
+        return out if rows.codes.dim() == 2 else out.view(rows.shape)
 
     def linear(self, rows, weight, bias=None, residual=None, dtype=None):
         """rows [..., K] . weight [N, K]^T (both Int8Rows) + bias [N] + residual [..., N], in `dtype` (default: the type the
         rows were made from; bias and residual have it too)."""
         self._inference(bias, residual)
-        shape = rows.shape[:-1] + weight.shape[:1]
-        if residual is not None and residual.shape != shape:
-            raise RuntimeError("residual [..., N]")
-        codes = _flat(rows.codes)
-        out = torch.empty((codes.shape[0], weight.shape[0]), dtype=dtype or rows.dtype, device=codes.device)
-        self.module.int8_linear(codes, rows.scales.reshape(-1), weight.codes, weight.scales, out, bias,
-                                None if residual is None else _flat(residual))
-        return out if len(shape) == 2 else out.view(shape)
+        codes, scales = rows._flat()
+        if codes.dim() != 2 or weight.codes.dim() != 2:
+            raise RuntimeError("rows [..., K] and weight [N, K]")
+        flat = rows.codes.dim() == 2
+        out = torch.empty((codes.shape[0], weight.codes.shape[0]), dtype=dtype or rows.dtype, device=codes.device)
+        if residual is not None and not flat:
+            if residual.shape != rows.shape[:-1] + out.shape[1:]:
+                raise RuntimeError("residual [..., N]")
+            residual = _flat(residual)
+        self.module.int8_linear(codes, scales, weight.codes, weight.scales, out, bias, residual)
+        return out if flat else out.view(rows.shape[:-1] + out.shape[1:])
