@@ -140,7 +140,10 @@ def test_rows_strided_offset_and_shaped(ops):
         assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
         w = wide[0, 3 + off:1003 + off]
         (got, total), (want, sums) = ops.rms_norm(x, w, 1e-6, residual=up), ops.rms_norm(x.contiguous(), w.clone(), 1e-6, residual=up.contiguous())
-        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales) and torch.equal(total, sums)
+        # Codes do not depend on the sum of squares; scales do, and rows that lie differently are summed in another order: at most
+        # 32 terms in turn and a tree of 10 (42 half steps) on each side, halved by the root, and four roundings after it.
+        assert torch.equal(got.codes, want.codes) and torch.equal(total, sums)
+        torch.testing.assert_close(got.scales, want.scales, rtol=46 * U, atol=0)
     one = randn(1, 96, seed=10)
     many = ops.quantize_rows(one.expand(5, 96))
     assert torch.equal(many.codes, ops.quantize_rows(one).codes.expand(5, 96))
