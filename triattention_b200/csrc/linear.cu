@@ -9,17 +9,18 @@
 // 32 neighbouring channels of one token, which needs no alignment of the output rows.
 //   warp 0      producer: TMA copies of the weights' and tokens' 128-byte columns (128-byte swizzle, edges zero-filled)
 //   warp 1      issues the MMAs (one elected thread), accumulators alternate between two TMEM buffers
-//   warps 2-5   epilogue: TMEM -> scales, bias, residual -> global, while the next tile's MMAs run
+//   warps 2-9   epilogue: TMEM -> scales, bias, residual -> global, while the next tile's MMAs run
 // A CTA takes tiles in turn (persistent).  Where there are fewer tiles than SMs the width is split over a cluster of 2, 4 or 8
 // CTAs; their integer partial sums are joined through distributed shared memory, so no workspace and no atomics are involved.
 // Every wait on a barrier is bounded; after one has run out the CTA runs through, reports it and its output is void.
 #include "tcgen05.cuh"
 #include "abi_internal.h"
+#include <cstdlib>
 
 namespace tri {
 
-constexpr int LinChannels = 128, LinDepth = 128;             // channels of a tile; bytes of width per stage
-constexpr int LinThreads = 192, LinEpilogue = 128;
+constexpr int LinChannels = 128, LinDepth = 128;             // channels of a CTA's tile; bytes of width per stage
+constexpr int LinEpilogueWarps = 8, LinThreads = 64 + 32 * LinEpilogueWarps;
 constexpr int LinWeightBytes = LinChannels * LinDepth;
 constexpr int LinShared = 216 * 1024;                        // stages (and, after a split tile, its partial sums); also keeps
                                                              // a second CTA that allocates TMEM off the SM
@@ -33,6 +34,8 @@ struct LinearArgs {
   int tokens, outputs, width;
   int token_tile, stages, columns;                           // columns: TMEM columns allocated
   int channel_tiles, tiles, group;                           // group: token tiles that share a sweep over the channels
+  int splits;                                                // CTAs of a cluster that share a tile's width
+  int shared;                                                // dynamic shared memory
   int* error;
 };
 
@@ -50,175 +53,411 @@ __device__ __forceinline__ void lin_arrive(uint64_t* bar) {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int cluster_load(uint32_t address, uint32_t rank) {   // the word at `address` of the cluster's CTA `rank`
-  int v;
-  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.s32 %0, [a];\n\t}"
-               : "=r"(v) : "r"(address), "r"(rank) : "memory");
+__device__ __forceinline__ int4 cluster_load(uint32_t address, uint32_t rank) {   // 16 bytes at `address` of the cluster's CTA `rank`
+  int4 v;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [a];\n\t}"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address), "r"(rank) : "memory");
   return v;
+}
+
+// The same operations as in common.cuh on 32-bit shared-memory addresses.
+__device__ __forceinline__ bool lin_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool lin_wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  const uint64_t t0 = globaltimer_ns();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (lin_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > 2000000000ull) { *abort_flag = 1; return false; }
+  }
+}
+__device__ __forceinline__ bool lin_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (lin_try_wait(bar, parity)) return true;
+  return lin_wait_long(bar, parity, abort_flag);
+}
+__device__ __forceinline__ void lin_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void lin_copy(uint32_t to, const CUtensorMap* map, int column, int row, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(column), "r"(row), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void lin_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void lin_prefetch(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
+// The forms for a pair of CTAs.  Barrier addresses with the peer bit cleared name the even CTA's barrier at the same place.
+constexpr uint32_t PairEven = 0xfeffffffu;
+__device__ __forceinline__ void pair_alloc(uint32_t* slot, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_dealloc(uint32_t tmem, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void pair_copy(uint32_t to, const CUtensorMap* map, int column, int row, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(column), "r"(row), "r"(bar & PairEven) : "memory");
+}
+__device__ __forceinline__ void pair_umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pair_commit(uint32_t bar) {        // arrives at this barrier of both CTAs
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void pair_arrive(uint32_t bar) {        // arrives at the even CTA's barrier
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar) : "memory");
 }
 
 struct LinearBarriers {
   uint64_t full[LinMaxStages], empty[LinMaxStages], done[2], free[2];
 };
 
-// grid = CTAs (persistent) when cluster size is 1, otherwise tiles * cluster size with one tile per cluster.
-template <typename T> __global__ void __launch_bounds__(LinThreads, 1) linear_kernel(const __grid_constant__ CUtensorMap map_w,
-    const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearArgs p, int splits) {
+// tile -> first channel and first token: sweeps of `group` token tiles over all channels, so that the tiles that run at the
+// same time share both operands in L2.
+__device__ __forceinline__ void lin_origin(const LinearArgs& p, int tile, int channels, int& n0, int& t0) {
+  const int sweep = tile / (p.group * p.channel_tiles), within = tile % (p.group * p.channel_tiles);
+  const int token_tiles = p.tiles / p.channel_tiles, wide = min(p.group, token_tiles - sweep * p.group);
+  n0 = within / wide * channels;
+  t0 = (sweep * p.group + within % wide) * p.token_tile;
+}
+
+// Epilogue of one tile by the epilogue warps: 128 channels from n0 on (TMEM lanes), `valid` tokens from t0 on (columns).  Two warps
+// per lane quadrant take alternate blocks of 16 tokens.  `ready` is called once, when everything that does not depend on the
+// sums is under way.
+template <typename T, typename Ready>
+__device__ __forceinline__ void lin_epilogue(const LinearArgs& p, uint32_t column, int n0, int t0, int valid, float* token_scales, Ready ready) {
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, quad = warp % 4, half = (warp - 2) / 4;
+  const int out_n = n0 + quad * 32 + lane;
+  const bool live = out_n < p.outputs;
+  const int safe_n = live ? out_n : p.outputs - 1;            // what a lane past the last channel may read
+  column += (uint32_t)(quad * 32) << 16;
+  // the residual's block for the next 16 tokens is asked for while this one is worked on (the first one under the MMAs)
+  const T* residual = p.residual == nullptr ? nullptr : static_cast<const T*>(p.residual) + (int64_t)t0 * p.residual_stride + safe_n;
+  T ahead[16];
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) ahead[j] = residual[(int64_t)min(c + j, valid - 1) * p.residual_stride];
+  };
+  if (residual != nullptr) fetch(min(half * 16, valid - 1));
+  for (int t = tid - 64; t < valid; t += 32 * LinEpilogueWarps) token_scales[t] = p.scales[t0 + t];
+  const float sw = p.weight_scales[safe_n];
+  const float bias = p.bias != nullptr ? lin_in(static_cast<const T*>(p.bias)[safe_n]) : 0.f;
+  // token_scales of this tile are complete (and the other buffer's readers a tile behind); waits have no early exit, because
+  // the other epilogue warps count on this one at the barrier
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * LinEpilogueWarps) : "memory");
+  ready();
+  tc_fence_after();
+  T* out = static_cast<T*>(p.out) + (int64_t)t0 * p.out_stride + out_n;
+  for (int c = half * 16; c < valid; c += 32) {
+    uint32_t a[16];
+    tmem_ld16(column + c, a);
+    float y[16], r[16];
+    if (residual != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) r[j] = lin_in(ahead[j]);
+      if (c + 32 < valid) fetch(c + 32);
+    }
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      const float4 st = *reinterpret_cast<const float4*>(&token_scales[c + j]);
+      y[j] = __fmul_rn(__fmul_rn((float)(int)a[j], sw), st.x);
+      y[j + 1] = __fmul_rn(__fmul_rn((float)(int)a[j + 1], sw), st.y);
+      y[j + 2] = __fmul_rn(__fmul_rn((float)(int)a[j + 2], sw), st.z);
+      y[j + 3] = __fmul_rn(__fmul_rn((float)(int)a[j + 3], sw), st.w);
+    }
+    if (p.bias != nullptr)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j] += bias;
+    if (residual != nullptr)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j] += r[j];
+    T* to = out + (int64_t)c * p.out_stride;
+    if (c + 16 <= valid) {
+      if (live)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) to[j * p.out_stride] = lin_out<T>(y[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) if (live && c + j < valid) to[j * p.out_stride] = lin_out<T>(y[j]);
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+}
+
+// One CTA per tile of 128 channels.  grid = CTAs (persistent) when splits is 1, otherwise tiles * splits with one tile per cluster.
+template <typename T> __global__ void __launch_bounds__(LinThreads, 2) linear_kernel(const __grid_constant__ CUtensorMap map_w,
+    const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearArgs p) {
   extern __shared__ uint8_t raw_smem[];
   __shared__ __align__(8) LinearBarriers bars;
-  __shared__ float token_scales[2][256];
+  __shared__ __align__(16) float token_scales[2][256];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int bt = p.token_tile, stage_bytes = LinWeightBytes + bt * LinDepth;
+  const int bt = p.token_tile, stage_bytes = LinWeightBytes + bt * LinDepth, splits = p.splits;
   const int rank = blockIdx.x % splits, first = blockIdx.x / splits, step = gridDim.x / splits;
   const int all_steps = (p.width + LinDepth - 1) / LinDepth;
   const int k0 = (int)((int64_t)all_steps * rank / splits), k1 = (int)((int64_t)all_steps * (rank + 1) / splits);
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) { mbar_init(&bars.full[s], 1); mbar_init(&bars.empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&bars.done[b], 1); mbar_init(&bars.free[b], LinEpilogue / 32); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&bars.done[b], 1); mbar_init(&bars.free[b], LinEpilogueWarps); }
     mbar_fence_init();
     abort_flag = 0;
   }
+  if (tid == 32) { lin_prefetch(&map_w); lin_prefetch(&map_x); }
   if (warp == 0) { tmem_alloc(&tmem_slot, p.columns); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_launch_dependents();
+  grid_dependency_wait();            // the set-up above overlaps the tail of the kernel before this one in the stream
   volatile int* abortp = &abort_flag;
   const uint32_t tmem = tmem_slot, buffer = p.columns / 2;    // columns of an accumulator buffer
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_parked(bar, parity & 1u, abortp); };
-  // tile -> first channel and first token: sweeps of `group` token tiles over all channels, so that the tiles that run at the
-  // same time share both operands in L2
-  auto origin = [&](int tile, int& n0, int& t0) {
-    const int sweep = tile / (p.group * p.channel_tiles), within = tile % (p.group * p.channel_tiles);
-    const int token_tiles = p.tiles / p.channel_tiles, wide = min(p.group, token_tiles - sweep * p.group);
-    n0 = within / wide * LinChannels;
-    t0 = (sweep * p.group + within % wide) * bt;
-  };
-
+  // (The loops of the two issuing threads are serial code that the whole CTA waits for: shared-memory addresses as 32-bit numbers
+  // that only advance, no divisions.  With indexes and remainders a stage took 640 cycles, however little it held.)
+  const uint32_t smem_base = smem_u32(smem), full_base = smem_u32(&bars.full[0]), empty_base = smem_u32(&bars.empty[0]);
+  const int stages = p.stages;
   if (warp == 0) {
     if (lane == 0) {
-      int i = 0;                                              // stages filled so far
+      uint32_t at = smem_base, full = full_base, empty = empty_base, phase = 1;
+      int stage = 0, filled = 0;
       bool ok = true;
       for (int tile = first; ok && tile < p.tiles; tile += step) {
         int n0, t0;
-        origin(tile, n0, t0);
-        for (int k = k0; k < k1; ++k, ++i) {
-          const int s = i % p.stages, round = i / p.stages;
-          if (round > 0 && !(ok = wait(&bars.empty[s], round - 1))) break;
-          uint8_t* stage = smem + s * stage_bytes;
-          mbar_expect_tx(&bars.full[s], stage_bytes);
-          tma_load_2d(stage, &map_w, k * LinDepth, n0, &bars.full[s]);
-          tma_load_2d(stage + LinWeightBytes, &map_x, k * LinDepth, t0, &bars.full[s]);
+        lin_origin(p, tile, LinChannels, n0, t0);
+        for (int k = k0 * LinDepth; k < k1 * LinDepth; k += LinDepth) {
+          if (filled >= stages && !(ok = lin_wait(empty, phase, abortp))) break;
+          lin_expect(full, stage_bytes);
+          lin_copy(at, &map_w, k, n0, full);
+          lin_copy(at + LinWeightBytes, &map_x, k, t0, full);
+          ++filled;
+          at += stage_bytes; full += 8; empty += 8;
+          if (++stage == stages) { stage = 0; at = smem_base; full = full_base; empty = empty_base; phase ^= 1u; }
         }
       }
       if (*abortp)                                            // the copies in flight land before the CTA may leave
-        for (int j = max(0, i - p.stages); j < i; ++j) mbar_wait(&bars.full[j % p.stages], (j / p.stages) & 1u, 100000000ull);
+        for (int j = max(0, filled - stages); j < filled; ++j) mbar_wait(&bars.full[j % stages], (j / stages) & 1u, 100000000ull);
     }
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc = instr_desc(2, 1, 1, LinChannels, bt);
-      const uint32_t base = smem_u32(smem);
-      int i = 0, n = 0;
+      const uint64_t desc = smem_desc(smem_base, 0, 1024, Layout128B);
+      const uint32_t stage_units = stage_bytes >> 4;          // descriptors address 16-byte units; a stage's all lie below 2^14 of them
+      uint32_t full = full_base, empty = empty_base, phase = 0;
+      int stage = 0, n = 0;
+      uint64_t dw = desc;
       bool ok = true;
       for (int tile = first; ok && tile < p.tiles; tile += step, ++n) {
         const int b = n & 1;
-        if (n >= 2 && !(ok = wait(&bars.free[b], (n >> 1) - 1))) break;
+        if (n >= 2 && !(ok = lin_wait(smem_u32(&bars.free[b]), ((n >> 1) - 1) & 1, abortp))) break;
         tc_fence_after();
-        for (int k = k0; k < k1; ++k, ++i) {
-          const int s = i % p.stages;
-          if (!(ok = wait(&bars.full[s], i / p.stages))) break;
+        const uint32_t acc = tmem + b * buffer;
+        uint32_t accumulate = 0;
+        for (int k = k0; k < k1; ++k) {
+          if (!(ok = lin_wait(full, phase, abortp))) break;
           tc_fence_after();
-          const uint64_t dw = smem_desc(base + s * stage_bytes, 0, 1024, Layout128B);
-          const uint64_t dx = smem_desc(base + s * stage_bytes + LinWeightBytes, 0, 1024, Layout128B);
+          const uint64_t dx = dw + (LinWeightBytes >> 4);
+          umma_i8(acc, dw, dx, idesc, accumulate);            // 32 codes per MMA: 2 units of 16 bytes along the row
 #pragma unroll
-          for (int kk = 0; kk < LinDepth / 32; ++kk)          // 32 codes per MMA: 2 units of 16 bytes along the row
-            umma_i8(tmem + b * buffer, dw + 2 * kk, dx + 2 * kk, idesc, (k > k0 || kk > 0) ? 1u : 0u);
-          tc_commit(&bars.empty[s]);
+          for (int kk = 1; kk < LinDepth / 32; ++kk) umma_i8(acc, dw + 2 * kk, dx + 2 * kk, idesc, 1u);
+          lin_commit(empty);
+          accumulate = 1;
+          dw += stage_units; full += 8; empty += 8;
+          if (++stage == stages) { stage = 0; phase ^= 1u; dw = desc; full = full_base; empty = empty_base; }
         }
         tc_commit(&bars.done[b]);
       }
     }
-  } else {
-    const int quad = warp % 4, channel = quad * 32 + lane, et = tid - 64;
-    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+  } else if (splits == 1) {
     int n = 0;
     for (int tile = first; tile < p.tiles; tile += step, ++n) {
       const int b = n & 1;
       int n0, t0;
-      origin(tile, n0, t0);
-      const int valid = min(bt, p.tokens - t0), out_n = n0 + channel;
-      const bool live = out_n < p.outputs;
-      for (int t = et; t < valid; t += LinEpilogue) token_scales[b][t] = p.scales[t0 + t];
-      const float sw = live ? p.weight_scales[out_n] : 0.f;
-      const float bias = live && p.bias != nullptr ? lin_in(static_cast<const T*>(p.bias)[out_n]) : 0.f;
-      asm volatile("bar.sync 1, 128;" ::: "memory");          // token_scales of this tile; the other buffer's readers are a tile behind
-      wait(&bars.done[b], n >> 1);                            // (no early exit: the other epilogue warps count on this one's bar.sync)
-      tc_fence_after();
-      if (splits > 1) {                                       // one tile per cluster: this CTA's partial sums, [token][channel]
-        int* partial = reinterpret_cast<int*>(smem);
-        for (int c = 0; c < valid; c += 16) {
-          uint32_t a[16];
-          tmem_ld16(lanes + b * buffer + c, a);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) partial[(c + j) * LinChannels + channel] = (int)a[j];
-        }
-        break;
-      }
-      T* out = static_cast<T*>(p.out) + (int64_t)t0 * p.out_stride + out_n;
-      const T* residual = p.residual == nullptr ? nullptr : static_cast<const T*>(p.residual) + (int64_t)t0 * p.residual_stride + out_n;
-      for (int c = 0; c < valid; c += 16) {
-        uint32_t a[16];
-        tmem_ld16(lanes + b * buffer + c, a);
-        float r[16];
-        if (residual != nullptr)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = live && c + j < valid ? lin_in(residual[(c + j) * p.residual_stride]) : 0.f;
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float y = __fmul_rn(__fmul_rn((float)(int)a[j], sw), token_scales[b][c + j]);
-          if (p.bias != nullptr) y += bias;
-          if (residual != nullptr) y += r[j];
-          if (live && c + j < valid) out[(c + j) * p.out_stride] = lin_out<T>(y);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
+      lin_origin(p, tile, LinChannels, n0, t0);
+      lin_epilogue<T>(p, tmem + b * buffer, n0, t0, min(bt, p.tokens - t0), token_scales[b],
+                      [&] { lin_wait(smem_u32(&bars.done[b]), (n >> 1) & 1, abortp); });
       if (lane == 0) lin_arrive(&bars.free[b]);
+    }
+  } else {                                                    // one tile per cluster: this CTA's partial sums, [token][channel]
+    const int quad = warp % 4, half = (warp - 2) / 4, channel = quad * 32 + lane;
+    int n0, t0;
+    lin_origin(p, first, LinChannels, n0, t0);
+    const int valid = min(bt, p.tokens - t0);
+    lin_wait(smem_u32(&bars.done[0]), 0, abortp);
+    tc_fence_after();
+    int* partial = reinterpret_cast<int*>(smem);
+    for (int c = half * 16; c < valid; c += 32) {
+      uint32_t a[16];
+      tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + c, a);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) partial[(c + j) * LinChannels + channel] = (int)a[j];
     }
   }
   if (splits > 1) {
-    // every rank finishes its share of the tokens from all ranks' partial sums
+    // Every rank finishes its share of the tokens from all ranks' partial sums: a warp takes a token, a lane four channels.
+    int n0, t0;
+    lin_origin(p, first, LinChannels, n0, t0);
+    const int valid = min(bt, p.tokens - t0), n = n0 + 4 * lane, count = min(4, p.outputs - n);
+    float sw[4], bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int safe = min(n + i, p.outputs - 1);
+      sw[i] = p.weight_scales[safe];
+      bias[i] = p.bias != nullptr ? lin_in(static_cast<const T*>(p.bias)[safe]) : 0.f;
+    }
     __syncwarp();
     cluster_sync_all();
-    if (warp >= 2) {
-      int n0, t0;
-      origin(first, n0, t0);
-      const int valid = min(bt, p.tokens - t0), channel = tid - 64, out_n = n0 + channel;
-      if (out_n < p.outputs) {
-        const uint32_t partial = smem_u32(smem) + channel * 4;
-        const float sw = p.weight_scales[out_n], bias = p.bias != nullptr ? lin_in(static_cast<const T*>(p.bias)[out_n]) : 0.f;
-        for (int t = rank; t < valid; t += splits) {
-          int sum = 0;
-#pragma unroll 8
-          for (int r = 0; r < splits; ++r) sum += cluster_load(partial + t * LinChannels * 4, r);
-          float y = __fmul_rn(__fmul_rn((float)sum, sw), p.scales[t0 + t]);
-          if (p.bias != nullptr) y += bias;
-          if (p.residual != nullptr) y += lin_in(static_cast<const T*>(p.residual)[(int64_t)(t0 + t) * p.residual_stride + out_n]);
-          static_cast<T*>(p.out)[(int64_t)(t0 + t) * p.out_stride + out_n] = lin_out<T>(y);
-        }
+    const uint32_t partial = smem_base + lane * 16;
+    for (int t = rank + warp * splits; t < valid; t += splits * (LinThreads / 32)) {
+      const float st = p.scales[t0 + t];
+      float r[4] = {};
+      if (p.residual != nullptr) {
+        const T* from = static_cast<const T*>(p.residual) + (int64_t)(t0 + t) * p.residual_stride;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = lin_in(from[min(n + i, p.outputs - 1)]);
       }
-      __syncwarp();
+      int4 v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = q < splits ? cluster_load(partial + t * LinChannels * 4, q) : make_int4(0, 0, 0, 0);
+      int sum[4] = {};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) { sum[0] += v[q].x; sum[1] += v[q].y; sum[2] += v[q].z; sum[3] += v[q].w; }
+      T* to = static_cast<T*>(p.out) + (int64_t)(t0 + t) * p.out_stride + n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float y = __fmul_rn(__fmul_rn((float)sum[i], sw[i]), st);
+        if (p.bias != nullptr) y += bias[i];
+        if (p.residual != nullptr) y += r[i];
+        if (i < count) to[i] = lin_out<T>(y);
+      }
     }
+    __syncwarp();
     cluster_sync_all();                                       // nobody's shared memory goes away while it is read
   }
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && abort_flag) atomicExch(p.error, ErrBarrierTimeout);
   if (warp == 0) tmem_dealloc(tmem, p.columns);
+}
+
+// Two CTAs (a cluster of 2) per tile of 256 channels x token_tile tokens: MMAs of M = 256 that run on both SMs' tensor cores
+// (cta_group::2).  Each CTA holds its own 128 channels and half of the tokens, so an SM fetches 32 KB per 128 bytes of width
+// where a CTA alone fetches 48 KB for the same work, and the SM's port to L2 is what bounds the product of two large operands.
+// The even CTA issues the MMAs of both; copies of both report to its `full` barriers, commits arrive at both CTAs' barriers.
+template <typename T> __global__ void __launch_bounds__(LinThreads, 1) linear_pair_kernel(const __grid_constant__ CUtensorMap map_w,
+    const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearArgs p) {
+  extern __shared__ uint8_t raw_smem[];
+  __shared__ __align__(8) LinearBarriers bars;
+  __shared__ __align__(16) float token_scales[2][256];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int bt = p.token_tile, stage_bytes = LinWeightBytes + bt / 2 * LinDepth;
+  const int rank = blockIdx.x & 1, first = blockIdx.x / 2, step = gridDim.x / 2;
+  const int steps = (p.width + LinDepth - 1) / LinDepth, stages = p.stages;
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(&bars.full[s], 1); mbar_init(&bars.empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&bars.done[b], 1); mbar_init(&bars.free[b], 2 * LinEpilogueWarps); }
+    mbar_fence_init();
+    abort_flag = 0;
+  }
+  if (tid == 32) { lin_prefetch(&map_w); lin_prefetch(&map_x); }
+  if (warp == 0) pair_alloc(&tmem_slot, p.columns);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                         // both CTAs' barriers exist before anything arrives at them
+  tc_fence_after();
+  grid_launch_dependents();
+  grid_dependency_wait();
+  volatile int* abortp = &abort_flag;
+  const uint32_t tmem = tmem_slot, buffer = p.columns / 2;
+  const uint32_t smem_base = smem_u32(smem), full_base = smem_u32(&bars.full[0]), empty_base = smem_u32(&bars.empty[0]);
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t at = smem_base, full = full_base, empty = empty_base, phase = 1;
+      int stage = 0, filled = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < p.tiles; tile += step) {
+        int n0, t0;
+        lin_origin(p, tile, 2 * LinChannels, n0, t0);
+        n0 += rank * LinChannels; t0 += rank * (bt / 2);
+        for (int k = 0; k < steps * LinDepth; k += LinDepth) {
+          if (filled >= stages && !(ok = lin_wait(empty, phase, abortp))) break;
+          if (rank == 0) lin_expect(full, 2 * stage_bytes);   // what both CTAs' copies bring
+          pair_copy(at, &map_w, k, n0, full);
+          pair_copy(at + LinWeightBytes, &map_x, k, t0, full);
+          ++filled;
+          at += stage_bytes; full += 8; empty += 8;
+          if (++stage == stages) { stage = 0; at = smem_base; full = full_base; empty = empty_base; phase ^= 1u; }
+        }
+      }
+      if (*abortp && rank == 0)                               // the copies in flight land before the CTAs may leave
+        for (int j = max(0, filled - stages); j < filled; ++j) mbar_wait(&bars.full[j % stages], (j / stages) & 1u, 100000000ull);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = instr_desc(2, 1, 1, 2 * LinChannels, bt);
+      const uint64_t desc = smem_desc(smem_base, 0, 1024, Layout128B);
+      const uint32_t stage_units = stage_bytes >> 4;
+      uint32_t full = full_base, empty = empty_base, phase = 0;
+      int stage = 0, n = 0;
+      uint64_t dw = desc;
+      bool ok = true;
+      for (int tile = first; ok && tile < p.tiles; tile += step, ++n) {
+        const int b = n & 1;
+        if (n >= 2 && !(ok = lin_wait(smem_u32(&bars.free[b]), ((n >> 1) - 1) & 1, abortp))) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + b * buffer;
+        uint32_t accumulate = 0;
+        for (int k = 0; k < steps; ++k) {
+          if (!(ok = lin_wait(full, phase, abortp))) break;
+          tc_fence_after();
+          const uint64_t dx = dw + (LinWeightBytes >> 4);
+          pair_umma(acc, dw, dx, idesc, accumulate);
+#pragma unroll
+          for (int kk = 1; kk < LinDepth / 32; ++kk) pair_umma(acc, dw + 2 * kk, dx + 2 * kk, idesc, 1u);
+          pair_commit(empty);
+          accumulate = 1;
+          dw += stage_units; full += 8; empty += 8;
+          if (++stage == stages) { stage = 0; phase ^= 1u; dw = desc; full = full_base; empty = empty_base; }
+        }
+        pair_commit(smem_u32(&bars.done[b]));
+      }
+    }
+  } else {
+    int n = 0;
+    for (int tile = first; tile < p.tiles; tile += step, ++n) {
+      const int b = n & 1;
+      int n0, t0;
+      lin_origin(p, tile, 2 * LinChannels, n0, t0);
+      lin_epilogue<T>(p, tmem + b * buffer, n0 + rank * LinChannels, t0, min(bt, p.tokens - t0), token_scales[b],
+                      [&] { lin_wait(smem_u32(&bars.done[b]), (n >> 1) & 1, abortp); });
+      if (lane == 0) pair_arrive(smem_u32(&bars.free[b]));
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  cluster_sync_all();                                         // the partner's MMAs and arrivals reach into this CTA until here
+  if (tid == 0 && abort_flag) atomicExch(p.error, ErrBarrierTimeout);
+  if (warp == 0) pair_dealloc(tmem, p.columns);
 }
 
 // int8 rows: box = `box` rows x 128 bytes, 128-byte swizzle; what lies past the last row or the width reads as zero.
@@ -235,21 +474,25 @@ static int make_code_map(CUtensorMap* map, const void* base, int64_t rows, int w
 }
 
 template <typename T> static int launch_linear(const CUtensorMap& map_w, const CUtensorMap& map_x, const LinearArgs& p, int ctas,
-                                               int splits, cudaStream_t s) {
+                                               bool pair, cudaStream_t s) {
   static TriPerDevice configured;
   const int device = configured.pending();
   TRI_CHECK(device != -2, "int8_linear: no current CUDA device");
   if (device >= 0) {
     TRI_CUDA(cudaFuncSetAttribute(linear_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinShared), "int8_linear");
+    TRI_CUDA(cudaFuncSetAttribute(linear_pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinShared), "int8_linear");
     configured.mark(device);
   }
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)splits; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = pair ? 2u : (unsigned)p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(LinThreads); cfg.dynamicSmemBytes = LinShared; cfg.stream = s;
-  cfg.attrs = &attr; cfg.numAttrs = splits > 1 ? 1 : 0;
-  TRI_CUDA(cudaLaunchKernelEx(&cfg, linear_kernel<T>, map_w, map_x, p, splits), "int8_linear");
+  cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(LinThreads); cfg.dynamicSmemBytes = (size_t)p.shared; cfg.stream = s;
+  cfg.attrs = attr; cfg.numAttrs = attr[1].val.clusterDim.x > 1 ? 2 : 1;
+  if (pair) TRI_CUDA(cudaLaunchKernelEx(&cfg, linear_pair_kernel<T>, map_w, map_x, p), "int8_linear");
+  else TRI_CUDA(cudaLaunchKernelEx(&cfg, linear_kernel<T>, map_w, map_x, p), "int8_linear");
   return tri_launch_status("int8_linear");
 }
 
@@ -286,25 +529,32 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
   LinearArgs p{};
   p.residual_stride = residual_stride; p.out_stride = out_stride; p.scales = scales; p.weight_scales = weight_scales;
   p.bias = bias; p.residual = residual; p.out = out; p.tokens = (int)tokens; p.outputs = outputs; p.width = width; p.error = device_error;
+  const bool pair = getenv("TRI_PAIR") ? atoi(getenv("TRI_PAIR")) != 0 : tokens > 256;
   p.token_tile = (int)(tokens >= 256 ? 256 : (tokens + 15) / 16 * 16);
-  p.channel_tiles = (outputs + LinChannels - 1) / LinChannels;
+  if (getenv("TRI_BT")) p.token_tile = atoi(getenv("TRI_BT"));
+  if (pair) p.token_tile = (p.token_tile + 31) / 32 * 32;
+  const int channels = pair ? 2 * LinChannels : LinChannels, box = pair ? p.token_tile / 2 : p.token_tile;
+  p.channel_tiles = (outputs + channels - 1) / channels;
   const int64_t tiles = (tokens + p.token_tile - 1) / p.token_tile * (int64_t)p.channel_tiles;
   TRI_CHECK(tiles <= 0x7fffffff / 8, "int8_linear: tokens * outputs");
   p.tiles = (int)tiles;
-  p.group = 8;
-  p.stages = (LinShared - 1024) / (LinWeightBytes + p.token_tile * LinDepth);
+  p.group = getenv("TRI_GROUP") ? atoi(getenv("TRI_GROUP")) : 8;
+  p.shared = p.token_tile <= 64 && !pair ? 108 * 1024 : LinShared;
+  p.stages = (p.shared - 1024) / (LinWeightBytes + box * LinDepth);
   if (p.stages > LinMaxStages) p.stages = LinMaxStages;
   p.columns = 32;
   while (p.columns < 2 * p.token_tile) p.columns *= 2;
+  TRI_CHECK(p.columns <= 512, "columns");
   const int steps = (width + LinDepth - 1) / LinDepth;
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 * 2 <= steps) splits *= 2;
-  const int ctas = splits > 1 ? p.tiles * splits : (p.tiles < sms ? p.tiles : sms);
+  p.splits = 1;
+  if (const char* force = getenv("TRI_SPLITS")) p.splits = atoi(force);
+  else if (!pair) { p.splits = (int)(sms / tiles); if (p.splits > 8) p.splits = 8; if (p.splits > steps / 4) p.splits = steps / 4; if (p.splits < 1) p.splits = 1; }
+  const int ctas = pair ? 2 * (p.tiles < sms / 2 ? p.tiles : sms / 2) : p.splits > 1 ? p.tiles * p.splits : (p.tiles < sms ? p.tiles : sms);
   CUtensorMap map_w, map_x;
   if (make_code_map(&map_w, weight, outputs, width, weight_stride, LinChannels) != TRI_OK) return TRI_ERR_CUDA;
-  if (make_code_map(&map_x, codes, tokens, width, codes_stride, (unsigned)p.token_tile) != TRI_OK) return TRI_ERR_CUDA;
+  if (make_code_map(&map_x, codes, tokens, width, codes_stride, (unsigned)box) != TRI_OK) return TRI_ERR_CUDA;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, splits, s);
-  if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, splits, s);
-  return launch_linear<float>(map_w, map_x, p, ctas, splits, s);
+  if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, pair, s);
+  if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, pair, s);
+  return launch_linear<float>(map_w, map_x, p, ctas, pair, s);
 }
