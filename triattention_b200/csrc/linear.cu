@@ -15,7 +15,7 @@
 // Every wait on a barrier is bounded; after one has run out the CTA runs through, reports it and its output is void.
 #include "tcgen05.cuh"
 #include "abi_internal.h"
-#include <cstdlib>
+#include <mutex>
 
 namespace tri {
 
@@ -24,6 +24,7 @@ constexpr int LinEpilogueWarps = 8, LinThreads = 64 + 32 * LinEpilogueWarps;
 constexpr int LinWeightBytes = LinChannels * LinDepth;
 constexpr int LinShared = 216 * 1024;                        // stages (and, after a split tile, its partial sums); also keeps
                                                              // a second CTA that allocates TMEM off the SM
+constexpr int LinSmallTile = 64, LinSharedSmall = 108 * 1024; // up to this token tile two CTAs fit on an SM (and in TMEM)
 constexpr int LinMaxStages = 12;
 
 struct LinearArgs {
@@ -496,6 +497,102 @@ template <typename T> static int launch_linear(const CUtensorMap& map_w, const C
   return tri_launch_status("int8_linear");
 }
 
+// ---- which tile, how many CTAs per tile --------------------------------------------------------------------------------
+struct LinearPlan {
+  int token_tile, splits;
+  bool pair;
+};
+struct LinearDevice {                  // of one GPU, asked for once
+  int sms;
+  int clusters[2][9];                  // clusters of n CTAs that are resident at once, by shared memory (0: LinShared, 1: LinSharedSmall)
+};
+
+// Estimated time (us) of a plan, less what every plan takes.  The constants are a fit to measured times of 150 shapes (1 to 2048
+// tokens, 512 to 28672 channels, widths 512 to 14336) under every tile and split: the plan that the estimate picks is within 1 %
+// of the best one on average and within 13 % on each.  A stage of 128 bytes of width costs what the issuing thread needs for it
+// (0.27 us) or what the SM's port to L2 does (0.14 MB/us); tiles run in rounds of as many as are resident; a split adds a
+// cluster barrier and the exchange of the partial sums; and all of it overlaps with reading the operands once from HBM.
+static float plan_time(const LinearPlan& plan, int64_t tokens, int outputs, int width, const LinearDevice& d) {
+  const int steps = (width + LinDepth - 1) / LinDepth, bt = plan.token_tile;
+  const int channels = plan.pair ? 2 * LinChannels : LinChannels;
+  const int64_t tiles = (tokens + bt - 1) / bt * (int64_t)((outputs + channels - 1) / channels);
+  float t;
+  if (plan.pair) {
+    const float rounds = (float)((tiles + d.sms / 2 - 1) / (d.sms / 2)), epilogue = 0.0108f * bt;
+    t = rounds * fmaxf(0.266f * steps, epilogue) + epilogue;
+  } else {
+    const bool small = bt <= LinSmallTile;
+    const int64_t ctas = tiles * plan.splits, slots = (int64_t)d.clusters[small][plan.splits] * plan.splits;
+    const float rounds = (float)((ctas + slots - 1) / slots);
+    float stage = fmaxf(0.266f, (LinWeightBytes + bt * LinDepth) * (1.f / 141400.f));
+    if (small && ctas > d.sms) stage *= 1.95f;               // two CTAs per SM share its port and its tensor core
+    const float mine = (float)((steps + plan.splits - 1) / plan.splits) * stage, live = (float)(tokens < bt ? tokens : bt);
+    if (plan.splits > 1) t = rounds * (mine + 2.18f + 0.0074f * live);
+    else t = rounds * fmaxf(mine, 0.0068f * live) + 0.0068f * live;
+  }
+  const float memory = ((float)outputs + (float)tokens) * (float)width * (1.f / 6.2e6f);
+  return fmaxf(t, memory) + 0.15f * fminf(t, memory);
+}
+
+// The current GPU's figures; null after an error.
+static const LinearDevice* linear_device() {
+  static LinearDevice devices[TriPerDevice::MaxDevices];
+  static TriPerDevice known;
+  static std::mutex guard;
+  const int pending = known.pending();
+  int device = -1;
+  if (pending == -2 || cudaGetDevice(&device) != cudaSuccess) { tri_set_error("int8_linear: no current CUDA device"); return nullptr; }
+  if (pending >= 0) {
+    std::lock_guard<std::mutex> lock(guard);
+    LinearDevice d{};
+    cudaError_t e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinShared);
+    for (int small = 0; small < 2; ++small)
+      for (int n = 1; n <= 8 && e == cudaSuccess; ++n) {
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)n; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(n * 64)); cfg.blockDim = dim3(LinThreads); cfg.dynamicSmemBytes = small ? LinSharedSmall : LinShared;
+        cfg.attrs = &attr; cfg.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&d.clusters[small][n], linear_kernel<__nv_bfloat16>, &cfg);
+        if (e == cudaSuccess && d.clusters[small][n] < 1) d.clusters[small][n] = 1;
+      }
+    if (e != cudaSuccess) { tri_set_error(cudaGetErrorString(e)); return nullptr; }
+    devices[device] = d;
+    known.mark(device);
+  }
+  return &devices[device];
+}
+
+static LinearPlan choose_plan(int64_t tokens, int outputs, int width, const LinearDevice& d) {
+  const int steps = (width + LinDepth - 1) / LinDepth;
+  LinearPlan best{16, 1, false};
+  float best_time = 1e30f;
+  int tried = 0;
+  const auto consider = [&](int64_t bt) {                     // a token tile, in steps of 16 (a pair's: 32)
+    bt = bt < 16 ? 16 : bt > 256 ? 256 : (bt + 15) / 16 * 16;
+    const int bit = 1 << (bt / 16 - 1);
+    if (tried & bit) return;
+    tried |= bit;
+    const int64_t tiles = (tokens + bt - 1) / bt * (int64_t)((outputs + LinChannels - 1) / LinChannels);
+    for (int splits = 1; splits <= 8 && splits <= steps && (splits == 1 || tiles * splits <= 2 * (int64_t)d.sms); ++splits) {
+      const LinearPlan plan{(int)bt, splits, false};
+      const float time = plan_time(plan, tokens, outputs, width, d);
+      if (time < best_time) { best_time = time; best = plan; }
+    }
+    if (bt >= 64 && bt % 32 == 0) {
+      const LinearPlan plan{(int)bt, 1, true};
+      const float time = plan_time(plan, tokens, outputs, width, d);
+      if (time < best_time) { best_time = time; best = plan; }
+    }
+  };
+  const int64_t least = (tokens + 255) / 256;                 // token tiles at their largest; then evenly cut into a few more
+  for (int64_t more = 0; more < 4; ++more) consider((tokens + least + more - 1) / (least + more));
+  for (int bt : {256, 192, 128, 96, 64, 32}) if (bt < tokens + 16) consider(bt);
+  return best;
+}
+
 }  // namespace tri
 
 using namespace tri;
@@ -516,45 +613,33 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
                 reinterpret_cast<uintptr_t>(residual) % cell == 0,
             "int8_linear: output, bias and residual alignment");
   TRI_CHECK(out_stride >= outputs && (residual == nullptr || residual_stride >= 0), "int8_linear: output and residual rows");
-  static std::atomic<int> sm_count[TriPerDevice::MaxDevices];
-  int device = -1;
-  TRI_CUDA(cudaGetDevice(&device), "int8_linear");
-  TRI_CHECK(device >= 0 && device < TriPerDevice::MaxDevices, "int8_linear: device");
-  int sms = sm_count[device].load(std::memory_order_relaxed);
-  if (sms == 0) {
-    TRI_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "int8_linear");
-    sm_count[device].store(sms, std::memory_order_relaxed);
-  }
+  const LinearDevice* gpu = linear_device();
+  if (gpu == nullptr) return TRI_ERR_CUDA;
+  const LinearPlan plan = choose_plan(tokens, outputs, width, *gpu);
 
   LinearArgs p{};
   p.residual_stride = residual_stride; p.out_stride = out_stride; p.scales = scales; p.weight_scales = weight_scales;
   p.bias = bias; p.residual = residual; p.out = out; p.tokens = (int)tokens; p.outputs = outputs; p.width = width; p.error = device_error;
-  const bool pair = getenv("TRI_PAIR") ? atoi(getenv("TRI_PAIR")) != 0 : tokens > 256;
-  p.token_tile = (int)(tokens >= 256 ? 256 : (tokens + 15) / 16 * 16);
-  if (getenv("TRI_BT")) p.token_tile = atoi(getenv("TRI_BT"));
-  if (pair) p.token_tile = (p.token_tile + 31) / 32 * 32;
-  const int channels = pair ? 2 * LinChannels : LinChannels, box = pair ? p.token_tile / 2 : p.token_tile;
+  p.token_tile = plan.token_tile; p.splits = plan.splits;
+  const int channels = plan.pair ? 2 * LinChannels : LinChannels, box = plan.pair ? p.token_tile / 2 : p.token_tile;
   p.channel_tiles = (outputs + channels - 1) / channels;
   const int64_t tiles = (tokens + p.token_tile - 1) / p.token_tile * (int64_t)p.channel_tiles;
   TRI_CHECK(tiles <= 0x7fffffff / 8, "int8_linear: tokens * outputs");
   p.tiles = (int)tiles;
-  p.group = getenv("TRI_GROUP") ? atoi(getenv("TRI_GROUP")) : 8;
-  p.shared = p.token_tile <= 64 && !pair ? 108 * 1024 : LinShared;
+  p.group = 8;
+  p.shared = !plan.pair && p.token_tile <= LinSmallTile ? LinSharedSmall : LinShared;
   p.stages = (p.shared - 1024) / (LinWeightBytes + box * LinDepth);
   if (p.stages > LinMaxStages) p.stages = LinMaxStages;
   p.columns = 32;
   while (p.columns < 2 * p.token_tile) p.columns *= 2;
-  TRI_CHECK(p.columns <= 512, "columns");
-  const int steps = (width + LinDepth - 1) / LinDepth;
-  p.splits = 1;
-  if (const char* force = getenv("TRI_SPLITS")) p.splits = atoi(force);
-  else if (!pair) { p.splits = (int)(sms / tiles); if (p.splits > 8) p.splits = 8; if (p.splits > steps / 4) p.splits = steps / 4; if (p.splits < 1) p.splits = 1; }
-  const int ctas = pair ? 2 * (p.tiles < sms / 2 ? p.tiles : sms / 2) : p.splits > 1 ? p.tiles * p.splits : (p.tiles < sms ? p.tiles : sms);
+  const int resident = plan.pair ? gpu->sms / 2 : p.shared == LinShared ? gpu->sms : 2 * gpu->sms;
+  const int ctas = plan.pair ? 2 * (p.tiles < resident ? p.tiles : resident)
+                             : p.splits > 1 ? p.tiles * p.splits : (p.tiles < resident ? p.tiles : resident);
   CUtensorMap map_w, map_x;
   if (make_code_map(&map_w, weight, outputs, width, weight_stride, LinChannels) != TRI_OK) return TRI_ERR_CUDA;
   if (make_code_map(&map_x, codes, tokens, width, codes_stride, (unsigned)box) != TRI_OK) return TRI_ERR_CUDA;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, pair, s);
-  if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, pair, s);
-  return launch_linear<float>(map_w, map_x, p, ctas, pair, s);
+  if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, plan.pair, s);
+  if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, plan.pair, s);
+  return launch_linear<float>(map_w, map_x, p, ctas, plan.pair, s);
 }
