@@ -19,6 +19,7 @@
 namespace tri {
 
 enum RowMode : int { RowPlain = 0, RowGated = 1, RowNorm = 2 };
+constexpr int RowShared = 200 * 1024;                // per SM, for the rows ahead
 constexpr float RowTiny = 1.504632769052528e-36f;   // 2^-119
 constexpr float RowLargestScale = 0x1.0204060000000p+121f;   // the largest float of which 127 times is no infinity
 
@@ -41,25 +42,29 @@ struct RowArgs {
   float* scales;
   int64_t rows;
   int width;
-  float eps;
+  float eps, inverse_width;
 };
 
 // Largest magnitude as the bits of |y|: an integer maximum, so that a NaN (whose bits lie above every number's) survives.
 __device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
 
-// Sum and maximum over the CTA; every thread gets both.
-__device__ __forceinline__ void row_reduce(float& sum, uint32_t& peak, float* sums, uint32_t* peaks) {
+// Maximum (and, for the norm, sum) over the CTA; every thread gets both.
+template <bool Sum> __device__ __forceinline__ void row_reduce(float& sum, uint32_t& peak, float* sums, uint32_t* peaks) {
+  peak = __reduce_max_sync(0xffffffffu, peak);
+  if (Sum)
 #pragma unroll
-  for (int bit = 16; bit > 0; bit >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, bit);
-    peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, bit));
-  }
-  const int warps = blockDim.x / 32, warp = threadIdx.x / 32;
+    for (int bit = 16; bit > 0; bit >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, bit);
+  const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (warps == 1) return;
   __syncthreads();                    // the arrays may still be read from the call before
-  if (threadIdx.x % 32 == 0) { sums[warp] = sum; peaks[warp] = peak; }
+  if (lane == 0) { if (Sum) sums[warp] = sum; peaks[warp] = peak; }
   __syncthreads();
-  sum = 0.f; peak = 0;
-  for (int i = 0; i < warps; ++i) { sum += sums[i]; peak = max(peak, peaks[i]); }
+  peak = __reduce_max_sync(0xffffffffu, lane < warps ? peaks[lane] : 0u);
+  if (Sum) {
+    sum = lane < warps ? sums[lane] : 0.f;
+#pragma unroll
+    for (int bit = 16; bit > 0; bit >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, bit);
+  }
 }
 
 // silu(g) * u in IEEE arithmetic.  Below a gate of -87.3 the sum passes 2^126 and the product counts as zero (silu(g) is within
@@ -73,17 +78,26 @@ __device__ __forceinline__ float gated(float g, float u) {
 __device__ __forceinline__ bool squares_fit(float squares) { return squares < 3e38f && squares > 1e-24f; }
 
 struct RowScale {
-  float scale, inverse;                 // inverse: 127 / max|y| before the norm's common factor
+  float scale, inverse;                 // inverse: of max|y| / 127, before the norm's common factor
   bool live;                            // codes are not all zero
 };
-template <int Mode> __device__ __forceinline__ RowScale row_scale(uint32_t peak, float squares, float factor, float eps) {
-  const float largest = __uint_as_float(peak);
-  const bool finite = peak < 0x7f800000u && (Mode != RowNorm || squares < 3e38f);
-  const bool zero = largest < RowTiny || (Mode == RowNorm && squares == 0.f && eps == 0.f);
+// (Every thread of a row works this out, and it weighs as much as eight elements: approximate reciprocal and root, 2^-22.9.)
+template <int Mode> __device__ __forceinline__ RowScale row_scale(uint32_t peak, float squares, float eps, float inverse_width, float shift) {
+  const float step = __uint_as_float(peak) * (1.f / 127.f);
+  bool finite = peak < 0x7f800000u, zero = __uint_as_float(peak) < RowTiny;
   RowScale r;
+  r.scale = step;
+  if (Mode == RowNorm) {
+    const float power = fmaf(squares, inverse_width, eps * shift * shift);
+    finite = finite && squares < 3e38f;
+    zero = zero || power == 0.f;
+    float factor;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(factor) : "f"(power));
+    r.scale *= factor;
+  }
   r.live = finite && !zero;
-  r.scale = !finite ? CUDART_NAN_F : zero ? 0.f : fminf(largest * (1.f / 127.f) * factor, RowLargestScale);
-  r.inverse = r.live ? __fdiv_rn(127.f, largest) : 0.f;
+  r.scale = !finite ? CUDART_NAN_F : zero ? 0.f : fminf(r.scale, RowLargestScale);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inverse) : "f"(r.live ? step : 1.f));
   return r;
 }
 
@@ -119,15 +133,13 @@ template <typename T, int Mode> __device__ __noinline__ void row_general(const R
     squares = 0.f; peak = 0;
     for (int e = threadIdx.x; e < p.width; e += threads)
       peak = max(peak, magnitude(row_element<T, Mode>(p, a, b, sum, e, shift, squares)));
-    row_reduce(squares, peak, sums, peaks);
+    row_reduce<Mode == RowNorm>(squares, peak, sums, peaks);
     if (Mode == RowNorm && sum != nullptr) { a = sum; b = nullptr; sum = nullptr; }   // from here on h is read (a thread reads
                                                                                       // what it wrote; residual may be gone)
     if (Mode != RowNorm || squares_fit(squares) || (squares == 0.f && peak == 0)) break;
     shift = squares > 1.f || squares != squares ? 8.271806125530277e-25f : 1.152921504606847e18f;   // 2^-80, 2^60
   }
-  float factor = 1.f;
-  if (Mode == RowNorm) factor = __frsqrt_rn(__fdiv_rn(squares, (float)p.width) + p.eps * shift * shift);
-  const RowScale r = row_scale<Mode>(peak, squares, factor, p.eps);
+  const RowScale r = row_scale<Mode>(peak, squares, p.eps, p.inverse_width, shift);
   if (threadIdx.x == 0) p.scales[row] = r.scale;
   int8_t* codes = p.codes + row * p.codes_stride;
   for (int e = threadIdx.x; e < p.width; e += threads) {
@@ -139,19 +151,76 @@ template <typename T, int Mode> __device__ __noinline__ void row_general(const R
 template <typename T, int Mode> __global__ void __launch_bounds__(1024) rows_general_kernel(const RowArgs p) {
   __shared__ float sums[32];
   __shared__ uint32_t peaks[32];
+  grid_launch_dependents();
+  grid_dependency_wait();
   row_general<T, Mode>(p, blockIdx.x, false, sums, peaks);
 }
 
 // ---- rows held in registers ---------------------------------------------------------------------------------------------
-// A thread holds V vectors of 16 bytes of the row (vector j of thread i is number j * threads + i), loaded at once, so the row
-// is read from memory once whatever the mode.  Rows * width decides nothing here; the work is bound by HBM for long batches
-// and by one round trip to memory plus one reduction for short ones.
-// Gated: the y that a thread keeps are computed with the fast exponential and reciprocal (12 instead of 30 instructions per
-// element, which would bound the kernel); they are within GatedError of the IEEE values.  Where that could show, at elements
+// A thread holds V vectors of 16 bytes (or V * N single elements) of a row, so the row is read from memory once whatever the
+// mode.  Long batches are bound by HBM: a CTA takes rows in turn and copies the rows after the current one into shared memory
+// meanwhile (cp.async, every thread its own vectors, so no barrier is involved): without that the loads of a row wait for the
+// reduction of the row before.  Short batches are bound by one trip to memory and one reduction.
+// Gated: the y that a thread keeps are computed with the fast exponential and reciprocal (8 instead of 30 instructions per
+// element, which would bound the kernel).  Where that could show, at elements
 // that may be the row's largest and at quotients next to a tie, the element is computed again in IEEE arithmetic.
-constexpr float GatedError = 2e-5f;     // relative: __expf 2 + 1.17 |g| steps of 2^-23 with |g| < 88, reciprocal 2, rest 3: 1.3e-5
-constexpr float PlainError = 3e-7f;     // y * (1/s) against y / s: three roundings of 2^-24
+// Relative error of the fast y and of y / s worked out from it, in steps of 2^-24: 1.5 |g| for the exponent's argument, 4 for the
+// exponential, 5 for sum, reciprocal and products, 5 for the IEEE evaluation itself, 4 for the quotient: 42 for |g| <= 16 (which
+// gates hardly ever leave), 150 for the |g| < 88 that give a y at all.
+constexpr float GatedNear = 3e-6f, GatedFar = 1.2e-5f, GateNear = -16.f;
+constexpr float PlainError = 5e-7f;     // y * (1/s) against y / s: 2^-23 for the reciprocal, 2^-24 for product and quotient each, 2^-22
 constexpr float Round = 12582912.f;     // 1.5 * 2^23: x + Round has rint(x) in its low bits
+
+enum RowLayout : int { RowCta = 0, RowWarp = 1, RowElements = 2 };
+
+// max(|a|, |b|, |c|); NaN where any is.
+__device__ __forceinline__ float max_magnitude(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two fp32 operations in one instruction; the kernels are bound by the instructions they issue as much as by HBM.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\tfma.rn.f32x2 z, x, y, w;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float2 gated_fast2(float2 g, float2 u) {
+  const float2 x = mul2(g, both(-1.4426950408889634f));
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(x.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(x.y));
+  e = add2(e, both(1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+  return mul2(mul2(g, r), u);
+}
+__device__ __forceinline__ float gated_fast(float g, float u) { return gated_fast2(both(g), both(u)).x; }
+__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait(int pending) {      // until at most `pending` of this thread's groups are under way
+  if (pending >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (pending == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
 
 template <typename T> struct RowVector {
   static constexpr int N = 16 / sizeof(T);
@@ -197,127 +266,236 @@ template <typename T> __device__ __noinline__ float gated_exact(const T* gate, c
   return gated(row_to_float(gate[e]), row_to_float(up[e]));
 }
 
-// Rows that start on 16-byte boundaries (all inputs) with a width of whole vectors.  Warp = true: a warp per row, several rows
-// per CTA; otherwise a CTA per row.
-template <typename T, int Mode, int V, bool Warp> __global__ void __launch_bounds__(Warp ? 128 : 1024) rows_kernel(const RowArgs p) {
+// RowCta: inputs start on 16-byte boundaries and hold whole vectors; a CTA per row, gridDim.x rows at a time, `depth` rows in
+// shared memory.  RowWarp: the same for short rows, a warp per row, four per CTA.  RowElements: any alignment and width, a CTA
+// per row, single elements.
+template <typename T, int Mode, int V, int Layout> __global__ void __launch_bounds__(Layout == RowWarp ? 128 : 1024)
+    rows_kernel(const RowArgs p, int depth) {
   constexpr int N = RowVector<T>::N;
+  extern __shared__ uint4 ring[];       // RowCta: [depth][a, b][V][thread]
   __shared__ float sums[32];
   __shared__ uint32_t peaks[32];
   __shared__ uint32_t exact_peak;
-  const int threads = Warp ? 32 : blockDim.x, me = Warp ? threadIdx.x % 32 : threadIdx.x;
-  const int64_t row = Warp ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
-  if (Warp && row >= p.rows) return;
-  const int vectors = p.width / N;
-  const T* a = static_cast<const T*>(p.a) + row * p.a_stride;
-  const T* b = p.b == nullptr ? nullptr : static_cast<const T*>(p.b) + row * p.b_stride;
-  RowVector<T> va[V], vb[V];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int threads = Layout == RowWarp ? 32 : blockDim.x, me = Layout == RowWarp ? threadIdx.x % 32 : threadIdx.x;
+  const int64_t first = Layout == RowWarp ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
+  const int64_t stride = Layout == RowWarp ? (int64_t)gridDim.x * 4 : gridDim.x;
+  const int vectors = p.width / N;      // (not RowElements)
+  const bool two = Mode != RowPlain && p.b != nullptr;
+  const T *a0 = static_cast<const T*>(p.a), *b0 = static_cast<const T*>(p.b);
+  const auto element = [&](int j, int i) { return Layout == RowElements ? (j * N + i) * threads + me : (j * threads + me) * N + i; };
+
+  const int parts = two ? 2 : 1;
+  const auto slot = [&](int d, int part, int j) { return ring + ((d * parts + part) * V + j) * threads + me; };
+  const auto prefetch = [&](int d, int64_t row) {
+    if (row < p.rows) {
+      const uint4 *a = reinterpret_cast<const uint4*>(a0 + row * p.a_stride), *b = reinterpret_cast<const uint4*>(b0 + row * p.b_stride);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int v = j * threads + me;
-    va[j].raw = v < vectors ? __ldcs(reinterpret_cast<const uint4*>(a) + v) : make_uint4(0, 0, 0, 0);
-    if (Mode != RowPlain && b != nullptr) vb[j].raw = v < vectors ? __ldcs(reinterpret_cast<const uint4*>(b) + v) : make_uint4(0, 0, 0, 0);
-  }
-  if (!Warp && Mode == RowGated && threadIdx.x == 0) exact_peak = 0;
-  float y[V][N], squares = 0.f;
-  float largest = 0.f, odd = 0.f;      // odd turns NaN with any y that is not finite
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int v = j * threads + me;
-    va[j].unpack(y[j]);
-    if constexpr (Mode == RowGated) {
-      float u[N];
-      vb[j].unpack(u);
-#pragma unroll
-      for (int i = 0; i < N; ++i) y[j][i] = __fdividef(y[j][i], 1.f + __expf(-y[j][i])) * u[i];
-    }
-    if constexpr (Mode == RowNorm) {
-      if (b != nullptr) {
-        float r[N];
-        vb[j].unpack(r);
-#pragma unroll
-        for (int i = 0; i < N; ++i) y[j][i] += r[i];
-        RowVector<T> h;
-        h.pack(y[j]);
-        h.unpack(y[j]);
-        if (v < vectors) reinterpret_cast<uint4*>(static_cast<T*>(p.sum) + row * p.sum_stride)[v] = h.raw;
-      }
-      RowVector<T> vw;
-      vw.raw = v < vectors ? __ldg(reinterpret_cast<const uint4*>(p.weight) + v) : make_uint4(0, 0, 0, 0);
-      float w[N];
-      vw.unpack(w);
-#pragma unroll
-      for (int i = 0; i < N; ++i) { squares = fmaf(y[j][i], y[j][i], squares); y[j][i] *= w[i]; }
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) { largest = fmaxf(largest, fabsf(y[j][i])); odd = fmaf(y[j][i], 0.f, odd); }
-  }
-  uint32_t peak = odd == 0.f ? __float_as_uint(largest) : 0x7fc00000u;
-  if constexpr (Warp) {
-#pragma unroll
-    for (int bit = 16; bit > 0; bit >>= 1) {
-      squares += __shfl_xor_sync(0xffffffffu, squares, bit);
-      peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, bit));
-    }
-  } else {
-    row_reduce(squares, peak, sums, peaks);
-  }
-  if constexpr (Mode == RowNorm && !Warp) {
-    if (!squares_fit(squares) && !(squares == 0.f && peak == 0)) {      // (the same for the whole CTA)
-      row_general<T, Mode>(p, row, b != nullptr, sums, peaks);
-      return;
-    }
-  }
-  if constexpr (Mode == RowGated) {
-    if (peak != 0 && peak < 0x7f800000u) {
-      const float bar = __uint_as_float(peak) * (1.f - 2.f * GatedError);
-      uint32_t exact = 0;
-      if (largest >= bar) {
-        for (int j = 0; j < V; ++j) {
-          const int v = j * threads + me;
-          for (int i = 0; i < N; ++i)
-            if (v < vectors && fabsf(reinterpret_cast<float(&)[V][N]>(y)[j][i]) >= bar) exact = max(exact, magnitude(gated_exact(a, b, v * N + i)));
+      for (int j = 0; j < V; ++j) {
+        const int v = j * threads + me;
+        if (v < vectors) {
+          copy_async(slot(d, 0, j), a + v);
+          if (two) copy_async(slot(d, 1, j), b + v);
         }
       }
-      if constexpr (Warp) {
-        peak = __reduce_max_sync(0xffffffffu, exact);
-      } else {
-        if (exact != 0) atomicMax(&exact_peak, exact);
-        __syncthreads();
-        peak = exact_peak;
-      }
+    }
+    copy_commit();
+  };
+  if constexpr (Layout == RowCta)
+    for (int d = 0; d < depth; ++d) prefetch(d, first + d * stride);
+  RowVector<T> vw[V];                   // norm: this thread's part of the weight, which every row needs
+  if constexpr (Mode == RowNorm && Layout == RowCta && V <= 2) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int v = j * threads + me;
+      vw[j].raw = v < vectors ? __ldg(reinterpret_cast<const uint4*>(p.weight) + v) : make_uint4(0, 0, 0, 0);
     }
   }
-  const float factor = Mode == RowNorm ? __frsqrt_rn(__fdiv_rn(squares, (float)p.width) + p.eps) : 1.f;
-  const RowScale r = row_scale<Mode>(peak, squares, factor, p.eps);
-  if (me == 0) p.scales[row] = r.scale;
-  const float inverse = Mode == RowNorm ? r.inverse : r.live ? __frcp_rn(r.scale) : 0.f;
-  int8_t* codes = p.codes + row * p.codes_stride;
+
+  int turn = 0;                         // ring slot of the current row
+  for (int64_t row = first; row < p.rows; row += stride) {
+    const T *a = a0 + row * p.a_stride, *b = b0 + row * p.b_stride;
+    T* sum = Mode == RowNorm && two ? static_cast<T*>(p.sum) + row * p.sum_stride : nullptr;
+    float y[V][N], squares = 0.f, largest = 0.f, lowest = 0.f;   // lowest: of the gates
+    if constexpr (Layout == RowCta) copy_wait(depth - 1);
+    if constexpr (Mode == RowGated && Layout != RowWarp) if (threadIdx.x == 0) exact_peak = 0;
+    if constexpr (Layout == RowElements) {
+      float r[V][N], w[V][N];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int v = j * threads + me;
-    uint32_t c[N];
-    float off = 0.f;                    // above 0.5: some quotient may lie on the other side of a tie
+      for (int j = 0; j < V; ++j)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float q = y[j][i] * inverse, up = q + Round;
-      c[i] = __float_as_uint(up);
-      if (Mode != RowNorm) off = fmaxf(off, fmaf(fabsf(q), Mode == RowGated ? GatedError : PlainError, fabsf(q - (up - Round))));
+        for (int i = 0; i < N; ++i) {
+          const int e = min(element(j, i), p.width - 1);      // (unconditional, so that all loads are under way at once)
+          y[j][i] = row_to_float(a[e]);
+          if (two) r[j][i] = row_to_float(b[e]);
+          if (Mode == RowNorm) w[j][i] = row_to_float(static_cast<const T*>(p.weight)[e]);
+        }
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int e = element(j, i);
+          const bool live = e < p.width;
+          if (Mode == RowGated) { lowest = fminf(lowest, y[j][i]); y[j][i] = gated_fast(y[j][i], r[j][i]); }
+          if (Mode == RowNorm) {
+            if (two) {
+              const T h = row_from_float<T>(y[j][i] + r[j][i]);
+              if (live) sum[e] = h;
+              y[j][i] = row_to_float(h);
+            }
+            if (!live) y[j][i] = 0.f;
+            squares = fmaf(y[j][i], y[j][i], squares);
+            y[j][i] *= w[j][i];
+          }
+          if (!live) y[j][i] = 0.f;
+        }
+    } else {
+      RowVector<T> va[V], vb[V];
+      float2 squares2 = both(0.f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int v = j * threads + me;
+        if constexpr (Layout == RowCta) {
+          va[j].raw = v < vectors ? *slot(turn, 0, j) : make_uint4(0, 0, 0, 0);
+          if (two) vb[j].raw = v < vectors ? *slot(turn, 1, j) : make_uint4(0, 0, 0, 0);
+        } else {
+          va[j].raw = v < vectors ? __ldcs(reinterpret_cast<const uint4*>(a) + v) : make_uint4(0, 0, 0, 0);
+          if (two) vb[j].raw = v < vectors ? __ldcs(reinterpret_cast<const uint4*>(b) + v) : make_uint4(0, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int v = j * threads + me;
+        va[j].unpack(y[j]);
+        if (two) {
+          float r[N];
+          vb[j].unpack(r);
+          if constexpr (Mode == RowGated) {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+              lowest = fminf(lowest, fminf(y[j][i], y[j][i + 1]));
+              const float2 t = gated_fast2(make_float2(y[j][i], y[j][i + 1]), make_float2(r[i], r[i + 1]));
+              y[j][i] = t.x; y[j][i + 1] = t.y;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+              const float2 t = add2(make_float2(y[j][i], y[j][i + 1]), make_float2(r[i], r[i + 1]));
+              y[j][i] = t.x; y[j][i + 1] = t.y;
+            }
+            RowVector<T> h;
+            h.pack(y[j]);
+            h.unpack(y[j]);
+            if (v < vectors) reinterpret_cast<uint4*>(sum)[v] = h.raw;
+          }
+        }
+        if constexpr (Mode == RowNorm) {
+          if constexpr (Layout != RowCta || V > 2) vw[j].raw = v < vectors ? __ldg(reinterpret_cast<const uint4*>(p.weight) + v) : make_uint4(0, 0, 0, 0);
+          float w[N];
+          vw[j].unpack(w);
+#pragma unroll
+          for (int i = 0; i < N; i += 2) {
+            const float2 h = make_float2(y[j][i], y[j][i + 1]), t = mul2(h, make_float2(w[i], w[i + 1]));
+            squares2 = fma2(h, h, squares2);
+            y[j][i] = t.x; y[j][i + 1] = t.y;
+          }
+        }
+      }
+      squares = squares2.x + squares2.y;
     }
-    if (Mode != RowNorm && off >= 0.5f && r.live && v < vectors) {
-      for (int i = 0; i < N; ++i) {
-        const float exact = Mode == RowGated ? gated_exact(a, b, v * N + i) : row_to_float(a[v * N + i]);
-        const uint32_t code = (uint32_t)__float2int_rn(exact / r.scale);
 #pragma unroll
-        for (int k = 0; k < N; ++k) if (k == i) c[k] = code;
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < N; i += 2) largest = max_magnitude(largest, y[j][i], y[j][i + 1]);
+    const float error = Mode == RowPlain ? PlainError : lowest < GateNear ? GatedFar : GatedNear;
+    const auto advance = [&] {          // the slot takes the row `depth` turns ahead
+      if constexpr (Layout == RowCta) {
+        prefetch(turn, row + depth * stride);
+        turn = turn + 1 == depth ? 0 : turn + 1;
+      }
+    };
+    // (the row's inputs are in registers; a gated row looks a few of them up again below, in its slot if it can wait that long)
+    const bool keep = Mode == RowGated && Layout == RowCta && depth > 1;
+    if (!keep) advance();
+    uint32_t peak = __float_as_uint(largest);
+    if constexpr (Layout == RowWarp) {
+      peak = __reduce_max_sync(0xffffffffu, peak);
+    } else {
+      row_reduce<Mode == RowNorm>(squares, peak, sums, peaks);
+    }
+    if constexpr (Mode == RowNorm) {
+      if (!squares_fit(squares) && !(squares == 0.f && peak == 0)) {      // (the same for the whole CTA)
+        row_general<T, Mode>(p, row, two, sums, peaks);
+        continue;
       }
     }
-    if (v < vectors) {
-      uint32_t w[N / 4];
+    if constexpr (Mode == RowGated) {
+      if (peak != 0 && peak < 0x7f800000u) {
+        const float bar = __uint_as_float(peak) * (1.f - 2.f * GatedFar);
+        uint32_t exact = 0;
+        if (largest >= bar) {
 #pragma unroll
-      for (int k = 0; k < N / 4; ++k)
-        w[k] = r.live ? __byte_perm(__byte_perm(c[4 * k], c[4 * k + 1], 0x0040), __byte_perm(c[4 * k + 2], c[4 * k + 3], 0x0040), 0x5410) : 0u;
-      if constexpr (N == 8) reinterpret_cast<uint2*>(codes)[v] = make_uint2(w[0], w[1]);
-      else reinterpret_cast<uint32_t*>(codes)[v] = w[0];
+          for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              if (fabsf(y[j][i]) >= bar)
+                exact = max(exact, magnitude(keep ? gated_exact(reinterpret_cast<const T*>(slot(turn, 0, j)), reinterpret_cast<const T*>(slot(turn, 1, j)), i)
+                                                  : gated_exact(a, b, element(j, i))));
+        }
+        if constexpr (Layout == RowWarp) {
+          peak = __reduce_max_sync(0xffffffffu, exact);
+        } else {
+          if (exact != 0) atomicMax(&exact_peak, exact);
+          __syncthreads();
+          peak = exact_peak;
+        }
+      }
+    }
+    if (keep) advance();
+    const RowScale r = row_scale<Mode>(peak, squares, p.eps, p.inverse_width, 1.f);
+    if (me == 0) p.scales[row] = r.scale;
+    const float inverse = r.inverse;
+    int8_t* codes = p.codes + row * p.codes_stride;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      uint32_t c[N];
+      float off = 0.f, size = 0.f;      // largest distance from the next code, largest quotient
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 q = mul2(make_float2(y[j][i], y[j][i + 1]), both(inverse)), up = add2(q, both(Round));
+        c[i] = __float_as_uint(up.x); c[i + 1] = __float_as_uint(up.y);
+        if (Mode != RowNorm) {
+          const float2 back = add2(up, both(-Round)), from = fma2(back, both(-1.f), q);
+          off = max_magnitude(off, from.x, from.y);
+          size = max_magnitude(size, q.x, q.y);
+        }
+      }
+      if (Mode != RowNorm && fmaf(size, error, off) >= 0.5f && r.live) {
+        // some quotient of these may lie on the other side of a tie
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float q = y[j][i] * inverse, from = fabsf(q - (q + Round - Round));
+          if (fmaf(fabsf(q), error, from) >= 0.5f) {
+            const float exact = Mode == RowGated ? gated_exact(a, b, element(j, i)) : y[j][i];
+            c[i] = (uint32_t)__float2int_rn(exact / r.scale);
+          }
+        }
+      }
+      if constexpr (Layout == RowElements) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) if (element(j, i) < p.width) codes[element(j, i)] = r.live ? (int8_t)c[i] : (int8_t)0;
+      } else {
+        const int v = j * threads + me;
+        if (v < vectors) {
+          uint32_t w[N / 4];
+#pragma unroll
+          for (int k = 0; k < N / 4; ++k)
+            w[k] = r.live ? __byte_perm(__byte_perm(c[4 * k], c[4 * k + 1], 0x0040), __byte_perm(c[4 * k + 2], c[4 * k + 3], 0x0040), 0x5410) : 0u;
+          if constexpr (N == 8) reinterpret_cast<uint2*>(codes)[v] = make_uint2(w[0], w[1]);
+          else reinterpret_cast<uint32_t*>(codes)[v] = w[0];
+        }
+      }
     }
   }
 }
@@ -326,6 +504,8 @@ template <typename T, int Mode, int V, bool Warp> __global__ void __launch_bound
 template <typename T, bool Vector> __global__ void __launch_bounds__(256) dequantize_rows_kernel(const int8_t* codes, int64_t codes_stride,
     const float* scales, T* out, int64_t out_stride, int64_t rows, int width) {
   constexpr int N = Vector ? 8 : 1;
+  grid_launch_dependents();
+  grid_dependency_wait();
   const int per_row = width / N;
   const int64_t total = rows * per_row;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -352,48 +532,101 @@ template <typename T, bool Vector> __global__ void __launch_bounds__(256) dequan
   }
 }
 
-template <typename T, int Mode> static void launch_rows_type(int64_t rows, const RowArgs& p, cudaStream_t s) {
+// One call of rows_kernel with as many CTAs as are resident at once (RowCta) or as the rows need.
+template <typename T, int Mode, int V, int Layout> static int launch_rows_kernel(const RowArgs& p, int sms, cudaStream_t s) {
   constexpr int N = RowVector<T>::N;
-  const auto vector_rows = [](const void* base, int64_t stride) { return aligned16(base) && stride % N == 0; };
-  const int vectors = p.width / N;
-  const bool fast = p.width % N == 0 && vectors <= 4096 && vector_rows(p.a, p.a_stride) && vector_rows(p.b, p.b_stride) &&
-                    vector_rows(p.weight, 0) && vector_rows(p.sum, p.sum_stride);
-  if (!fast) {
-    const int threads = p.width <= 256 ? 128 : p.width <= 2048 ? 256 : 512;
-    rows_general_kernel<T, Mode><<<(unsigned)rows, threads, 0, s>>>(p);
-    return;
+  const auto kernel = rows_kernel<T, Mode, V, Layout>;
+  if (Layout == RowWarp) {
+    TRI_CUDA(launch_chained(kernel, dim3((unsigned)((p.rows + 3) / 4)), dim3(128), 0, s, p, 1), "rows");
+    return tri_launch_status("rows");
   }
-  if constexpr (Mode != RowNorm) {
-    if (vectors <= 64) {
-      const unsigned grid = (unsigned)((rows + 3) / 4);
-      if (vectors <= 32) rows_kernel<T, Mode, 1, true><<<grid, 128, 0, s>>>(p);
-      else rows_kernel<T, Mode, 2, true><<<grid, 128, 0, s>>>(p);
-      return;
-    }
+  const int items = Layout == RowElements ? p.width : p.width / N, each = Layout == RowElements ? V * N : V;
+  const int threads = ((items + each - 1) / each + 31) / 32 * 32;
+  if (Layout == RowElements) {
+    TRI_CUDA(launch_chained(kernel, dim3((unsigned)p.rows), dim3(threads), 0, s, p, 1), "rows");
+    return tri_launch_status("rows");
   }
-  // one vector per thread while that gives every SM little to do (one round trip bounds the call), four otherwise
-  const int want = rows <= 592 ? 1 : 4, least = (vectors + 1023) / 1024;
-  const int v = want < least ? (least <= 2 ? 2 : 4) : want;
-  int threads = ((vectors + v - 1) / v + 31) / 32 * 32;
-  if (v == 1) rows_kernel<T, Mode, 1, false><<<(unsigned)rows, threads, 0, s>>>(p);
-  else if (v == 2) rows_kernel<T, Mode, 2, false><<<(unsigned)rows, threads, 0, s>>>(p);
-  else rows_kernel<T, Mode, 4, false><<<(unsigned)rows, threads, 0, s>>>(p);
-}
-
-template <int Mode> static int launch_rows(int type, int64_t rows, const RowArgs& p, cudaStream_t s) {
-  if (type == TRI_BF16) launch_rows_type<__nv_bfloat16, Mode>(rows, p, s);
-  else if (type == TRI_FP16) launch_rows_type<__half, Mode>(rows, p, s);
-  else launch_rows_type<float, Mode>(rows, p, s);
+  static TriPerDevice configured;
+  static std::atomic<int> registers{0};
+  const int device = configured.pending();
+  TRI_CHECK(device != -2, "rows: no current CUDA device");
+  if (device >= 0) {
+    cudaFuncAttributes attributes;
+    TRI_CUDA(cudaFuncGetAttributes(&attributes, kernel), "rows");
+    TRI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RowShared), "rows");
+    registers.store(attributes.numRegs, std::memory_order_relaxed);
+    configured.mark(device);
+  }
+  // resident CTAs per SM by threads, registers and shared memory, then the depth that the rest of the shared memory gives
+  const int row_bytes = (Mode != RowPlain && p.b != nullptr ? 2 : 1) * V * threads * 16;
+  int resident = 2048 / threads;
+  const int by_registers = 65536 / ((registers.load(std::memory_order_relaxed) + 7) / 8 * 8 * threads);
+  if (by_registers < resident) resident = by_registers;
+  if (RowShared / row_bytes < resident) resident = RowShared / row_bytes;
+  if (resident < 1) resident = 1;
+  int depth = RowShared / (resident * row_bytes);
+  if (depth > 4) depth = 4;
+  if (p.rows <= (int64_t)resident * sms) depth = 1;
+  const int64_t slots = (int64_t)resident * sms, grid = p.rows < slots ? p.rows : slots;
+  TRI_CUDA(launch_chained(kernel, dim3((unsigned)grid), dim3(threads), (size_t)depth * row_bytes, s, p, depth), "rows");
   return tri_launch_status("rows");
 }
 
-template <typename T> static void launch_values(const void* codes, int64_t codes_stride, const float* scales, int64_t rows, int width,
-                                                void* out, int64_t out_stride, cudaStream_t s) {
+template <typename T, int Mode> static int launch_rows_type(const RowArgs& p, int sms, cudaStream_t s) {
+  constexpr int N = RowVector<T>::N;
+  const auto vector_rows = [](const void* base, int64_t stride) { return aligned16(base) && stride % N == 0; };
+  const int vectors = p.width / N;
+  if (p.width % N == 0 && vector_rows(p.a, p.a_stride) && vector_rows(p.b, p.b_stride) && vector_rows(p.weight, 0) &&
+      vector_rows(p.sum, p.sum_stride) && vectors <= 4096) {
+    if constexpr (Mode != RowNorm) {
+      if (vectors <= 32) return launch_rows_kernel<T, Mode, 1, RowWarp>(p, sms, s);
+      if (vectors <= 64) return launch_rows_kernel<T, Mode, 2, RowWarp>(p, sms, s);
+    }
+    // Vectors per thread.  One while there are few rows (a trip to memory and a reduction bound the call); for long batches as
+    // many as pay for what a thread does once a row, as few as keep warps on the SM.  Measured (us, 1 / 2 / 4 vectors): norm
+    // 16384 x 3584 with residual 70 / 73 / 82, 16384 x 8192 162 / 158 / 171; gated 8192 x 4096 61 / 49 / 56, 8192 x 8192
+    // 121 / 98 / 95, 8192 x 14336 191 / 191 / 163; plain 16384 x 4096 58 / 47 / 46, 16384 x 8192 112 / 90 / 86.
+    const int want = p.rows <= 2 * sms ? 1 : Mode == RowNorm ? (vectors <= 512 ? 1 : 2) : (vectors <= 512 ? 2 : 4);
+    if (want == 1 && vectors <= 1024) return launch_rows_kernel<T, Mode, 1, RowCta>(p, sms, s);
+    if (want <= 2 && vectors <= 2048) return launch_rows_kernel<T, Mode, 2, RowCta>(p, sms, s);
+    return launch_rows_kernel<T, Mode, 4, RowCta>(p, sms, s);
+  }
+  if (p.width <= 8192 / 8 * N) return launch_rows_kernel<T, Mode, 1, RowElements>(p, sms, s);
+  if (p.width <= 16384 / 8 * N) return launch_rows_kernel<T, Mode, 2, RowElements>(p, sms, s);
+  TRI_CUDA(launch_chained(rows_general_kernel<T, Mode>, dim3((unsigned)p.rows), dim3(1024), 0, s, p), "rows");
+  return tri_launch_status("rows");
+}
+
+// SMs of the current GPU, asked for once; -1 after an error.
+static int row_sms() {
+  static std::atomic<int> counts[TriPerDevice::MaxDevices];
+  int device = -1, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= TriPerDevice::MaxDevices) { tri_set_error("rows: no current CUDA device"); return -1; }
+  n = counts[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { tri_set_error("rows: no current CUDA device"); return -1; }
+    counts[device].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+template <int Mode> static int launch_rows(int type, const RowArgs& p, cudaStream_t s) {
+  const int sms = row_sms();
+  if (sms < 0) return TRI_ERR_CUDA;
+  if (type == TRI_BF16) return launch_rows_type<__nv_bfloat16, Mode>(p, sms, s);
+  if (type == TRI_FP16) return launch_rows_type<__half, Mode>(p, sms, s);
+  return launch_rows_type<float, Mode>(p, sms, s);
+}
+
+template <typename T> static int launch_values(const void* codes, int64_t codes_stride, const float* scales, int64_t rows, int width,
+                                               void* out, int64_t out_stride, cudaStream_t s) {
   const bool vector = width % 8 == 0 && aligned16(out) && out_stride * sizeof(T) % 16 == 0;
   const int64_t blocks = (rows * (vector ? width / 8 : width) + 255) / 256;
-  const unsigned grid = (unsigned)(blocks < 148 * 64 ? blocks : 148 * 64);
-  if (vector) dequantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<const int8_t*>(codes), codes_stride, scales, static_cast<T*>(out), out_stride, rows, width);
-  else dequantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<const int8_t*>(codes), codes_stride, scales, static_cast<T*>(out), out_stride, rows, width);
+  const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+  const int8_t* c = static_cast<const int8_t*>(codes);
+  if (vector) TRI_CUDA(launch_chained(dequantize_rows_kernel<T, true>, grid, dim3(256), 0, s, c, codes_stride, scales, static_cast<T*>(out), out_stride, rows, width), "values");
+  else TRI_CUDA(launch_chained(dequantize_rows_kernel<T, false>, grid, dim3(256), 0, s, c, codes_stride, scales, static_cast<T*>(out), out_stride, rows, width), "values");
+  return tri_launch_status("dequantize_rows");
 }
 
 }  // namespace tri
@@ -415,7 +648,7 @@ extern "C" int tri_quantize_rows(const void* x, int type, int64_t rows, int widt
   RowArgs p{};
   p.rows = rows;
   p.a = x; p.a_stride = x_stride; p.codes = static_cast<int8_t*>(codes); p.codes_stride = codes_stride; p.scales = scales; p.width = width;
-  return launch_rows<RowPlain>(type, rows, p, static_cast<cudaStream_t>(stream));
+  return launch_rows<RowPlain>(type, p, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tri_silu_mul_rows(const void* gate, const void* up, int type, int64_t rows, int width, int64_t gate_stride,
@@ -429,7 +662,7 @@ extern "C" int tri_silu_mul_rows(const void* gate, const void* up, int type, int
   p.rows = rows;
   p.a = gate; p.b = up; p.a_stride = gate_stride; p.b_stride = up_stride;
   p.codes = static_cast<int8_t*>(codes); p.codes_stride = codes_stride; p.scales = scales; p.width = width;
-  return launch_rows<RowGated>(type, rows, p, static_cast<cudaStream_t>(stream));
+  return launch_rows<RowGated>(type, p, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tri_rms_norm_rows(const void* x, const void* residual, const void* weight, int type, int64_t rows, int width,
@@ -449,8 +682,8 @@ extern "C" int tri_rms_norm_rows(const void* x, const void* residual, const void
   p.rows = rows;
   p.a = x; p.b = residual; p.weight = weight; p.a_stride = x_stride; p.b_stride = residual_stride;
   p.sum = residual_out; p.sum_stride = residual_out_stride;
-  p.codes = static_cast<int8_t*>(codes); p.codes_stride = codes_stride; p.scales = scales; p.width = width; p.eps = (float)eps;
-  return launch_rows<RowNorm>(type, rows, p, static_cast<cudaStream_t>(stream));
+  p.codes = static_cast<int8_t*>(codes); p.codes_stride = codes_stride; p.scales = scales; p.width = width; p.eps = (float)eps; p.inverse_width = 1.f / (float)width;
+  return launch_rows<RowNorm>(type, p, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tri_dequantize_rows(const void* codes, int64_t codes_stride, const float* scales, int type, int64_t rows, int width,
@@ -461,8 +694,7 @@ extern "C" int tri_dequantize_rows(const void* codes, int64_t codes_stride, cons
   TRI_CHECK(code_rows(codes, codes_stride, width), "dequantize_rows: code rows start on 16-byte boundaries");
   TRI_CHECK(row_pointer(out, type) && out_stride >= width, "dequantize_rows: output rows");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (type == TRI_BF16) launch_values<__nv_bfloat16>(codes, codes_stride, scales, rows, width, out, out_stride, s);
-  else if (type == TRI_FP16) launch_values<__half>(codes, codes_stride, scales, rows, width, out, out_stride, s);
-  else launch_values<float>(codes, codes_stride, scales, rows, width, out, out_stride, s);
-  return tri_launch_status("dequantize_rows");
+  if (type == TRI_BF16) return launch_values<__nv_bfloat16>(codes, codes_stride, scales, rows, width, out, out_stride, s);
+  if (type == TRI_FP16) return launch_values<__half>(codes, codes_stride, scales, rows, width, out, out_stride, s);
+  return launch_values<float>(codes, codes_stride, scales, rows, width, out, out_stride, s);
 }
