@@ -447,16 +447,21 @@ class Module:
     def _launch(self, fn, index, *args):
         """fn(*args, stream) on the current stream of GPU `index`."""
         if index == torch.cuda.current_device():
-            return self._check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
-        with torch.cuda.device(index):
-            return self._check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(index):
+                status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if status < 0:
+            self._check(status)
 
     @staticmethod
     def _rows(x, name):
         """(type, GPU) of rows [T,H] with contiguous features."""
         kind, index = ROW_TYPES.get(x.dtype), x.get_device()
         if kind is None or index < 0 or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] != 1):
-            raise RuntimeError(f"{name}: rows [T,H] of bf16, fp16 or fp32 on a GPU with contiguous features")
+            width = x.shape[-1] if x.dim() else 0
+            raise RuntimeError(f"{name}: rows of 1..{MAX_WIDTH} features" if not 1 <= width <= MAX_WIDTH else
+                               f"{name}: rows [T,H] of bf16, fp16 or fp32 on a GPU with contiguous features")
         return kind, index
 
     @staticmethod
@@ -478,6 +483,18 @@ class Module:
         if scales.dtype != torch.float32 or scales.shape != (rows,) or scales.get_device() != index or not scales.is_contiguous():
             raise RuntimeError(f"{name}: float32 scales [{rows}], one a row, on the same GPU")
         return pitch
+
+    @staticmethod
+    def _norm_weight(weight, x, width):
+        if (weight.dtype != x.dtype or weight.shape != (width,) or weight.get_device() != x.get_device() or
+                (weight.stride(0) != 1 and width != 1)):
+            raise RuntimeError("norm weight [H] of the type and on the device of x")
+
+    @staticmethod
+    def _bias(bias, out, outputs):
+        if (bias.dtype != out.dtype or bias.shape != (outputs,) or bias.get_device() != out.get_device() or
+                (bias.stride(0) != 1 and outputs != 1)):
+            raise RuntimeError("bias [N] of the output's type, on its device")
 
     def quantize_rows(self, x, codes, scales):
         """codes [T,H] and scales [T] of the rows x [T,H]."""
@@ -505,8 +522,7 @@ class Module:
         rows, width = x.shape
         if codes.shape != x.shape:
             raise RuntimeError("codes have the shape of x")
-        if weight.dtype != x.dtype or weight.shape != (width,) or weight.get_device() != index or (weight.stride(0) != 1 and width != 1):
-            raise RuntimeError("norm weight [H] of the type and on the device of x")
+        self._norm_weight(weight, x, width)
         if residual is None and residual_out is None:
             self._launch(self.lib.tri_rms_norm_rows, index, x.data_ptr(), None, weight.data_ptr(), kind, rows, width, x.stride(0), 0,
                          eps, None, 0, codes.data_ptr(), pitch, scales.data_ptr())
@@ -537,9 +553,8 @@ class Module:
         width = codes.shape[1]
         if codes.shape[0] != tokens or weight.shape != (outputs, width) or outputs < 1:
             raise RuntimeError("codes [T,K], weight [N,K], out [T,N]")
-        if bias is not None and (bias.dtype != out.dtype or bias.shape != (outputs,) or bias.get_device() != index or
-                                 (bias.stride(0) != 1 and outputs != 1)):
-            raise RuntimeError("bias [N] of the output's type, on its device")
+        if bias is not None:
+            self._bias(bias, out, outputs)
         residual_stride = 0
         if residual is not None:
             self._like(residual, out, "residual")

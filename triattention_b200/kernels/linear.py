@@ -13,41 +13,74 @@ from __future__ import annotations
 
 import torch
 
-from triattention_b200.kernels.extension import MAX_WIDTH
+from triattention_b200.kernels.extension import MAX_WIDTH, ROW_TYPES
 
 CODE_ALIGN = 16     # code rows start on 16-byte boundaries
 
 
 class Int8Rows:
     """Codes int8 [..., H] and scales f32 [...]: row t stands for scales[t] * codes[t].  `dtype` is the type of the values the
-    rows were made from, which `dequantize` and `linear` give back unless they are told otherwise."""
+    rows were made from, which `dequantize` and `linear` give back unless they are told otherwise.  Those calls want code rows
+    that start on 16-byte boundaries (`H` itself may be anything).
 
-    __slots__ = ("codes", "scales", "dtype")
+    Rows that a call of `Int8Ops` made lie in one allocation, codes first; the tensors `codes` and `scales` are made when they
+    are first asked for (a call is as short as the host is, and most rows are only handed on)."""
+
+    __slots__ = ("shape", "dtype", "device", "index", "rows", "width", "pitch", "codes_ptr", "scales_ptr", "_codes", "_scales", "_buffer")
 
     def __init__(self, codes, scales, dtype=torch.bfloat16):
-        if codes.dtype != torch.int8 or scales.dtype != torch.float32 or codes.shape[:-1] != scales.shape:
+        shape = codes.shape
+        if codes.dtype != torch.int8 or scales.dtype != torch.float32 or not shape or scales.shape != shape[:-1]:
             raise RuntimeError("Int8Rows: int8 codes [..., H] and float32 scales [...]")
-        self.codes, self.scales, self.dtype = codes, scales, dtype
+        if codes.dim() != 2:
+            codes, scales = codes.reshape(-1, shape[-1]), scales.reshape(-1)
+        rows, width = codes.shape
+        index = codes.get_device()
+        pitch = codes.stride(0) if rows > 1 else -(-width // CODE_ALIGN) * CODE_ALIGN
+        pointer = codes.data_ptr()
+        if scales.get_device() != index:
+            raise RuntimeError("Int8Rows: codes and scales on one device")
+        if (not 1 <= width <= MAX_WIDTH or pointer % CODE_ALIGN or pitch % CODE_ALIGN or (width > 1 and codes.stride(1) != 1) or
+                (rows > 1 and scales.stride(0) != 1)):
+            pitch = -1      # rows that the calls refuse
+        self.shape, self.dtype, self.device, self.index = shape, dtype, codes.device, index
+        self.rows, self.width, self.pitch = rows, width, pitch
+        self.codes_ptr, self.scales_ptr = pointer, scales.data_ptr()
+        self._codes, self._scales, self._buffer = codes, scales, None
 
     @classmethod
-    def _of(cls, codes, scales, dtype):
-        self = cls.__new__(cls)     # made by a call of this file: nothing to check
-        self.codes, self.scales, self.dtype = codes, scales, dtype
+    def _empty(cls, shape, rows, width, dtype, device, index):
+        """Uninitialised rows for a call to fill."""
+        if not 1 <= width <= MAX_WIDTH:
+            raise RuntimeError(f"rows of 1..{MAX_WIDTH} features")
+        self = cls.__new__(cls)
+        pitch = -(-width // CODE_ALIGN) * CODE_ALIGN
+        self._buffer = buffer = torch.empty(rows * (pitch + 4), dtype=torch.int8, device=device)
+        self.shape, self.dtype, self.device, self.index = shape, dtype, device, index
+        self.rows, self.width, self.pitch = rows, width, pitch
+        self.codes_ptr = buffer.data_ptr()
+        self.scales_ptr = self.codes_ptr + rows * pitch
+        self._codes = self._scales = None
         return self
 
-    def _flat(self):
-        """codes [T, H] and scales [T]."""
-        if self.codes.dim() == 2:
-            return self.codes, self.scales
-        return self.codes.reshape(-1, self.codes.shape[-1]), self.scales.reshape(-1)
+    def _refuse(self, name):
+        raise RuntimeError(f"{name}: rows of 1..{MAX_WIDTH} codes that start on 16-byte boundaries, with contiguous features and "
+                           "scales, on a GPU")
+
+    def _views(self):
+        if self._codes is None:
+            end = self.rows * self.pitch
+            self._codes = self._buffer[:end].view(self.rows, self.pitch)[:, :self.width]
+            self._scales = self._buffer[end:].view(torch.float32)
+        return self._codes, self._scales
 
     @property
-    def shape(self):
-        return self.codes.shape
+    def codes(self):
+        return self._views()[0].view(self.shape)
 
     @property
-    def device(self):
-        return self.codes.device
+    def scales(self):
+        return self._views()[1].view(self.shape[:-1])
 
 
 def _flat(x):
@@ -71,75 +104,92 @@ class Int8Ops:
                     raise RuntimeError("the INT8 projections have no backward pass: call them under torch.no_grad() or "
                                        "inference_mode()")
 
-    @staticmethod
-    def _empty_codes(x):
-        """Uninitialised codes [T,H], rows a multiple of 16 bytes apart, and scales [T], for the rows x [T,H]."""
-        rows, width = x.shape
-        if not 1 <= width <= MAX_WIDTH:
-            raise RuntimeError(f"rows of 1..{MAX_WIDTH} features")
-        pitch = -(-width // CODE_ALIGN) * CODE_ALIGN
-        codes = torch.empty((rows, pitch), dtype=torch.int8, device=x.device)
-        return (codes if pitch == width else codes[:, :width]), torch.empty(rows, dtype=torch.float32, device=x.device)
-
-    @staticmethod
-    def _shaped(codes, scales, like):
-        if like.dim() != 2:
-            codes, scales = codes.view(like.shape), scales.view(like.shape[:-1])
-        return Int8Rows._of(codes, scales, like.dtype)
-
     def quantize_rows(self, x):
         """x [..., H] (bf16, fp16 or fp32) -> Int8Rows."""
         self._inference(x)
-        flat = _flat(x)
-        codes, scales = self._empty_codes(flat)
-        self.module.quantize_rows(flat, codes, scales)
-        return self._shaped(codes, scales, x)
+        m, flat = self.module, _flat(x)
+        kind, index = m._rows(flat, "x")
+        rows, width = flat.shape
+        out = Int8Rows._empty(x.shape, rows, width, x.dtype, x.device, index)
+        m._launch(m.lib.tri_quantize_rows, index, flat.data_ptr(), kind, rows, width, flat.stride(0), out.codes_ptr, out.pitch,
+                  out.scales_ptr)
+        return out
 
     def silu_mul(self, gate, up):
         """silu(gate) * up -> Int8Rows; gate and up [..., H] may be the halves of one tensor."""
         self._inference(gate, up)
         if gate.shape != up.shape:
             raise RuntimeError("gate and up have one shape")
-        flat = _flat(gate)
-        codes, scales = self._empty_codes(flat)
-        self.module.silu_mul_rows(flat, _flat(up), codes, scales)
-        return self._shaped(codes, scales, gate)
+        m, flat, other = self.module, _flat(gate), _flat(up)
+        kind, index = m._rows(flat, "gate")
+        m._like(other, flat, "up")
+        rows, width = flat.shape
+        out = Int8Rows._empty(gate.shape, rows, width, gate.dtype, gate.device, index)
+        m._launch(m.lib.tri_silu_mul_rows, index, flat.data_ptr(), other.data_ptr(), kind, rows, width, flat.stride(0),
+                  other.stride(0), out.codes_ptr, out.pitch, out.scales_ptr)
+        return out
 
     def rms_norm(self, x, weight, eps, residual=None):
         """h = x + residual (rounded to x's type); h / sqrt(mean h^2 + eps) * weight -> Int8Rows, or (Int8Rows, h) with a
         residual."""
         self._inference(x, weight, residual)
-        flat = _flat(x)
-        if residual is None:
-            codes, scales = self._empty_codes(flat)
-            self.module.rms_norm_rows(flat, weight, eps, codes, scales)
-            return self._shaped(codes, scales, x)
-        if residual.shape != x.shape:
+        if residual is not None and residual.shape != x.shape:
             raise RuntimeError("x and residual have one shape")
-        codes, scales = self._empty_codes(flat)
-        total = flat.new_empty(flat.shape)
-        self.module.rms_norm_rows(flat, weight, eps, codes, scales, _flat(residual), total)
-        return self._shaped(codes, scales, x), total if x.dim() == 2 else total.view(x.shape)
+        m, flat = self.module, _flat(x)
+        kind, index = m._rows(flat, "x")
+        rows, width = flat.shape
+        m._norm_weight(weight, flat, width)
+        if residual is None:
+            out = Int8Rows._empty(x.shape, rows, width, x.dtype, x.device, index)
+            m._launch(m.lib.tri_rms_norm_rows, index, flat.data_ptr(), None, weight.data_ptr(), kind, rows, width, flat.stride(0), 0,
+                      eps, None, 0, out.codes_ptr, out.pitch, out.scales_ptr)
+            return out
+        other = _flat(residual)
+        m._like(other, flat, "residual")
+        out = Int8Rows._empty(x.shape, rows, width, x.dtype, x.device, index)
+        total = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+        m._launch(m.lib.tri_rms_norm_rows, index, flat.data_ptr(), other.data_ptr(), weight.data_ptr(), kind, rows, width,
+                  flat.stride(0), other.stride(0), eps, total.data_ptr(), width, out.codes_ptr, out.pitch, out.scales_ptr)
+        return out, total
 
     def dequantize(self, rows, dtype=None):
         """The values that rows of codes stand for, in `dtype` (default: the type they were made from)."""
-        codes, scales = rows._flat()
-        out = torch.empty(codes.shape, dtype=dtype or rows.dtype, device=codes.device)
-        self.module.dequantize_rows(codes, scales, out)
-        return out if rows.codes.dim() == 2 else out.view(rows.shape)
+        m, out = self.module, torch.empty(rows.shape, dtype=dtype or rows.dtype, device=rows.device)
+        kind = ROW_TYPES.get(out.dtype)
+        if rows.pitch < 0 or rows.index < 0:
+            rows._refuse("dequantize")
+        if kind is None:
+            raise RuntimeError("dequantize: bf16, fp16 or fp32 values")
+        m._launch(m.lib.tri_dequantize_rows, rows.index, rows.codes_ptr, rows.pitch, rows.scales_ptr, kind, rows.rows, rows.width,
+                  out.data_ptr(), rows.width)
+        return out
 
     def linear(self, rows, weight, bias=None, residual=None, dtype=None):
         """rows [..., K] . weight [N, K]^T (both Int8Rows) + bias [N] + residual [..., N], in `dtype` (default: the type the
         rows were made from; bias and residual have it too)."""
         self._inference(bias, residual)
-        codes, scales = rows._flat()
-        if codes.dim() != 2 or weight.codes.dim() != 2:
-            raise RuntimeError("rows [..., K] and weight [N, K]")
-        flat = rows.codes.dim() == 2
-        out = torch.empty((codes.shape[0], weight.codes.shape[0]), dtype=dtype or rows.dtype, device=codes.device)
-        if residual is not None and not flat:
-            if residual.shape != rows.shape[:-1] + out.shape[1:]:
+        m, index, outputs = self.module, rows.index, weight.rows
+        if rows.pitch < 0 or index < 0:
+            rows._refuse("linear")
+        if weight.pitch < 0:
+            weight._refuse("weight")
+        if rows.width != weight.width or len(weight.shape) != 2 or weight.index != index or outputs < 1:
+            raise RuntimeError("codes [..., K] and weight [N, K] on one GPU")
+        out = torch.empty((*rows.shape[:-1], outputs), dtype=dtype or rows.dtype, device=rows.device)
+        kind = ROW_TYPES.get(out.dtype)
+        if kind is None:
+            raise RuntimeError("linear: bf16, fp16 or fp32 outputs")
+        if bias is not None:
+            m._bias(bias, out, outputs)
+        residual_ptr, residual_stride = None, 0
+        if residual is not None:
+            if residual.shape != out.shape:
                 raise RuntimeError("residual [..., N]")
             residual = _flat(residual)
-        self.module.int8_linear(codes, scales, weight.codes, weight.scales, out, bias, residual)
-        return out if flat else out.view(rows.shape[:-1] + out.shape[1:])
+            if residual.dtype != out.dtype or residual.get_device() != index or (residual.stride(1) != 1 and outputs != 1):
+                raise RuntimeError("residual of the output's type, on its device, with contiguous features")
+            residual_ptr, residual_stride = residual.data_ptr(), residual.stride(0)
+        m._launch(m.lib.tri_int8_linear, index, rows.codes_ptr, rows.pitch, rows.scales_ptr, weight.codes_ptr, weight.pitch,
+                  weight.scales_ptr, None if bias is None else bias.data_ptr(), residual_ptr, residual_stride, out.data_ptr(),
+                  outputs, kind, rows.rows, outputs, rows.width, m._error_pointer(index))
+        return out
