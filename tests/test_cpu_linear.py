@@ -121,3 +121,104 @@ def test_a_library_without_an_entry_point_asks_to_be_rebuilt(monkeypatch):
     monkeypatch.setitem(extension.SIGNATURES, "tri_not_there", [])
     with pytest.raises(RuntimeError, match="tri_not_there: rebuild"):
         load_library()
+
+
+# ---- in a model ------------------------------------------------------------------------------------------------------
+
+class ExactOps:
+    """The interface of Int8Ops without any quantisation: rows are the values themselves."""
+
+    class Rows:
+        def __init__(self, values):
+            self.values, self.shape = values, values.shape
+
+    def quantize_rows(self, x):
+        return self.Rows(x)
+
+    def silu_mul(self, gate, up):
+        return self.Rows(torch.nn.functional.silu(gate) * up)
+
+    def rms_norm(self, x, weight, eps, residual=None):
+        h = x if residual is None else x + residual
+        rows = self.Rows(h / (h.square().mean(-1, keepdim=True) + eps).sqrt() * weight)
+        return rows if residual is None else (rows, h)
+
+    def linear(self, rows, weight, bias=None, residual=None, dtype=None):
+        y = torch.nn.functional.linear(rows.values, weight.values, bias)
+        return y if residual is None else y + residual
+
+
+def toy(kind, **more):
+    import transformers
+    torch.manual_seed(0)
+    config = getattr(transformers, kind + "Config")(hidden_size=96, intermediate_size=160, num_hidden_layers=3, num_attention_heads=4,
+                                                    num_key_value_heads=2, head_dim=32, vocab_size=200, **more)
+    return getattr(transformers, kind + "ForCausalLM")(config).eval()
+
+
+@pytest.mark.parametrize("kind,more", [("Llama", {}), ("Llama", dict(attention_bias=True, mlp_bias=True)), ("Qwen2", {}), ("Mistral", {}),
+                                       ("Qwen3", {})])
+def test_wrapped_layers_compute_the_model(kind, more):
+    """Every weight, bias, norm and residual in its place: with operators that do not quantise, the wrapped model is the model.
+    fp32 sums in another order: 3 layers of products over at most 160 terms, far below 1e-4 of logits of order one."""
+    from triattention_b200.models import int8_projections
+    model = toy(kind, **more)
+    with torch.no_grad():
+        for p in model.parameters():           # (norm weights of one and biases of zero would hide a mix-up)
+            p.add_(0.1 * torch.randn_like(p))
+        ids = torch.randint(0, 200, (2, 11))
+        want = model(input_ids=ids, use_cache=False).logits
+        assert int8_projections(model, ExactOps()) is model
+        got = model(input_ids=ids, use_cache=False).logits
+        torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-4 * float(want.abs().max()))
+        # and with a cache of its own, token by token
+        out = model(input_ids=ids[:, :10], use_cache=True)
+        step = model(input_ids=ids[:, 10:], past_key_values=out.past_key_values, use_cache=True).logits
+        torch.testing.assert_close(step[:, 0], want[:, 10], rtol=1e-3, atol=1e-3 * float(want.abs().max()))
+
+
+def test_models_without_such_layers_are_refused():
+    import transformers
+    from triattention_b200.models import int8_projections
+    other = transformers.GPT2LMHeadModel(transformers.GPT2Config(n_embd=32, n_layer=1, n_head=2, vocab_size=50))
+    with pytest.raises(RuntimeError, match="no decoder layer"):
+        int8_projections(other, ExactOps())
+    with pytest.raises(RuntimeError, match="no decoder layer"):
+        int8_projections(toy("Llama", hidden_act="gelu"), ExactOps())
+    wrapped = int8_projections(toy("Llama"), ExactOps())
+    with pytest.raises(RuntimeError, match="no decoder layer"):
+        int8_projections(wrapped, ExactOps())   # once is enough
+
+
+def test_infer_flag(monkeypatch):
+    """--int8-projections wraps the model before the engine is made; without it nothing is wrapped."""
+    import sys
+    from triattention_b200 import infer
+    done = []
+
+    class Engine:
+        def __init__(self, model, *args):
+            done.append("engine")
+
+        def generate(self, *args):
+            return [1, 2]
+
+    class Tokenizer:
+        def __call__(self, *args, **kwargs):
+            import types
+            return types.SimpleNamespace(input_ids=types.SimpleNamespace(cuda=lambda: None))
+
+        def decode(self, tokens, **kwargs):
+            return "text"
+
+    monkeypatch.setattr(infer, "load_tokenizer", lambda path: Tokenizer())
+    monkeypatch.setattr(infer, "load_model", lambda path: "model")
+    monkeypatch.setattr(infer, "render_prompt", lambda *a: "")
+    monkeypatch.setattr(infer, "eos_ids", lambda *a: set())
+    monkeypatch.setattr(infer, "TriAttention", Engine)
+    monkeypatch.setattr(infer, "int8_projections", lambda model: done.append("int8"))
+    for flags, want in (([], ["engine"]), (["--int8-projections"], ["int8", "engine"])):
+        done.clear()
+        monkeypatch.setattr(sys, "argv", ["infer", "--model", "m", "--prompt", "p", *flags])
+        infer.main()
+        assert done == want

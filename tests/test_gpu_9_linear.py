@@ -370,3 +370,111 @@ def test_refusals_on_the_gpu(ops):
         ops.quantize_rows(y.clone().requires_grad_())
     with torch.no_grad():
         ops.quantize_rows(y.clone().requires_grad_())
+
+
+# ---- in a model ------------------------------------------------------------------------------------------------------
+
+class DefinedOps:
+    """The operators' definitions in float64, results in the types of Int8Ops: what the model computes with INT8 projections."""
+
+    class Rows:
+        def __init__(self, y, dtype):
+            largest = y.abs().amax(-1, keepdim=True)
+            step = torch.where(largest > 0, largest / 127, torch.ones_like(largest))
+            self.values, self.dtype, self.shape = torch.round(y / step) * step, dtype, y.shape
+
+    def quantize_rows(self, x):
+        return self.Rows(x.double(), x.dtype)
+
+    def silu_mul(self, gate, up):
+        g = gate.double()
+        return self.Rows(g * torch.sigmoid(g) * up.double(), gate.dtype)
+
+    def rms_norm(self, x, weight, eps, residual=None):
+        kept = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+        h = kept.double()
+        rows = self.Rows(h / (h.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double(), x.dtype)
+        return rows if residual is None else (rows, kept)
+
+    def linear(self, rows, weight, bias=None, residual=None, dtype=None):
+        y = rows.values @ weight.values.T
+        for more in (bias, residual):
+            if more is not None:
+                y = y + more.double()
+        return y.to(dtype or rows.dtype)
+
+
+def toy_llama():
+    from transformers import LlamaConfig, LlamaForCausalLM
+    torch.manual_seed(0)
+    cfg = LlamaConfig(hidden_size=512, intermediate_size=1000, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2,
+                      head_dim=128, vocab_size=1024, max_position_embeddings=1024, rope_theta=500000.0, attention_bias=True)
+    return LlamaForCausalLM(cfg).to(BF16).cuda().eval()
+
+
+@torch.inference_mode()
+def test_model_with_int8_projections_is_what_the_definitions_say():
+    """Both forms round at the same places, so they differ where a number lies next to a rounding border: per stage at most one
+    element in 2^13 by a bf16 step (2^-8) and one code in 2^14 by 1/127 of a row's largest element (some 4 times its root mean
+    square): 3e-4 of a stage's norm.  30 stages, each worth twice its error in what follows: 2 % of the logits' norm."""
+    import copy
+    from triattention_b200.models import int8_projections
+    model = toy_llama()
+    model.set_attn_implementation("sdpa")
+    ids = torch.randint(0, 1024, (3, 50), generator=torch.Generator().manual_seed(1)).cuda()
+    plain = model(input_ids=ids, use_cache=False).logits.float()
+    defined = int8_projections(copy.deepcopy(model), DefinedOps())
+    want = defined(input_ids=ids, use_cache=False).logits.float()
+    got = int8_projections(model)(input_ids=ids, use_cache=False).logits.float()
+    assert float((got - want).norm() / want.norm()) < 0.02
+    assert float((got - plain).norm()) > 0          # (it is not the bf16 model)
+
+
+@torch.inference_mode()
+def test_generate_with_int8_projections(module):
+    """Prompt pass, eager steps and the captured step over the quantised attention: the same tokens either way, whichever of the
+    two is put into the model first."""
+    from triattention_b200.maps import per_kv_head
+    from triattention_b200.models import TriAttention, int8_projections
+    ids = torch.randint(0, 1024, (3, 150), generator=torch.Generator().manual_seed(5)).cuda()
+    rows = []
+    for first in (True, False):
+        model = toy_llama()
+        if first:
+            int8_projections(model)
+        engine = TriAttention(model, per_kv_head(["int8", "int4"], 2), max_new_tokens=20)
+        if not first:
+            int8_projections(model)
+        rows.append(engine.generate(ids, 20, eos=()))
+        assert engine.generate(ids, 20, eos=(), cuda_graph=True) == rows[-1]
+    assert rows[0] == rows[1] and all(len(r) == 20 for r in rows[0])
+    module.check_device_error()
+
+
+def test_a_first_call_inside_a_capture_is_refused(ops, monkeypatch):
+    """The error word would be allocated from the capture's pool: the call says so instead."""
+    x, w = codes_rows(2, 64, 50), codes_rows(16, 64, 51)
+    ops.linear(x, w)
+    kept = dict(ops.module._errors)
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            ops.module._errors.clear()
+            with pytest.raises(RuntimeError, match="outside of a stream capture"):
+                ops.linear(x, w)
+            ops.module._errors.update(kept)
+            out = ops.linear(x, w)
+    finally:
+        ops.module._errors.update(kept)
+    graph.replay()
+    assert torch.equal(out, ops.linear(x, w))
+
+
+@pytest.mark.skipif("torch.cuda.device_count() < 2")
+def test_on_another_device_than_the_current_one(ops):
+    x, w = codes_rows(5, 200, 52), codes_rows(70, 200, 53)
+    def move(rows):
+        codes = torch.zeros(rows.shape[0], 208, dtype=torch.int8, device="cuda:1")[:, :200]
+        return Int8Rows(codes.copy_(rows.codes), rows.scales.to("cuda:1"))
+
+    assert torch.equal(ops.linear(move(x), move(w)).cpu(), ops.linear(x, w).cpu())

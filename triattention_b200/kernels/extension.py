@@ -566,7 +566,9 @@ class Module:
         return out
 
     def _error_pointer(self, index):
-        return (self._errors[index] if index in self._errors else self.error_word(index)).data_ptr()
+        if index not in self._errors and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a GPU belongs outside of a stream capture (it allocates the error word)")
+        return self.error_word(index).data_ptr() if index not in self._errors else self._errors[index].data_ptr()
 
     # -- parity helpers --------------------------------------------------------------------------
     def qk_accumulators(self, requests, q8, q4x, k8, k4x, batch, heads_q, heads_kv, tokens):

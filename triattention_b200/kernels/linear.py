@@ -6,8 +6,8 @@ output channel, exact 32-bit integer sums (``csrc/linear.cu``), and the kernels 
 precedes a projection anyway (``csrc/rows.cu``): the root-mean-square norm with the residual's addition, the gated
 activation, or plain rows.
 
-``Int8Ops`` is the executor (it allocates, checks and calls the library, on the caller's current stream); ``Int8Linear``,
-``Int8RMSNorm``, ``Int8MLP`` and ``Int8DecoderLayer`` put it into a Hugging Face model (``models.int8_projections``).
+``Int8Ops`` is the executor (it allocates, checks and calls the library, on the caller's current stream); ``Int8Linear`` and
+``Int8DecoderLayer`` put it into a Hugging Face model (``models.int8_projections``).
 """
 from __future__ import annotations
 
@@ -193,3 +193,68 @@ class Int8Ops:
                   weight.scales_ptr, None if bias is None else bias.data_ptr(), residual_ptr, residual_stride, out.data_ptr(),
                   outputs, kind, rows.rows, outputs, rows.width, m._error_pointer(index))
         return out
+
+
+class Int8Linear(torch.nn.Module):
+    """A projection with INT8 weights (one scale per output channel).  Takes rows of codes as they are, quantises anything else.
+    The weights are plain attributes, made on the device of the layer they replace: for inference, not for saving or moving."""
+
+    def __init__(self, ops, weight, bias=None):
+        super().__init__()
+        self.ops, self.rows, self.bias_row = ops, ops.quantize_rows(weight.detach()), None if bias is None else bias.detach()
+
+    @classmethod
+    def of(cls, ops, *linears):
+        """One projection of torch.nn.Linear layers that read the same rows; their outputs come side by side."""
+        biases = [l.bias for l in linears]
+        if any(b is None for b in biases) and any(b is not None for b in biases):
+            biases = [torch.zeros_like(l.weight[:, 0]) if b is None else b for l, b in zip(linears, biases)]
+        weight = linears[0].weight if len(linears) == 1 else torch.cat([l.weight.detach() for l in linears])
+        bias = None if biases[0] is None else biases[0] if len(linears) == 1 else torch.cat([b.detach() for b in biases])
+        return cls(ops, weight, bias)
+
+    def forward(self, x, residual=None):
+        rows = self.ops.quantize_rows(x) if isinstance(x, torch.Tensor) else x
+        return self.ops.linear(rows, self.rows, bias=self.bias_row, residual=residual)
+
+
+class Int8DecoderLayer(torch.nn.Module):
+    """A decoder layer of the Llama kind (two RMS norms, q / k / v / o projections, a gated SiLU feed-forward block) whose
+    projections run on INT8 codes.  Both norms, the addition of the attention's output to the residual stream and the gated
+    activation end in the codes that the next projection reads; the down projection adds the residual stream itself.  The
+    attention in between is the model's own module, with its projections replaced: whatever attention implementation the model
+    is set to runs as before."""
+
+    def __init__(self, ops, layer):
+        super().__init__()
+        attention, mlp = layer.self_attn, layer.mlp
+        self.ops, self.self_attn = ops, attention
+        for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
+            setattr(attention, name, Int8Linear.of(ops, getattr(attention, name)))
+        self.gate_up, self.down = Int8Linear.of(ops, mlp.gate_proj, mlp.up_proj), Int8Linear.of(ops, mlp.down_proj)
+        norms = layer.input_layernorm, layer.post_attention_layernorm
+        self.norm_weights, self.eps = [n.weight.detach() for n in norms], [n.variance_epsilon for n in norms]
+        for name, value in vars(layer).items():         # what the model looks up on its layers (attention_type and the like)
+            if not name.startswith("_") and name not in self.__dict__:
+                setattr(self, name, value)
+
+    @staticmethod
+    def fits(layer):
+        """Whether `layer` is built like that."""
+        linear = lambda m: type(m) is torch.nn.Linear
+        norm = lambda m: hasattr(m, "variance_epsilon") and getattr(m, "weight", None) is not None
+        attention, mlp = getattr(layer, "self_attn", None), getattr(layer, "mlp", None)
+        return (attention is not None and mlp is not None and
+                all(linear(getattr(attention, n, None)) for n in ("q_proj", "k_proj", "v_proj", "o_proj")) and
+                all(linear(getattr(mlp, n, None)) for n in ("gate_proj", "up_proj", "down_proj")) and
+                type(getattr(mlp, "act_fn", None)).__name__ in ("SiLU", "SiLUActivation") and
+                all(norm(getattr(layer, n, None)) for n in ("input_layernorm", "post_attention_layernorm")) and
+                sum(1 for _ in layer.children()) == 4)
+
+    def forward(self, hidden_states, **kwargs):
+        ops = self.ops
+        attended = self.self_attn(hidden_states=ops.rms_norm(hidden_states, self.norm_weights[0], self.eps[0]), **kwargs)[0]
+        rows, hidden_states = ops.rms_norm(attended, self.norm_weights[1], self.eps[1], residual=hidden_states)
+        both = self.gate_up(rows)
+        inner = both.shape[-1] // 2
+        return self.down(ops.silu_mul(both[..., :inner], both[..., inner:]), residual=hidden_states)

@@ -15,6 +15,7 @@ from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
 from triattention_b200.kernels.decode import DecodeCache
 from triattention_b200.kernels.extension import LONG_TAIL_ROWS, load_extension
+from triattention_b200.kernels.linear import Int8DecoderLayer, Int8Ops
 from triattention_b200.kernels.prefill import Prefill
 from triattention_b200.maps import load_map, preset
 
@@ -57,6 +58,23 @@ def use_attention(model, name, fn):
 
     ALL_ATTENTION_FUNCTIONS[name] = attention
     model.set_attn_implementation(name)
+
+
+@torch.no_grad()
+def int8_projections(model, ops=None):
+    """Run the projections of every decoder layer on INT8 codes (kernels/linear.py): weights quantised in place, one scale per
+    output channel; activations per token.  Changes numerics, so it is off unless asked for; independent of the attention
+    implementation, before or after ``TriAttention(model, ...)``.  Embeddings, the final norm and the vocabulary projection stay
+    as they are, and so does what a model records of its own layer classes (output_hidden_states finds none).  Returns the
+    model; a model without a layer of the Llama kind (RMS norms, q / k / v / o, gated SiLU) is refused."""
+    ops = Int8Ops(load_extension()) if ops is None else ops
+    found = [(parent, name, child) for parent in model.modules() for name, child in parent.named_children()
+             if Int8DecoderLayer.fits(child)]
+    if not found:
+        raise RuntimeError("int8_projections: no decoder layer with RMS norms, q / k / v / o projections and a gated SiLU block")
+    for parent, name, child in found:
+        parent._modules[name] = Int8DecoderLayer(ops, child)
+    return model
 
 
 class TriAttention:
