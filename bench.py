@@ -648,6 +648,9 @@ def run_model(args):
         kinds = rng.permutation(np.array(["int8"] * 5 + ["int4"] * 2 + ["bf16"]))
         bands[str(layer)] = [[1, INF] if kind == "int4" else [INF, INF] for kind in kinds for _ in range(hq // hk)]
         bf16[str(layer)] = [i for i, kind in enumerate(kinds) if kind == "bf16"]
+    if args.int8_projections:
+        from triattention_b200.models import int8_projections
+        int8_projections(model)
     engine = TriAttention(model, from_bands(bands, model, bf16), max_new_tokens=new + 1)
     ids = torch.randint(0, cfg.vocab_size, (batch, prompt), generator=torch.Generator().manual_seed(1)).cuda()
 
@@ -710,7 +713,8 @@ def run_model(args):
                    decode_share_of_graph_step=ms["decode"] / max(1, few - 1) / (graph_s * 1e3 / (new - 1)),
                    by_call_ms={k: round(v, 3) for k, v in ms.items()})
     print(json.dumps(dict(metric="generate_tokens_per_s", value=batch * (new - 1) / graph_s, unit="tokens/s", n_gpus=1,
-                          higher_is_better=True, dtype="bf16 model, int8 / int4 / bf16 KV cache", data="synthetic",
+                          higher_is_better=True, data="synthetic",
+                          dtype=("int8 projections, " if args.int8_projections else "") + "bf16 model, int8 / int4 / bf16 KV cache",
                           config=dict(workload=f"end to end C4: random-init Llama-3.2-3B architecture, batch {batch} x {prompt} prompt "
                                                f"tokens, {new} greedy new tokens, per-layer map 5 INT8 / 2 INT4 / 1 BF16 KV heads"),
                           prompt_tokens_per_s=batch * prompt / prefill_s, prompt_pass_s=prefill_s,
@@ -750,6 +754,9 @@ def main():
                              "131072 cached tokens, 13.5 GB per step), prefill = config 3, model = config 4 end to end "
                              "through the Hugging Face hook: secondary metrics")
     parser.add_argument("--new-tokens", type=int, default=128, help="greedy new tokens of the model workload")
+    parser.add_argument("--int8-projections", action="store_true",
+                        help="model workload: the decoder layers' matrix products on INT8 codes too (other numerics than the "
+                             "configuration's bf16 model; said in the line)")
     parser.add_argument("--tokens", type=int, default=16384, help="prompt length of the prefill workload")
     parser.add_argument("--gpus", type=int, default=1)
     parser.add_argument("--steps", type=int, default=200)
