@@ -32,21 +32,21 @@ class Int8Rows:
         shape = codes.shape
         if codes.dtype != torch.int8 or scales.dtype != torch.float32 or not shape or scales.shape != shape[:-1]:
             raise RuntimeError("Int8Rows: int8 codes [..., H] and float32 scales [...]")
-        if codes.dim() != 2:
+        self.shape, self.dtype, self.device, self.index = shape, dtype, codes.device, codes.get_device()
+        if len(shape) != 2:
             codes, scales = codes.reshape(-1, shape[-1]), scales.reshape(-1)
-        rows, width = codes.shape
-        index = codes.get_device()
-        pitch = codes.stride(0) if rows > 1 else -(-width // CODE_ALIGN) * CODE_ALIGN
-        pointer = codes.data_ptr()
-        if scales.get_device() != index:
-            raise RuntimeError("Int8Rows: codes and scales on one device")
-        if (not 1 <= width <= MAX_WIDTH or pointer % CODE_ALIGN or pitch % CODE_ALIGN or (width > 1 and codes.stride(1) != 1) or
-                (rows > 1 and scales.stride(0) != 1)):
+            shape = codes.shape
+        self.rows, self.width = rows, width = shape
+        self.codes_ptr, self.scales_ptr = pointer, _ = codes.data_ptr(), scales.data_ptr()
+        pitch, feature = codes.stride()
+        if rows <= 1:
+            pitch = -(-width // CODE_ALIGN) * CODE_ALIGN
+        if (not 1 <= width <= MAX_WIDTH or pointer % CODE_ALIGN or pitch % CODE_ALIGN or (width > 1 and feature != 1) or
+                (rows > 1 and not scales.is_contiguous())):
             pitch = -1      # rows that the calls refuse
-        self.shape, self.dtype, self.device, self.index = shape, dtype, codes.device, index
-        self.rows, self.width, self.pitch = rows, width, pitch
-        self.codes_ptr, self.scales_ptr = pointer, scales.data_ptr()
-        self._codes, self._scales, self._buffer = codes, scales, None
+        self.pitch, self._codes, self._scales, self._buffer = pitch, codes, scales, None
+        if scales.get_device() != self.index:
+            raise RuntimeError("Int8Rows: codes and scales on one device")
 
     @classmethod
     def _empty(cls, shape, rows, width, dtype, device, index):
@@ -147,15 +147,15 @@ class Int8Ops:
         other = _flat(residual)
         m._like(other, flat, "residual")
         out = Int8Rows._empty(x.shape, rows, width, x.dtype, x.device, index)
-        total = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+        total = torch.empty_like(x) if x.is_contiguous() else x.new_empty(*x.shape)
         m._launch(m.lib.tri_rms_norm_rows, index, flat.data_ptr(), other.data_ptr(), weight.data_ptr(), kind, rows, width,
                   flat.stride(0), other.stride(0), eps, total.data_ptr(), width, out.codes_ptr, out.pitch, out.scales_ptr)
         return out, total
 
     def dequantize(self, rows, dtype=None):
         """The values that rows of codes stand for, in `dtype` (default: the type they were made from)."""
-        m, out = self.module, torch.empty(rows.shape, dtype=dtype or rows.dtype, device=rows.device)
-        kind = ROW_TYPES.get(out.dtype)
+        dtype = dtype or rows.dtype
+        m, out, kind = self.module, torch.empty(*rows.shape, dtype=dtype, device=rows.device), ROW_TYPES.get(dtype)
         if rows.pitch < 0 or rows.index < 0:
             rows._refuse("dequantize")
         if kind is None:
@@ -175,8 +175,9 @@ class Int8Ops:
             weight._refuse("weight")
         if rows.width != weight.width or len(weight.shape) != 2 or weight.index != index or outputs < 1:
             raise RuntimeError("codes [..., K] and weight [N, K] on one GPU")
-        out = torch.empty((*rows.shape[:-1], outputs), dtype=dtype or rows.dtype, device=rows.device)
-        kind = ROW_TYPES.get(out.dtype)
+        dtype = dtype or rows.dtype
+        shape = (rows.rows, outputs) if len(rows.shape) == 2 else (*rows.shape[:-1], outputs)
+        out, kind = torch.empty(*shape, dtype=dtype, device=rows.device), ROW_TYPES.get(dtype)
         if kind is None:
             raise RuntimeError("linear: bf16, fp16 or fp32 outputs")
         if bias is not None:
