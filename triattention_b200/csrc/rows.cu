@@ -48,20 +48,24 @@ struct RowArgs {
 // Largest magnitude as the bits of |y|: an integer maximum, so that a NaN (whose bits lie above every number's) survives.
 __device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
 
-// Maximum (and, for the norm, sum) over the CTA; every thread gets both.
-template <bool Sum> __device__ __forceinline__ void row_reduce(float& sum, uint32_t& peak, float* sums, uint32_t* peaks) {
+// Maximum (and, for the norm, sum) over the CTA; every thread gets both.  One barrier: consecutive calls use the two halves of the
+// arrays in turn, and a warp that writes a half again has passed the barrier of the call between.
+struct RowShare {
+  float sums[2][32];
+  uint32_t peaks[2][32];
+};
+template <bool Sum> __device__ __forceinline__ void row_reduce(float& sum, uint32_t& peak, RowShare& share, uint32_t turn) {
   peak = __reduce_max_sync(0xffffffffu, peak);
   if (Sum)
 #pragma unroll
     for (int bit = 16; bit > 0; bit >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, bit);
   const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (warps == 1) return;
-  __syncthreads();                    // the arrays may still be read from the call before
-  if (lane == 0) { if (Sum) sums[warp] = sum; peaks[warp] = peak; }
+  if (lane == 0) { if (Sum) share.sums[turn][warp] = sum; share.peaks[turn][warp] = peak; }
   __syncthreads();
-  peak = __reduce_max_sync(0xffffffffu, lane < warps ? peaks[lane] : 0u);
+  peak = __reduce_max_sync(0xffffffffu, lane < warps ? share.peaks[turn][lane] : 0u);
   if (Sum) {
-    sum = lane < warps ? sums[lane] : 0.f;
+    sum = lane < warps ? share.sums[turn][lane] : 0.f;
 #pragma unroll
     for (int bit = 16; bit > 0; bit >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, bit);
   }
@@ -118,8 +122,7 @@ __device__ __forceinline__ float row_element(const RowArgs& p, const T* a, const
 }
 
 // ---- general form: one CTA per row, two passes over it (the second from cache), any width and alignment ------------------
-template <typename T, int Mode> __device__ __noinline__ void row_general(const RowArgs& p, int64_t row, bool summed, float* sums,
-                                                                         uint32_t* peaks) {
+template <typename T, int Mode> __device__ __noinline__ void row_general(const RowArgs& p, int64_t row, bool summed, RowShare& share) {
   const int threads = blockDim.x;
   const T* a = static_cast<const T*>(p.a) + row * p.a_stride;
   const T* b = p.b == nullptr ? nullptr : static_cast<const T*>(p.b) + row * p.b_stride;
@@ -133,7 +136,8 @@ template <typename T, int Mode> __device__ __noinline__ void row_general(const R
     squares = 0.f; peak = 0;
     for (int e = threadIdx.x; e < p.width; e += threads)
       peak = max(peak, magnitude(row_element<T, Mode>(p, a, b, sum, e, shift, squares)));
-    row_reduce<Mode == RowNorm>(squares, peak, sums, peaks);
+    __syncthreads();                  // (a call before this one may have used the same half)
+    row_reduce<Mode == RowNorm>(squares, peak, share, attempt);
     if (Mode == RowNorm && sum != nullptr) { a = sum; b = nullptr; sum = nullptr; }   // from here on h is read (a thread reads
                                                                                       // what it wrote; residual may be gone)
     if (Mode != RowNorm || squares_fit(squares) || (squares == 0.f && peak == 0)) break;
@@ -149,11 +153,10 @@ template <typename T, int Mode> __device__ __noinline__ void row_general(const R
 }
 
 template <typename T, int Mode> __global__ void __launch_bounds__(1024) rows_general_kernel(const RowArgs p) {
-  __shared__ float sums[32];
-  __shared__ uint32_t peaks[32];
+  __shared__ RowShare share;
   grid_launch_dependents();
   grid_dependency_wait();
-  row_general<T, Mode>(p, blockIdx.x, false, sums, peaks);
+  row_general<T, Mode>(p, blockIdx.x, false, share);
 }
 
 // ---- rows held in registers ---------------------------------------------------------------------------------------------
@@ -171,7 +174,7 @@ constexpr float GatedNear = 3e-6f, GatedFar = 1.2e-5f, GateNear = -16.f;
 constexpr float PlainError = 5e-7f;     // y * (1/s) against y / s: 2^-23 for the reciprocal, 2^-24 for product and quotient each, 2^-22
 constexpr float Round = 12582912.f;     // 1.5 * 2^23: x + Round has rint(x) in its low bits
 
-enum RowLayout : int { RowCta = 0, RowWarp = 1, RowElements = 2 };
+enum RowLayout : int { RowCta = 0, RowFull = 1, RowWarp = 2, RowElements = 3 };
 
 // max(|a|, |b|, |c|); NaN where any is.
 __device__ __forceinline__ float max_magnitude(float a, float b, float c) {
@@ -211,8 +214,13 @@ __device__ __forceinline__ float2 gated_fast2(float2 g, float2 u) {
   return mul2(mul2(g, r), u);
 }
 __device__ __forceinline__ float gated_fast(float g, float u) { return gated_fast2(both(g), both(u)).x; }
-__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+__device__ __forceinline__ void copy_async(uint32_t to, const char* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared(uint32_t from) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+  return v;
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copy_wait(int pending) {      // until at most `pending` of this thread's groups are under way
@@ -261,65 +269,75 @@ template <typename T> struct RowVector {
   }
 };
 
-// One gated element in IEEE arithmetic, for the few that need it.
-template <typename T> __device__ __noinline__ float gated_exact(const T* gate, const T* up, int e) {
-  return gated(row_to_float(gate[e]), row_to_float(up[e]));
+// The same out of line, for the few elements that need it.
+__device__ __noinline__ float gated_exact(float gate, float up) { return gated(gate, up); }
+template <typename T> __device__ __forceinline__ float load_shared_element(uint32_t from) {
+  if constexpr (sizeof(T) == 4) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(from) : "memory");
+    return v;
+  } else {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+    return row_to_float(*reinterpret_cast<const T*>(&v));
+  }
 }
 
 // RowCta: inputs start on 16-byte boundaries and hold whole vectors; a CTA per row, gridDim.x rows at a time, `depth` rows in
-// shared memory.  RowWarp: the same for short rows, a warp per row, four per CTA.  RowElements: any alignment and width, a CTA
-// per row, single elements.
+// shared memory.  RowFull: the same where every thread has all of its vectors.  RowWarp: for short rows, a warp per row, four
+// per CTA.  RowElements: any alignment and width, a CTA per row, single elements.
 template <typename T, int Mode, int V, int Layout> __global__ void __launch_bounds__(Layout == RowWarp ? 128 : 1024)
     rows_kernel(const RowArgs p, int depth) {
   constexpr int N = RowVector<T>::N;
-  extern __shared__ uint4 ring[];       // RowCta: [depth][a, b][V][thread]
-  __shared__ float sums[32];
-  __shared__ uint32_t peaks[32];
-  __shared__ uint32_t exact_peak;
+  constexpr bool Ring = Layout == RowCta || Layout == RowFull, Full = Layout == RowFull;
+  extern __shared__ uint4 ring[];       // [depth][a, b][V][thread]
+  __shared__ RowShare share;
   grid_launch_dependents();
   grid_dependency_wait();
   const int threads = Layout == RowWarp ? 32 : blockDim.x, me = Layout == RowWarp ? threadIdx.x % 32 : threadIdx.x;
   const int64_t first = Layout == RowWarp ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
   const int64_t stride = Layout == RowWarp ? (int64_t)gridDim.x * 4 : gridDim.x;
   const int vectors = p.width / N;      // (not RowElements)
-  const bool two = Mode != RowPlain && p.b != nullptr;
-  const T *a0 = static_cast<const T*>(p.a), *b0 = static_cast<const T*>(p.b);
+  const bool two = Mode == RowGated || (Mode == RowNorm && p.b != nullptr);
   const auto element = [&](int j, int i) { return Layout == RowElements ? (j * N + i) * threads + me : (j * threads + me) * N + i; };
+  const auto mine = [&](int j) { return Full || j * threads + me < vectors; };     // whether this thread has a j-th vector
+  const auto row_a = [&](int64_t row) { return static_cast<const T*>(p.a) + row * p.a_stride; };
+  const auto row_b = [&](int64_t row) { return static_cast<const T*>(p.b) + row * p.b_stride; };
 
-  const int parts = two ? 2 : 1;
-  const auto slot = [&](int d, int part, int j) { return ring + ((d * parts + part) * V + j) * threads + me; };
-  const auto prefetch = [&](int d, int64_t row) {
-    if (row < p.rows) {
-      const uint4 *a = reinterpret_cast<const uint4*>(a0 + row * p.a_stride), *b = reinterpret_cast<const uint4*>(b0 + row * p.b_stride);
+  // Every address below is a start that advances by row plus j * `step` bytes, on both sides of the copies: with products worked
+  // out per vector the address arithmetic was a third of all instructions.
+  const int step = threads * 16, slot_bytes = (two ? 2 : 1) * V * step;
+  const uint32_t ring_start = smem_u32(ring) + me * 16, ring_end = ring_start + depth * slot_bytes;
+  const char *next_a = reinterpret_cast<const char*>(row_a(first)) + me * 16, *next_b = two ? reinterpret_cast<const char*>(row_b(first)) + me * 16 : nullptr;
+  const int64_t advance_a = stride * p.a_stride * (int64_t)sizeof(T), advance_b = stride * p.b_stride * (int64_t)sizeof(T);
+  int64_t next_row = first;
+  const auto prefetch = [&](uint32_t slot) {     // the next row that has not been asked for
+    if (next_row < p.rows) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int v = j * threads + me;
-        if (v < vectors) {
-          copy_async(slot(d, 0, j), a + v);
-          if (two) copy_async(slot(d, 1, j), b + v);
+      for (int j = 0; j < V; ++j)
+        if (mine(j)) {
+          copy_async(slot + j * step, next_a + j * step);
+          if (two) copy_async(slot + (V + j) * step, next_b + j * step);
         }
-      }
     }
     copy_commit();
+    next_row += stride; next_a += advance_a; next_b += advance_b;
   };
-  if constexpr (Layout == RowCta)
-    for (int d = 0; d < depth; ++d) prefetch(d, first + d * stride);
+  if constexpr (Ring)
+    for (uint32_t slot = ring_start; slot < ring_end; slot += slot_bytes) prefetch(slot);
   RowVector<T> vw[V];                   // norm: this thread's part of the weight, which every row needs
-  if constexpr (Mode == RowNorm && Layout == RowCta && V <= 2) {
+  if constexpr (Mode == RowNorm && Ring && V <= 2) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int v = j * threads + me;
-      vw[j].raw = v < vectors ? __ldg(reinterpret_cast<const uint4*>(p.weight) + v) : make_uint4(0, 0, 0, 0);
-    }
+    for (int j = 0; j < V; ++j) vw[j].raw = mine(j) ? __ldg(reinterpret_cast<const uint4*>(p.weight) + j * threads + me) : make_uint4(0, 0, 0, 0);
   }
 
-  int turn = 0;                         // ring slot of the current row
-  for (int64_t row = first; row < p.rows; row += stride) {
-    const T *a = a0 + row * p.a_stride, *b = b0 + row * p.b_stride;
-    T* sum = Mode == RowNorm && two ? static_cast<T*>(p.sum) + row * p.sum_stride : nullptr;
+  uint32_t slot = ring_start, parity = 0;
+  int8_t* codes = p.codes + first * p.codes_stride + (Layout == RowElements ? me : me * N);
+  char* sum = Mode == RowNorm && two ? reinterpret_cast<char*>(static_cast<T*>(p.sum) + first * p.sum_stride) + (Layout == RowElements ? 0 : me * 16) : nullptr;
+  const int64_t advance_codes = stride * p.codes_stride, advance_sum = stride * p.sum_stride * (int64_t)sizeof(T);
+  for (int64_t row = first; row < p.rows; row += stride, codes += advance_codes, sum += advance_sum, parity ^= 1) {
     float y[V][N], squares = 0.f, largest = 0.f, lowest = 0.f;   // lowest: of the gates
-    if constexpr (Layout == RowCta) copy_wait(depth - 1);
-    if constexpr (Mode == RowGated && Layout != RowWarp) if (threadIdx.x == 0) exact_peak = 0;
+    if constexpr (Ring) copy_wait(depth - 1);
     if constexpr (Layout == RowElements) {
       float r[V][N], w[V][N];
 #pragma unroll
@@ -327,8 +345,8 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int e = min(element(j, i), p.width - 1);      // (unconditional, so that all loads are under way at once)
-          y[j][i] = row_to_float(a[e]);
-          if (two) r[j][i] = row_to_float(b[e]);
+          y[j][i] = row_to_float(row_a(row)[e]);
+          if (two) r[j][i] = row_to_float(row_b(row)[e]);
           if (Mode == RowNorm) w[j][i] = row_to_float(static_cast<const T*>(p.weight)[e]);
         }
 #pragma unroll
@@ -341,7 +359,7 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
           if (Mode == RowNorm) {
             if (two) {
               const T h = row_from_float<T>(y[j][i] + r[j][i]);
-              if (live) sum[e] = h;
+              if (live) reinterpret_cast<T*>(sum)[e] = h;
               y[j][i] = row_to_float(h);
             }
             if (!live) y[j][i] = 0.f;
@@ -355,18 +373,16 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
       float2 squares2 = both(0.f);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int v = j * threads + me;
-        if constexpr (Layout == RowCta) {
-          va[j].raw = v < vectors ? *slot(turn, 0, j) : make_uint4(0, 0, 0, 0);
-          if (two) vb[j].raw = v < vectors ? *slot(turn, 1, j) : make_uint4(0, 0, 0, 0);
+        if constexpr (Ring) {
+          va[j].raw = mine(j) ? load_shared(slot + j * step) : make_uint4(0, 0, 0, 0);
+          if (two) vb[j].raw = mine(j) ? load_shared(slot + (V + j) * step) : make_uint4(0, 0, 0, 0);
         } else {
-          va[j].raw = v < vectors ? __ldcs(reinterpret_cast<const uint4*>(a) + v) : make_uint4(0, 0, 0, 0);
-          if (two) vb[j].raw = v < vectors ? __ldcs(reinterpret_cast<const uint4*>(b) + v) : make_uint4(0, 0, 0, 0);
+          va[j].raw = mine(j) ? __ldcs(reinterpret_cast<const uint4*>(row_a(row)) + j * threads + me) : make_uint4(0, 0, 0, 0);
+          if (two) vb[j].raw = mine(j) ? __ldcs(reinterpret_cast<const uint4*>(row_b(row)) + j * threads + me) : make_uint4(0, 0, 0, 0);
         }
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int v = j * threads + me;
         va[j].unpack(y[j]);
         if (two) {
           float r[N];
@@ -387,11 +403,11 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
             RowVector<T> h;
             h.pack(y[j]);
             h.unpack(y[j]);
-            if (v < vectors) reinterpret_cast<uint4*>(sum)[v] = h.raw;
+            if (mine(j)) *reinterpret_cast<uint4*>(sum + j * step) = h.raw;
           }
         }
         if constexpr (Mode == RowNorm) {
-          if constexpr (Layout != RowCta || V > 2) vw[j].raw = v < vectors ? __ldg(reinterpret_cast<const uint4*>(p.weight) + v) : make_uint4(0, 0, 0, 0);
+          if constexpr (!Ring || V > 2) vw[j].raw = mine(j) ? __ldg(reinterpret_cast<const uint4*>(p.weight) + j * threads + me) : make_uint4(0, 0, 0, 0);
           float w[N];
           vw[j].unpack(w);
 #pragma unroll
@@ -409,54 +425,49 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
 #pragma unroll
       for (int i = 0; i < N; i += 2) largest = max_magnitude(largest, y[j][i], y[j][i + 1]);
     const float error = Mode == RowPlain ? PlainError : lowest < GateNear ? GatedFar : GatedNear;
-    const auto advance = [&] {          // the slot takes the row `depth` turns ahead
-      if constexpr (Layout == RowCta) {
-        prefetch(turn, row + depth * stride);
-        turn = turn + 1 == depth ? 0 : turn + 1;
-      }
-    };
-    // (the row's inputs are in registers; a gated row looks a few of them up again below, in its slot if it can wait that long)
-    const bool keep = Mode == RowGated && Layout == RowCta && depth > 1;
-    if (!keep) advance();
     uint32_t peak = __float_as_uint(largest);
-    if constexpr (Layout == RowWarp) {
-      peak = __reduce_max_sync(0xffffffffu, peak);
-    } else {
-      row_reduce<Mode == RowNorm>(squares, peak, sums, peaks);
-    }
-    if constexpr (Mode == RowNorm) {
-      if (!squares_fit(squares) && !(squares == 0.f && peak == 0)) {      // (the same for the whole CTA)
-        row_general<T, Mode>(p, row, two, sums, peaks);
-        continue;
-      }
-    }
     if constexpr (Mode == RowGated) {
-      if (peak != 0 && peak < 0x7f800000u) {
-        const float bar = __uint_as_float(peak) * (1.f - 2.f * GatedFar);
+      // This warp's largest y in IEEE arithmetic: of the few elements (one, nearly always) that may be it.
+      const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, peak)), bar = top * (1.f - 2.f * GatedFar);
+      if (top > 0.f && top < CUDART_INF_F) {
         uint32_t exact = 0;
         if (largest >= bar) {
 #pragma unroll
           for (int j = 0; j < V; ++j)
 #pragma unroll
             for (int i = 0; i < N; ++i)
-              if (fabsf(y[j][i]) >= bar)
-                exact = max(exact, magnitude(keep ? gated_exact(reinterpret_cast<const T*>(slot(turn, 0, j)), reinterpret_cast<const T*>(slot(turn, 1, j)), i)
-                                                  : gated_exact(a, b, element(j, i))));
+              if (fabsf(y[j][i]) >= bar) {
+                float g, u;
+                if constexpr (Ring) {
+                  g = load_shared_element<T>(slot + j * step + i * (int)sizeof(T));
+                  u = load_shared_element<T>(slot + (V + j) * step + i * (int)sizeof(T));
+                } else {
+                  g = row_to_float(row_a(row)[element(j, i)]);
+                  u = row_to_float(row_b(row)[element(j, i)]);
+                }
+                exact = max(exact, magnitude(gated_exact(g, u)));
+              }
         }
-        if constexpr (Layout == RowWarp) {
-          peak = __reduce_max_sync(0xffffffffu, exact);
-        } else {
-          if (exact != 0) atomicMax(&exact_peak, exact);
-          __syncthreads();
-          peak = exact_peak;
-        }
+        peak = exact;
       }
     }
-    if (keep) advance();
+    if constexpr (Ring) {               // the row's inputs are in registers: its slot takes the row `depth` turns ahead
+      prefetch(slot);
+      slot += slot_bytes;
+      if (slot == ring_end) slot = ring_start;
+    }
+    if constexpr (Layout == RowWarp) peak = __reduce_max_sync(0xffffffffu, peak);
+    else row_reduce<Mode == RowNorm>(squares, peak, share, parity);
+    if constexpr (Mode == RowNorm) {
+      if (!squares_fit(squares) && !(squares == 0.f && peak == 0)) {      // (the same for the whole CTA)
+        row_general<T, Mode>(p, row, two, share);
+        __syncthreads();                // (it leaves either half in use)
+        continue;
+      }
+    }
     const RowScale r = row_scale<Mode>(peak, squares, p.eps, p.inverse_width, 1.f);
     if (me == 0) p.scales[row] = r.scale;
     const float inverse = r.inverse;
-    int8_t* codes = p.codes + row * p.codes_stride;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       uint32_t c[N];
@@ -477,62 +488,63 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
         for (int i = 0; i < N; ++i) {
           const float q = y[j][i] * inverse, from = fabsf(q - (q + Round - Round));
           if (fmaf(fabsf(q), error, from) >= 0.5f) {
-            const float exact = Mode == RowGated ? gated_exact(a, b, element(j, i)) : y[j][i];
+            const float exact = Mode == RowGated ? gated_exact(row_to_float(row_a(row)[element(j, i)]), row_to_float(row_b(row)[element(j, i)])) : y[j][i];
             c[i] = (uint32_t)__float2int_rn(exact / r.scale);
           }
         }
       }
       if constexpr (Layout == RowElements) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) if (element(j, i) < p.width) codes[element(j, i)] = r.live ? (int8_t)c[i] : (int8_t)0;
-      } else {
-        const int v = j * threads + me;
-        if (v < vectors) {
-          uint32_t w[N / 4];
+        for (int i = 0; i < N; ++i) if (element(j, i) < p.width) codes[(j * N + i) * threads] = r.live ? (int8_t)c[i] : (int8_t)0;
+      } else if (mine(j)) {
+        uint32_t w[N / 4];
 #pragma unroll
-          for (int k = 0; k < N / 4; ++k)
-            w[k] = r.live ? __byte_perm(__byte_perm(c[4 * k], c[4 * k + 1], 0x0040), __byte_perm(c[4 * k + 2], c[4 * k + 3], 0x0040), 0x5410) : 0u;
-          if constexpr (N == 8) reinterpret_cast<uint2*>(codes)[v] = make_uint2(w[0], w[1]);
-          else reinterpret_cast<uint32_t*>(codes)[v] = w[0];
-        }
+        for (int k = 0; k < N / 4; ++k)
+          w[k] = r.live ? __byte_perm(__byte_perm(c[4 * k], c[4 * k + 1], 0x0040), __byte_perm(c[4 * k + 2], c[4 * k + 3], 0x0040), 0x5410) : 0u;
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(codes + j * threads * N) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(codes + j * threads * N) = w[0];
       }
     }
   }
 }
 
-// out = scale * code.  One thread per 8 codes where the output rows allow 16-byte stores, else per element.
+// out = scale * code.  blockDim.x threads per row, blockDim.y rows per CTA at a time; a thread takes the codes of 16 bytes of
+// output where the output rows allow that (neighbouring threads then write neighbouring 16 bytes; 32 bytes a thread were 7 %
+// slower), else single ones.  Bound by HBM (the writes): no index is divided, a row's scale is read once.
 template <typename T, bool Vector> __global__ void __launch_bounds__(256) dequantize_rows_kernel(const int8_t* codes, int64_t codes_stride,
     const float* scales, T* out, int64_t out_stride, int64_t rows, int width) {
-  constexpr int N = Vector ? 8 : 1;
   grid_launch_dependents();
   grid_dependency_wait();
-  const int per_row = width / N;
-  const int64_t total = rows * per_row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = total <= 0x7fffffff ? (uint32_t)i / (uint32_t)per_row : i / per_row;
-    const int e = (int)(i - row * per_row) * N;
+  for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < rows; row += (int64_t)gridDim.x * blockDim.y) {
     const float scale = scales[row];
+    const int8_t* from = codes + row * codes_stride;
+    T* to = out + row * out_stride;
     if constexpr (!Vector) {
-      out[row * out_stride + e] = row_from_float<T>((float)codes[row * codes_stride + e] * scale);
+#pragma unroll 4
+      for (int e = threadIdx.x; e < width; e += blockDim.x) to[e] = row_from_float<T>((float)from[e] * scale);
     } else {
-      const uint2 c = *reinterpret_cast<const uint2*>(codes + row * codes_stride + e);
-      float x[8];
+      constexpr int N = RowVector<T>::N;
+#pragma unroll 4
+      for (int e = N * threadIdx.x; e < width; e += N * blockDim.x) {
+        uint32_t w[N / 4];
+        if constexpr (N == 8) {
+          const uint2 c = __ldcs(reinterpret_cast<const uint2*>(from + e));
+          w[0] = c.x; w[1] = c.y;
+        } else {
+          w[0] = __ldcs(reinterpret_cast<const uint32_t*>(from + e));
+        }
+        float x[N];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = (float)(int8_t)((k < 4 ? c.x : c.y) >> (8 * (k & 3))) * scale;
-      uint4* to = reinterpret_cast<uint4*>(out + row * out_stride + e);
-      if constexpr (sizeof(T) == 4) {
-        to[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-        to[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
-      } else {
+        for (int i = 0; i < N; ++i) x[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4))) * scale;
         RowVector<T> v;
         v.pack(x);
-        to[0] = v.raw;
+        *reinterpret_cast<uint4*>(to + e) = v.raw;
       }
     }
   }
 }
 
-// One call of rows_kernel with as many CTAs as are resident at once (RowCta) or as the rows need.
+// One call of rows_kernel with as many CTAs as are resident at once (RowCta, RowFull) or as the rows need.
 template <typename T, int Mode, int V, int Layout> static int launch_rows_kernel(const RowArgs& p, int sms, cudaStream_t s) {
   constexpr int N = RowVector<T>::N;
   const auto kernel = rows_kernel<T, Mode, V, Layout>;
@@ -572,6 +584,11 @@ template <typename T, int Mode, int V, int Layout> static int launch_rows_kernel
   return tri_launch_status("rows");
 }
 
+template <typename T, int Mode, int V> static int launch_rows_ring(const RowArgs& p, int sms, cudaStream_t s) {
+  if (p.width / RowVector<T>::N % (32 * V) == 0) return launch_rows_kernel<T, Mode, V, RowFull>(p, sms, s);
+  return launch_rows_kernel<T, Mode, V, RowCta>(p, sms, s);
+}
+
 template <typename T, int Mode> static int launch_rows_type(const RowArgs& p, int sms, cudaStream_t s) {
   constexpr int N = RowVector<T>::N;
   const auto vector_rows = [](const void* base, int64_t stride) { return aligned16(base) && stride % N == 0; };
@@ -584,12 +601,12 @@ template <typename T, int Mode> static int launch_rows_type(const RowArgs& p, in
     }
     // Vectors per thread.  One while there are few rows (a trip to memory and a reduction bound the call); for long batches as
     // many as pay for what a thread does once a row, as few as keep warps on the SM.  Measured (us, 1 / 2 / 4 vectors): norm
-    // 16384 x 3584 with residual 70 / 73 / 82, 16384 x 8192 162 / 158 / 171; gated 8192 x 4096 61 / 49 / 56, 8192 x 8192
-    // 121 / 98 / 95, 8192 x 14336 191 / 191 / 163; plain 16384 x 4096 58 / 47 / 46, 16384 x 8192 112 / 90 / 86.
-    const int want = p.rows <= 2 * sms ? 1 : Mode == RowNorm ? (vectors <= 512 ? 1 : 2) : (vectors <= 512 ? 2 : 4);
-    if (want == 1 && vectors <= 1024) return launch_rows_kernel<T, Mode, 1, RowCta>(p, sms, s);
-    if (want <= 2 && vectors <= 2048) return launch_rows_kernel<T, Mode, 2, RowCta>(p, sms, s);
-    return launch_rows_kernel<T, Mode, 4, RowCta>(p, sms, s);
+    // 16384 x 3584 with residual 73 / 76 / 81, 16384 x 8192 142 / 167 / 163; gated 8192 x 4096 51 / 43 / 39, 8192 x 8192
+    // 97 / 83 / 72, 8192 x 14336 146 / 147 / 129; plain 16384 x 4096 58 / 44 / 45, 16384 x 8192 116 / 83 / 79.
+    const int want = p.rows <= 2 * sms || Mode == RowNorm ? 1 : Mode == RowGated || vectors > 512 ? 4 : 2;
+    if (want == 1 && vectors <= 1024) return launch_rows_ring<T, Mode, 1>(p, sms, s);
+    if (want <= 2 && vectors <= 2048) return launch_rows_ring<T, Mode, 2>(p, sms, s);
+    return launch_rows_ring<T, Mode, 4>(p, sms, s);
   }
   if (p.width <= 8192 / 8 * N) return launch_rows_kernel<T, Mode, 1, RowElements>(p, sms, s);
   if (p.width <= 16384 / 8 * N) return launch_rows_kernel<T, Mode, 2, RowElements>(p, sms, s);
@@ -620,12 +637,16 @@ template <int Mode> static int launch_rows(int type, const RowArgs& p, cudaStrea
 
 template <typename T> static int launch_values(const void* codes, int64_t codes_stride, const float* scales, int64_t rows, int width,
                                                void* out, int64_t out_stride, cudaStream_t s) {
-  const bool vector = width % 8 == 0 && aligned16(out) && out_stride * sizeof(T) % 16 == 0;
-  const int64_t blocks = (rows * (vector ? width / 8 : width) + 255) / 256;
-  const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+  const bool vector = width % RowVector<T>::N == 0 && aligned16(out) && out_stride * sizeof(T) % 16 == 0;
+  const int items = vector ? width / RowVector<T>::N : width;
+  int across = 32;
+  while (across < 256 && across < items) across *= 2;
+  const dim3 block((unsigned)across, (unsigned)(256 / across));
+  const int64_t blocks = (rows + block.y - 1) / block.y;
+  const dim3 grid((unsigned)(blocks < 148 * 32 ? blocks : 148 * 32));
   const int8_t* c = static_cast<const int8_t*>(codes);
-  if (vector) TRI_CUDA(launch_chained(dequantize_rows_kernel<T, true>, grid, dim3(256), 0, s, c, codes_stride, scales, static_cast<T*>(out), out_stride, rows, width), "values");
-  else TRI_CUDA(launch_chained(dequantize_rows_kernel<T, false>, grid, dim3(256), 0, s, c, codes_stride, scales, static_cast<T*>(out), out_stride, rows, width), "values");
+  if (vector) TRI_CUDA(launch_chained(dequantize_rows_kernel<T, true>, grid, block, 0, s, c, codes_stride, scales, static_cast<T*>(out), out_stride, rows, width), "values");
+  else TRI_CUDA(launch_chained(dequantize_rows_kernel<T, false>, grid, block, 0, s, c, codes_stride, scales, static_cast<T*>(out), out_stride, rows, width), "values");
   return tri_launch_status("dequantize_rows");
 }
 
