@@ -9,7 +9,7 @@
 // 32 neighbouring channels of one token, which needs no alignment of the output rows.
 //   warp 0      producer: TMA copies of the weights' and tokens' 128-byte columns (128-byte swizzle, edges zero-filled)
 //   warp 1      issues the MMAs (one elected thread), accumulators alternate between two TMEM buffers
-//   warps 2-9   epilogue: TMEM -> scales, bias, residual -> global, while the next tile's MMAs run
+//   warps 2-    epilogue: TMEM -> scales, bias, residual -> global, while the next tile's MMAs run
 // A CTA takes tiles in turn (persistent).  Where there are fewer tiles than SMs the width is split over a cluster of 2, 4 or 8
 // CTAs; their integer partial sums are joined through distributed shared memory, so no workspace and no atomics are involved.
 // Every wait on a barrier is bounded; after one has run out the CTA runs through, reports it and its output is void.
@@ -20,11 +20,13 @@
 namespace tri {
 
 constexpr int LinChannels = 128, LinDepth = 128;             // channels of a CTA's tile; bytes of width per stage
-constexpr int LinEpilogueWarps = 8, LinThreads = 64 + 32 * LinEpilogueWarps;
+constexpr int LinWarps = 8, LinSmallWarps = 4;               // epilogue warps of a group, where a CTA has the SM to itself and where two
+                                                             // share it; two groups take a CTA's tiles in turn
+__host__ __device__ constexpr int lin_threads(int warps) { return 64 + 2 * 32 * warps; }
 constexpr int LinWeightBytes = LinChannels * LinDepth;
-constexpr int LinShared = 216 * 1024;                        // stages (and, after a split tile, its partial sums); also keeps
+constexpr int LinShared = 193 * 1024;                        // stages (and, after a split tile, its partial sums); also keeps
                                                              // a second CTA that allocates TMEM off the SM
-constexpr int LinSmallTile = 64, LinSharedSmall = 108 * 1024; // up to this token tile two CTAs fit on an SM (and in TMEM)
+constexpr int LinSmallTile = 64, LinSharedSmall = 97 * 1024;  // up to this token tile two CTAs fit on an SM (and in TMEM)
 constexpr int LinMaxStages = 12;
 
 struct LinearArgs {
@@ -135,77 +137,146 @@ __device__ __forceinline__ void lin_origin(const LinearArgs& p, int tile, int ch
   t0 = (sweep * p.group + within % wide) * p.token_tile;
 }
 
-// Epilogue of one tile by the epilogue warps: 128 channels from n0 on (TMEM lanes), `valid` tokens from t0 on (columns).  Two warps
-// per lane quadrant take alternate blocks of 16 tokens.  `ready` is called once, when everything that does not depend on the
-// sums is under way.
-template <typename T, typename Ready>
-__device__ __forceinline__ void lin_epilogue(const LinearArgs& p, uint32_t column, int n0, int t0, int valid, float* token_scales, Ready ready) {
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, quad = warp % 4, half = (warp - 2) / 4;
-  const int out_n = n0 + quad * 32 + lane;
-  const bool live = out_n < p.outputs;
-  const int safe_n = live ? out_n : p.outputs - 1;            // what a lane past the last channel may read
+// C neighbouring channels of one token as one access.
+template <typename T, int C> struct LinVector {
+  T v[C];
+};
+template <typename T, int C> __device__ __forceinline__ LinVector<T, C> lin_load(const T* from) {
+  LinVector<T, C> x;
+  constexpr int B = C * sizeof(T);
+  if constexpr (B == 16) *reinterpret_cast<uint4*>(x.v) = __ldcs(reinterpret_cast<const uint4*>(from));
+  else if constexpr (B == 8) *reinterpret_cast<uint2*>(x.v) = __ldcs(reinterpret_cast<const uint2*>(from));
+  else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(x.v) = __ldcs(reinterpret_cast<const uint32_t*>(from));
+  else x.v[0] = *from;
+  return x;
+}
+template <typename T, int C> __device__ __forceinline__ void lin_store(T* to, const LinVector<T, C>& x) {
+  constexpr int B = C * sizeof(T);
+  if constexpr (B == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(x.v);
+  else if constexpr (B == 8) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(x.v);
+  else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(x.v);
+  else *to = x.v[0];
+}
+
+// Epilogue of one tile by a group of Warps warps: 128 channels from n0 on (TMEM lanes), `valid` tokens from t0 on (columns).
+// The group's warps of a lane quadrant take blocks of 16 tokens x 32 channels in turn.  A lane holds one channel of 16 tokens; the scaled
+// block goes, 8 tokens at a time, through the warp's own shared memory, out of which a lane takes C neighbouring channels of a
+// token (C: what the rows of output and residual allow, 16 bytes at most), so that the residual is read and the result written in
+// wide accesses.  Two groups, because most of a tile's epilogue is latency (scales, the accumulators' barrier, TMEM, the residual):
+// they overlap those of two tiles (with a residual, 16384 x 4096 outputs of width 4096: 210 us, 249 with one group of all warps).
+// `ready` is called once, when everything that does not depend on the sums is under way.
+constexpr int LinPitch = 36, LinBlockTokens = 8, LinBlockFloats = LinBlockTokens * LinPitch;   // pitch: no two lanes on one bank either way
+template <typename T, int C, int Warps, bool Residual, typename Ready>
+__device__ __forceinline__ void lin_epilogue_as(const LinearArgs& p, uint32_t column, int n0, int t0, int valid, float* token_scales,
+                                                float* block, Ready ready) {
+  constexpr int Passes = 16 / C, Across = 32 / C;             // passes over a block's 16 tokens; lanes per token
+  constexpr int Step = 4 * Warps;                             // tokens from one block of a warp to its next
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, quad = warp % 4, member = (warp - 2) % Warps, c0 = member / 4 * 16;
+  const int first_n = n0 + quad * 32, safe_n = min(first_n + lane, p.outputs - 1);       // (what a lane past the last channel may read)
   column += (uint32_t)(quad * 32) << 16;
-  // the residual's block for the next 16 tokens is asked for while this one is worked on (the first one under the MMAs)
-  const T* residual = p.residual == nullptr ? nullptr : static_cast<const T*>(p.residual) + (int64_t)t0 * p.residual_stride + safe_n;
-  T ahead[16];
-  auto fetch = [&](int c) {
+  const int my_token = lane / Across, my_n = first_n + lane % Across * C, count = min(C, p.outputs - my_n);
+  const bool all = count >= C;
+  const int64_t out_step = C * p.out_stride, residual_step = C * p.residual_stride;      // from pass to pass
+  // the residual is asked for two blocks ahead (the first two under the MMAs): one trip to HBM outlasts a block by far
+  using Ahead = LinVector<T, C>[Residual ? Passes : 1];
+  Ahead even, odd;
+  auto fetch = [&](Ahead& ahead, int c) {
+    const T* from = static_cast<const T*>(p.residual) + (int64_t)(t0 + c + my_token) * p.residual_stride + my_n;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) ahead[j] = residual[(int64_t)min(c + j, valid - 1) * p.residual_stride];
+    for (int i = 0; i < (Residual ? Passes : 0); ++i, from += residual_step) {
+      if (c + i * C + my_token < valid) {
+        if (all) {
+          ahead[i] = lin_load<T, C>(from);
+        } else {
+#pragma unroll
+          for (int k = 0; k < C; ++k) if (k < count) ahead[i].v[k] = from[k];
+        }
+      }
+    }
   };
-  if (residual != nullptr) fetch(min(half * 16, valid - 1));
-  for (int t = tid - 64; t < valid; t += 32 * LinEpilogueWarps) token_scales[t] = p.scales[t0 + t];
-  const float sw = p.weight_scales[safe_n];
-  const float bias = p.bias != nullptr ? lin_in(static_cast<const T*>(p.bias)[safe_n]) : 0.f;
+  if (Residual && c0 < valid) fetch(even, c0);
+  if (Residual && c0 + Step < valid) fetch(odd, c0 + Step);
+  for (int t = 32 * member + lane; t < valid; t += 32 * Warps) token_scales[t] = p.scales[t0 + t];
+  const float sw = p.weight_scales[safe_n], bias = p.bias != nullptr ? lin_in(static_cast<const T*>(p.bias)[safe_n]) : 0.f;
   // token_scales of this tile are complete (and the other buffer's readers a tile behind); waits have no early exit, because
-  // the other epilogue warps count on this one at the barrier
-  asm volatile("bar.sync 1, %0;" ::"n"(32 * LinEpilogueWarps) : "memory");
+  // the group's other warps count on this one at the barrier
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + (warp - 2) / Warps), "n"(32 * Warps) : "memory");
   ready();
   tc_fence_after();
-  T* out = static_cast<T*>(p.out) + (int64_t)t0 * p.out_stride + out_n;
-  for (int c = half * 16; c < valid; c += 32) {
-    uint32_t a[16];
-    tmem_ld16(column + c, a);
-    float y[16], r[16];
-    if (residual != nullptr) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) r[j] = lin_in(ahead[j]);
-      if (c + 32 < valid) fetch(c + 32);
-    }
+  T* out = static_cast<T*>(p.out) + (int64_t)(t0 + c0 + my_token) * p.out_stride + my_n;
+  const int64_t block_step = Step * p.out_stride;
+  float* const mine = block + lane;
+  const float* const from = block + my_token * LinPitch + lane % Across * C;
+  uint32_t a[16];
+  if (c0 < valid) tmem_ld16(column + c0, a);
+  auto work = [&](Ahead& ahead, int c) {
     tmem_ld_wait();
+    T* to = out;
 #pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      const float4 st = *reinterpret_cast<const float4*>(&token_scales[c + j]);
-      y[j] = __fmul_rn(__fmul_rn((float)(int)a[j], sw), st.x);
-      y[j + 1] = __fmul_rn(__fmul_rn((float)(int)a[j + 1], sw), st.y);
-      y[j + 2] = __fmul_rn(__fmul_rn((float)(int)a[j + 2], sw), st.z);
-      y[j + 3] = __fmul_rn(__fmul_rn((float)(int)a[j + 3], sw), st.w);
+    for (int part = 0; part < 16; part += LinBlockTokens) {
+#pragma unroll
+      for (int j = 0; j < LinBlockTokens; j += 4) {
+        const float4 st = *reinterpret_cast<const float4*>(&token_scales[c + part + j]);
+        mine[j * LinPitch] = fmaf(__fmul_rn((float)(int)a[part + j], sw), st.x, bias);
+        mine[(j + 1) * LinPitch] = fmaf(__fmul_rn((float)(int)a[part + j + 1], sw), st.y, bias);
+        mine[(j + 2) * LinPitch] = fmaf(__fmul_rn((float)(int)a[part + j + 2], sw), st.z, bias);
+        mine[(j + 3) * LinPitch] = fmaf(__fmul_rn((float)(int)a[part + j + 3], sw), st.w, bias);
+      }
+      if (part + LinBlockTokens == 16 && c + Step < valid) tmem_ld16(column + c + Step, a);    // on its way while this block is written out
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < LinBlockTokens / C; ++i, to += out_step) {
+        constexpr int Skip = C * LinPitch;
+        const int pass = part / C + i;
+        float y[C];
+        if constexpr (C >= 4) {
+#pragma unroll
+          for (int k = 0; k < C; k += 4) *reinterpret_cast<float4*>(y + k) = *reinterpret_cast<const float4*>(from + i * Skip + k);
+        } else if constexpr (C == 2) {
+          *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(from + i * Skip);
+        } else {
+          y[0] = from[i * Skip];
+        }
+        LinVector<T, C> x;
+#pragma unroll
+        for (int k = 0; k < C; ++k) x.v[k] = lin_out<T>(Residual ? y[k] + lin_in(ahead[Residual ? pass : 0].v[k]) : y[k]);
+        if (c + pass * C + my_token < valid) {
+          if (all) {
+            lin_store<T, C>(to, x);
+          } else {
+#pragma unroll
+            for (int k = 0; k < C; ++k) if (k < count) to[k] = x.v[k];
+          }
+        }
+      }
+      __syncwarp();                                           // the block has been read
     }
-    if (p.bias != nullptr)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) y[j] += bias;
-    if (residual != nullptr)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) y[j] += r[j];
-    T* to = out + (int64_t)c * p.out_stride;
-    if (c + 16 <= valid) {
-      if (live)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) to[j * p.out_stride] = lin_out<T>(y[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) if (live && c + j < valid) to[j * p.out_stride] = lin_out<T>(y[j]);
-    }
+    if (Residual && c + 2 * Step < valid) fetch(ahead, c + 2 * Step);
+    out += block_step;
+  };
+  for (int c = c0; c < valid; c += 2 * Step) {
+    work(even, c);
+    if (c + Step < valid) work(odd, c + Step);
   }
   tc_fence_before();
   __syncwarp();
 }
+template <typename T, int C, int Warps, typename Ready>
+__device__ __forceinline__ void lin_epilogue(const LinearArgs& p, uint32_t column, int n0, int t0, int valid, float* token_scales,
+                                             float* blocks, Ready ready) {
+  float* block = blocks + (threadIdx.x / 32 - 2) * LinBlockFloats;
+  if (p.residual != nullptr) lin_epilogue_as<T, C, Warps, true>(p, column, n0, t0, valid, token_scales, block, ready);
+  else lin_epilogue_as<T, C, Warps, false>(p, column, n0, t0, valid, token_scales, block, ready);
+}
 
-// One CTA per tile of 128 channels.  grid = CTAs (persistent) when splits is 1, otherwise tiles * splits with one tile per cluster.
-template <typename T> __global__ void __launch_bounds__(LinThreads, 2) linear_kernel(const __grid_constant__ CUtensorMap map_w,
+// One CTA per tile of 128 channels; Small: two of them per SM.  grid = CTAs (persistent) when splits is 1, otherwise tiles * splits with one tile per cluster.
+template <typename T, int C, bool Small> __global__ void __launch_bounds__(lin_threads(Small ? LinSmallWarps : LinWarps), Small ? 2 : 1) linear_kernel(const __grid_constant__ CUtensorMap map_w,
     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearArgs p) {
   extern __shared__ uint8_t raw_smem[];
   __shared__ __align__(8) LinearBarriers bars;
-  __shared__ __align__(16) float token_scales[2][256];
+  __shared__ __align__(16) float token_scales[2][2][256];      // [group][the group's turn]
+  constexpr int Warps = Small ? LinSmallWarps : LinWarps;
+  __shared__ __align__(16) float blocks[2 * Warps * LinBlockFloats];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
@@ -216,7 +287,7 @@ template <typename T> __global__ void __launch_bounds__(LinThreads, 2) linear_ke
   const int k0 = (int)((int64_t)all_steps * rank / splits), k1 = (int)((int64_t)all_steps * (rank + 1) / splits);
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) { mbar_init(&bars.full[s], 1); mbar_init(&bars.empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&bars.done[b], 1); mbar_init(&bars.free[b], LinEpilogueWarps); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&bars.done[b], 1); mbar_init(&bars.free[b], Warps); }
     mbar_fence_init();
     abort_flag = 0;
   }
@@ -285,24 +356,32 @@ template <typename T> __global__ void __launch_bounds__(LinThreads, 2) linear_ke
       }
     }
   } else if (splits == 1) {
-    int n = 0;
-    for (int tile = first; tile < p.tiles; tile += step, ++n) {
-      const int b = n & 1;
+    if (p.tiles <= step) {                                    // one tile per CTA: all warps share it
+      if (first < p.tiles) {
+        int n0, t0;
+        lin_origin(p, first, LinChannels, n0, t0);
+        lin_epilogue<T, C, 2 * Warps>(p, tmem, n0, t0, min(bt, p.tokens - t0), token_scales[0][0], blocks,
+                                      [&] { lin_wait(smem_u32(&bars.done[0]), 0, abortp); });
+      }
+    }
+    const int b = (warp - 2) / Warps;                         // group, and the accumulator buffer that it empties
+    uint32_t turn = 0;
+    for (int tile = first + b * step; p.tiles > step && tile < p.tiles; tile += 2 * step, turn ^= 1) {
       int n0, t0;
       lin_origin(p, tile, LinChannels, n0, t0);
-      lin_epilogue<T>(p, tmem + b * buffer, n0, t0, min(bt, p.tokens - t0), token_scales[b],
-                      [&] { lin_wait(smem_u32(&bars.done[b]), (n >> 1) & 1, abortp); });
+      lin_epilogue<T, C, Warps>(p, tmem + b * buffer, n0, t0, min(bt, p.tokens - t0), token_scales[b][turn], blocks,
+                      [&] { lin_wait(smem_u32(&bars.done[b]), turn, abortp); });
       if (lane == 0) lin_arrive(&bars.free[b]);
     }
   } else {                                                    // one tile per cluster: this CTA's partial sums, [token][channel]
-    const int quad = warp % 4, half = (warp - 2) / 4, channel = quad * 32 + lane;
+    const int quad = warp % 4, channel = quad * 32 + lane;
     int n0, t0;
     lin_origin(p, first, LinChannels, n0, t0);
     const int valid = min(bt, p.tokens - t0);
     lin_wait(smem_u32(&bars.done[0]), 0, abortp);
     tc_fence_after();
     int* partial = reinterpret_cast<int*>(smem);
-    for (int c = half * 16; c < valid; c += 32) {
+    for (int c = (warp - 2) / 4 * 16; c < valid; c += 8 * Warps) {
       uint32_t a[16];
       tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + c, a);
       tmem_ld_wait();
@@ -325,7 +404,7 @@ template <typename T> __global__ void __launch_bounds__(LinThreads, 2) linear_ke
     __syncwarp();
     cluster_sync_all();
     const uint32_t partial = smem_base + lane * 16;
-    for (int t = rank + warp * splits; t < valid; t += splits * (LinThreads / 32)) {
+    for (int t = rank + warp * splits; t < valid; t += splits * (lin_threads(Warps) / 32)) {
       const float st = p.scales[t0 + t];
       float r[4] = {};
       if (p.residual != nullptr) {
@@ -361,11 +440,12 @@ template <typename T> __global__ void __launch_bounds__(LinThreads, 2) linear_ke
 // (cta_group::2).  Each CTA holds its own 128 channels and half of the tokens, so an SM fetches 32 KB per 128 bytes of width
 // where a CTA alone fetches 48 KB for the same work, and the SM's port to L2 is what bounds the product of two large operands.
 // The even CTA issues the MMAs of both; copies of both report to its `full` barriers, commits arrive at both CTAs' barriers.
-template <typename T> __global__ void __launch_bounds__(LinThreads, 1) linear_pair_kernel(const __grid_constant__ CUtensorMap map_w,
+template <typename T, int C> __global__ void __launch_bounds__(lin_threads(LinWarps), 1) linear_pair_kernel(const __grid_constant__ CUtensorMap map_w,
     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearArgs p) {
   extern __shared__ uint8_t raw_smem[];
   __shared__ __align__(8) LinearBarriers bars;
-  __shared__ __align__(16) float token_scales[2][256];
+  __shared__ __align__(16) float token_scales[2][2][256];      // [group][the group's turn]
+  __shared__ __align__(16) float blocks[2 * LinWarps * LinBlockFloats];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
@@ -375,7 +455,7 @@ template <typename T> __global__ void __launch_bounds__(LinThreads, 1) linear_pa
   const int steps = (p.width + LinDepth - 1) / LinDepth, stages = p.stages;
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&bars.full[s], 1); mbar_init(&bars.empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&bars.done[b], 1); mbar_init(&bars.free[b], 2 * LinEpilogueWarps); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&bars.done[b], 1); mbar_init(&bars.free[b], 2 * LinWarps); }
     mbar_fence_init();
     abort_flag = 0;
   }
@@ -443,13 +523,19 @@ template <typename T> __global__ void __launch_bounds__(LinThreads, 1) linear_pa
       }
     }
   } else {
-    int n = 0;
-    for (int tile = first; tile < p.tiles; tile += step, ++n) {
-      const int b = n & 1;
+    if (p.tiles <= step && first < p.tiles) {
+      int n0, t0;
+      lin_origin(p, first, 2 * LinChannels, n0, t0);
+      lin_epilogue<T, C, 2 * LinWarps>(p, tmem, n0 + rank * LinChannels, t0, min(bt, p.tokens - t0), token_scales[0][0], blocks,
+                                       [&] { lin_wait(smem_u32(&bars.done[0]), 0, abortp); });
+    }
+    const int b = (warp - 2) / LinWarps;
+    uint32_t turn = 0;
+    for (int tile = first + b * step; p.tiles > step && tile < p.tiles; tile += 2 * step, turn ^= 1) {
       int n0, t0;
       lin_origin(p, tile, 2 * LinChannels, n0, t0);
-      lin_epilogue<T>(p, tmem + b * buffer, n0 + rank * LinChannels, t0, min(bt, p.tokens - t0), token_scales[b],
-                      [&] { lin_wait(smem_u32(&bars.done[b]), (n >> 1) & 1, abortp); });
+      lin_epilogue<T, C, LinWarps>(p, tmem + b * buffer, n0 + rank * LinChannels, t0, min(bt, p.tokens - t0), token_scales[b][turn], blocks,
+                      [&] { lin_wait(smem_u32(&bars.done[b]), turn, abortp); });
       if (lane == 0) pair_arrive(smem_u32(&bars.free[b]));
     }
   }
@@ -474,15 +560,17 @@ static int make_code_map(CUtensorMap* map, const void* base, int64_t rows, int w
   return TRI_OK;
 }
 
-template <typename T> static int launch_linear(const CUtensorMap& map_w, const CUtensorMap& map_x, const LinearArgs& p, int ctas,
-                                               bool pair, cudaStream_t s) {
-  static TriPerDevice configured;
-  const int device = configured.pending();
+template <typename T, int C> static int launch_linear_as(const CUtensorMap& map_w, const CUtensorMap& map_x, const LinearArgs& p, int ctas,
+                                                         bool pair, cudaStream_t s) {
+  const bool small = !pair && p.shared == LinSharedSmall;
+  const auto kernel = pair ? linear_pair_kernel<T, C> : small ? linear_kernel<T, C, true> : linear_kernel<T, C, false>;
+  static TriPerDevice configured[3];
+  TriPerDevice& known = configured[pair ? 0 : small ? 1 : 2];
+  const int device = known.pending();
   TRI_CHECK(device != -2, "int8_linear: no current CUDA device");
   if (device >= 0) {
-    TRI_CUDA(cudaFuncSetAttribute(linear_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinShared), "int8_linear");
-    TRI_CUDA(cudaFuncSetAttribute(linear_pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinShared), "int8_linear");
-    configured.mark(device);
+    TRI_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, small ? LinSharedSmall : LinShared), "int8_linear");
+    known.mark(device);
   }
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -490,11 +578,17 @@ template <typename T> static int launch_linear(const CUtensorMap& map_w, const C
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = pair ? 2u : (unsigned)p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(LinThreads); cfg.dynamicSmemBytes = (size_t)p.shared; cfg.stream = s;
+  cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(lin_threads(small ? LinSmallWarps : LinWarps)); cfg.dynamicSmemBytes = (size_t)p.shared; cfg.stream = s;
   cfg.attrs = attr; cfg.numAttrs = attr[1].val.clusterDim.x > 1 ? 2 : 1;
-  if (pair) TRI_CUDA(cudaLaunchKernelEx(&cfg, linear_pair_kernel<T>, map_w, map_x, p), "int8_linear");
-  else TRI_CUDA(cudaLaunchKernelEx(&cfg, linear_kernel<T>, map_w, map_x, p), "int8_linear");
+  TRI_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, p), "int8_linear");
   return tri_launch_status("int8_linear");
+}
+template <typename T> static int launch_linear(const CUtensorMap& map_w, const CUtensorMap& map_x, const LinearArgs& p, int ctas,
+                                               int channels, bool pair, cudaStream_t s) {
+  constexpr int Widest = 16 / (int)sizeof(T);
+  if (channels == Widest) return launch_linear_as<T, Widest>(map_w, map_x, p, ctas, pair, s);
+  if (channels == 2) return launch_linear_as<T, 2>(map_w, map_x, p, ctas, pair, s);
+  return launch_linear_as<T, 1>(map_w, map_x, p, ctas, pair, s);
 }
 
 // ---- which tile, how many CTAs per tile --------------------------------------------------------------------------------
@@ -546,16 +640,18 @@ static const LinearDevice* linear_device() {
     std::lock_guard<std::mutex> lock(guard);
     LinearDevice d{};
     cudaError_t e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, LinShared);
+    const auto large_tiles = linear_kernel<__nv_bfloat16, 8, false>, small_tiles = linear_kernel<__nv_bfloat16, 8, true>;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(large_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, LinShared);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(small_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, LinSharedSmall);
     for (int small = 0; small < 2; ++small)
       for (int n = 1; n <= 8 && e == cudaSuccess; ++n) {
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = (unsigned)n; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(n * 64)); cfg.blockDim = dim3(LinThreads); cfg.dynamicSmemBytes = small ? LinSharedSmall : LinShared;
+        cfg.gridDim = dim3((unsigned)(n * 64)); cfg.blockDim = dim3(lin_threads(small ? LinSmallWarps : LinWarps)); cfg.dynamicSmemBytes = small ? LinSharedSmall : LinShared;
         cfg.attrs = &attr; cfg.numAttrs = 1;
-        e = cudaOccupancyMaxActiveClusters(&d.clusters[small][n], linear_kernel<__nv_bfloat16>, &cfg);
+        e = cudaOccupancyMaxActiveClusters(&d.clusters[small][n], small ? small_tiles : large_tiles, &cfg);
         if (e == cudaSuccess && d.clusters[small][n] < 1) d.clusters[small][n] = 1;
       }
     if (e != cudaSuccess) { tri_set_error(cudaGetErrorString(e)); return nullptr; }
@@ -621,6 +717,12 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
   p.residual_stride = residual_stride; p.out_stride = out_stride; p.scales = scales; p.weight_scales = weight_scales;
   p.bias = bias; p.residual = residual; p.out = out; p.tokens = (int)tokens; p.outputs = outputs; p.width = width; p.error = device_error;
   p.token_tile = plan.token_tile; p.splits = plan.splits;
+  const auto rows_allow = [&](int channels) {                // accesses of so many channels to the rows of output and residual
+    const int64_t bytes = channels * (int64_t)cell;
+    return reinterpret_cast<uintptr_t>(out) % bytes == 0 && reinterpret_cast<uintptr_t>(residual) % bytes == 0 && out_stride % channels == 0 &&
+           (residual == nullptr || residual_stride % channels == 0);
+  };
+  const int each = rows_allow(16 / (int)cell) ? 16 / (int)cell : rows_allow(2) ? 2 : 1;
   const int channels = plan.pair ? 2 * LinChannels : LinChannels, box = plan.pair ? p.token_tile / 2 : p.token_tile;
   p.channel_tiles = (outputs + channels - 1) / channels;
   const int64_t tiles = (tokens + p.token_tile - 1) / p.token_tile * (int64_t)p.channel_tiles;
@@ -639,7 +741,7 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
   if (make_code_map(&map_w, weight, outputs, width, weight_stride, LinChannels) != TRI_OK) return TRI_ERR_CUDA;
   if (make_code_map(&map_x, codes, tokens, width, codes_stride, (unsigned)box) != TRI_OK) return TRI_ERR_CUDA;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, plan.pair, s);
-  if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, plan.pair, s);
-  return launch_linear<float>(map_w, map_x, p, ctas, plan.pair, s);
+  if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, each, plan.pair, s);
+  if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, each, plan.pair, s);
+  return launch_linear<float>(map_w, map_x, p, ctas, each, plan.pair, s);
 }
