@@ -190,6 +190,27 @@ def test_models_without_such_layers_are_refused():
         int8_projections(wrapped, ExactOps())   # once is enough
 
 
+def test_a_layer_used_twice_stays_one_layer():
+    from triattention_b200.models import int8_projections
+    model = toy("Llama")
+    model.model.layers[2] = model.model.layers[0]
+    ids = torch.arange(12)[None]
+    with torch.no_grad():
+        want = model(input_ids=ids, use_cache=False).logits
+        int8_projections(model, ExactOps())
+        torch.testing.assert_close(model(input_ids=ids, use_cache=False).logits, want, rtol=1e-4, atol=1e-4 * float(want.abs().max()))
+    assert model.model.layers[2] is model.model.layers[0] is not model.model.layers[1]
+
+
+def test_more_channels_than_32_bits_count_are_refused(lib):
+    """(The C call takes an int: 2^32 + 5 channels must not become 5.)"""
+    rows, weight = Int8Rows(torch.zeros(1, 16, dtype=torch.int8), torch.ones(1)), Int8Rows(torch.zeros(1, 16, dtype=torch.int8), torch.ones(1))
+    rows.index = weight.index = 0           # as if on a GPU: the refusal comes before anything is allocated or launched
+    weight.rows = (1 << 32) + 5
+    with pytest.raises(RuntimeError, match="weight"):
+        Int8Ops(Module(lib)).linear(rows, weight)
+
+
 def test_infer_flag(monkeypatch):
     """--int8-projections wraps the model before the engine is made; without it nothing is wrapped."""
     import sys

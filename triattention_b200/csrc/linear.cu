@@ -639,6 +639,7 @@ static const LinearDevice* linear_device() {
   if (pending == -2 || cudaGetDevice(&device) != cudaSuccess) { tri_set_error("int8_linear: no current CUDA device"); return nullptr; }
   if (pending >= 0) {
     std::lock_guard<std::mutex> lock(guard);
+    if (known.pending() < 0) return &devices[device];         // another thread was first
     LinearDevice d{};
     cudaError_t e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device);
     const auto large_tiles = linear_kernel<__nv_bfloat16, 8, false>, small_tiles = linear_kernel<__nv_bfloat16, 8, true>;

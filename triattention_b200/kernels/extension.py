@@ -58,6 +58,7 @@ SIGNATURES = {
 ABI_VERSION = 5         # tri_abi_version() of the library these signatures describe
 ROW_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}    # TRI_BF16, TRI_FP16, TRI_FP32
 MAX_WIDTH = 131071      # widest row of INT8 codes: 128 * 128 * width stays below 2^31
+MAX_OUTPUTS = 0x7fffff00    # channels and tokens of tri_int8_linear (32-bit indexes there)
 LONG_TAIL_ROWS = 8      # tri_decode_tail_hint: above this many rows (or without a hint) the unrolled merge kernel runs
 
 
@@ -551,7 +552,7 @@ class Module:
         pitch, weight_pitch = self._code_rows(codes, scales, index), self._code_rows(weight, weight_scales, index, "weight")
         tokens, outputs = out.shape
         width = codes.shape[1]
-        if codes.shape[0] != tokens or weight.shape != (outputs, width) or outputs < 1:
+        if codes.shape[0] != tokens or weight.shape != (outputs, width) or not 1 <= outputs <= MAX_OUTPUTS:
             raise RuntimeError("codes [T,K], weight [N,K], out [T,N]")
         if bias is not None:
             self._bias(bias, out, outputs)

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import torch
 
-from triattention_b200.kernels.extension import MAX_WIDTH, ROW_TYPES
+from triattention_b200.kernels.extension import MAX_OUTPUTS, MAX_WIDTH, ROW_TYPES
 
 CODE_ALIGN = 16     # code rows start on 16-byte boundaries
 
@@ -173,7 +173,7 @@ class Int8Ops:
             rows._refuse("linear")
         if weight.pitch < 0:
             weight._refuse("weight")
-        if rows.width != weight.width or len(weight.shape) != 2 or weight.index != index or outputs < 1:
+        if rows.width != weight.width or len(weight.shape) != 2 or weight.index != index or not 1 <= outputs <= MAX_OUTPUTS:
             raise RuntimeError("codes [..., K] and weight [N, K] on one GPU")
         dtype = dtype or rows.dtype
         shape = (rows.rows, outputs) if len(rows.shape) == 2 else (*rows.shape[:-1], outputs)

@@ -68,12 +68,15 @@ def int8_projections(model, ops=None):
     as they are, and so does what a model records of its own layer classes (output_hidden_states finds none).  Returns the
     model; a model without a layer of the Llama kind (RMS norms, q / k / v / o, gated SiLU) is refused."""
     ops = Int8Ops(load_extension()) if ops is None else ops
-    found = [(parent, name, child) for parent in model.modules() for name, child in parent.named_children()
-             if Int8DecoderLayer.fits(child)]
+    found = [(parent, name, child) for parent in model.modules() for name, child in parent._modules.items()
+             if child is not None and Int8DecoderLayer.fits(child)]
     if not found:
         raise RuntimeError("int8_projections: no decoder layer with RMS norms, q / k / v / o projections and a gated SiLU block")
+    made = {}       # a layer that the model uses in several places stays one layer
     for parent, name, child in found:
-        parent._modules[name] = Int8DecoderLayer(ops, child)
+        if id(child) not in made:
+            made[id(child)] = Int8DecoderLayer(ops, child)
+        parent._modules[name] = made[id(child)]
     return model
 
 
