@@ -447,7 +447,7 @@ class Module:
     # (These calls are short against the host's own time per call, so the checks are few and flat.)
     def _launch(self, fn, index, *args):
         """fn(*args, stream) on the current stream of GPU `index`."""
-        if index == torch.cuda.current_device():
+        if index == torch._C._cuda_getDevice():
             status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
             with torch.cuda.device(index):
@@ -457,20 +457,25 @@ class Module:
 
     @staticmethod
     def _rows(x, name):
-        """(type, GPU) of rows [T,H] with contiguous features."""
+        """(type, GPU, rows, width, stride) of rows [T,H] with contiguous features."""
         kind, index = ROW_TYPES.get(x.dtype), x.get_device()
-        if kind is None or index < 0 or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] != 1):
-            width = x.shape[-1] if x.dim() else 0
-            raise RuntimeError(f"{name}: rows of 1..{MAX_WIDTH} features" if not 1 <= width <= MAX_WIDTH else
-                               f"{name}: rows [T,H] of bf16, fp16 or fp32 on a GPU with contiguous features")
-        return kind, index
+        if kind is not None and index >= 0 and x.dim() == 2:
+            rows, width = x.shape
+            stride, feature = x.stride()
+            if (feature == 1 or width == 1) and 1 <= width <= MAX_WIDTH:
+                return kind, index, rows, width, stride
+        width = x.shape[-1] if x.dim() else 0
+        raise RuntimeError(f"{name}: rows of 1..{MAX_WIDTH} features" if not 1 <= width <= MAX_WIDTH else
+                           f"{name}: rows [T,H] of bf16, fp16 or fp32 on a GPU with contiguous features")
 
     @staticmethod
-    def _like(x, other, name):
-        """Rows of the shape, type and GPU of `other`."""
-        if (x.shape != other.shape or x.dtype != other.dtype or x.get_device() != other.get_device() or
-                (x.stride(1) != 1 and x.shape[1] != 1)):
-            raise RuntimeError(f"{name}: shape, type and device of the other rows, with contiguous features")
+    def _like(x, other, index, name):
+        """Stride of rows of the shape, type and GPU of `other`."""
+        if x.dtype == other.dtype and x.shape == other.shape and x.get_device() == index:
+            stride, feature = x.stride()
+            if feature == 1 or x.shape[1] == 1:
+                return stride
+        raise RuntimeError(f"{name}: shape, type and device of the other rows, with contiguous features")
 
     @staticmethod
     def _code_rows(codes, scales, index, name="codes"):
@@ -486,83 +491,75 @@ class Module:
         return pitch
 
     @staticmethod
-    def _norm_weight(weight, x, width):
-        if (weight.dtype != x.dtype or weight.shape != (width,) or weight.get_device() != x.get_device() or
-                (weight.stride(0) != 1 and width != 1)):
+    def _norm_weight(weight, x, width, index):
+        if weight.dtype != x.dtype or weight.shape != (width,) or weight.get_device() != index or not weight.is_contiguous():
             raise RuntimeError("norm weight [H] of the type and on the device of x")
 
     @staticmethod
-    def _bias(bias, out, outputs):
-        if (bias.dtype != out.dtype or bias.shape != (outputs,) or bias.get_device() != out.get_device() or
-                (bias.stride(0) != 1 and outputs != 1)):
+    def _bias(bias, dtype, outputs, index):
+        if bias.dtype != dtype or bias.shape != (outputs,) or bias.get_device() != index or not bias.is_contiguous():
             raise RuntimeError("bias [N] of the output's type, on its device")
 
     def quantize_rows(self, x, codes, scales):
         """codes [T,H] and scales [T] of the rows x [T,H]."""
-        kind, index = self._rows(x, "x")
+        kind, index, rows, width, stride = self._rows(x, "x")
         pitch = self._code_rows(codes, scales, index)
         if codes.shape != x.shape:
             raise RuntimeError("codes have the shape of x")
-        self._launch(self.lib.tri_quantize_rows, index, x.data_ptr(), kind, *x.shape, x.stride(0), codes.data_ptr(), pitch,
+        self._launch(self.lib.tri_quantize_rows, index, x.data_ptr(), kind, rows, width, stride, codes.data_ptr(), pitch,
                      scales.data_ptr())
 
     def silu_mul_rows(self, gate, up, codes, scales):
         """codes and scales of silu(gate) * up."""
-        kind, index = self._rows(gate, "gate")
-        self._like(up, gate, "up")
+        kind, index, rows, width, stride = self._rows(gate, "gate")
+        up_stride = self._like(up, gate, index, "up")
         pitch = self._code_rows(codes, scales, index)
         if codes.shape != gate.shape:
             raise RuntimeError("codes have the shape of gate and up")
-        self._launch(self.lib.tri_silu_mul_rows, index, gate.data_ptr(), up.data_ptr(), kind, *gate.shape, gate.stride(0),
-                     up.stride(0), codes.data_ptr(), pitch, scales.data_ptr())
+        self._launch(self.lib.tri_silu_mul_rows, index, gate.data_ptr(), up.data_ptr(), kind, rows, width, stride, up_stride,
+                     codes.data_ptr(), pitch, scales.data_ptr())
 
     def rms_norm_rows(self, x, weight, eps, codes, scales, residual=None, residual_out=None):
         """codes and scales of the normed rows of h = x (+ residual, whose rounded sum goes to residual_out)."""
-        kind, index = self._rows(x, "x")
+        kind, index, rows, width, stride = self._rows(x, "x")
         pitch = self._code_rows(codes, scales, index)
-        rows, width = x.shape
         if codes.shape != x.shape:
             raise RuntimeError("codes have the shape of x")
-        self._norm_weight(weight, x, width)
-        if residual is None and residual_out is None:
-            self._launch(self.lib.tri_rms_norm_rows, index, x.data_ptr(), None, weight.data_ptr(), kind, rows, width, x.stride(0), 0,
-                         eps, None, 0, codes.data_ptr(), pitch, scales.data_ptr())
-            return
-        if residual is None or residual_out is None:
+        self._norm_weight(weight, x, width, index)
+        if (residual is None) != (residual_out is None):
             raise RuntimeError("the residual and where its sum goes (both or none)")
-        self._like(residual, x, "residual"), self._like(residual_out, x, "residual_out")
-        self._launch(self.lib.tri_rms_norm_rows, index, x.data_ptr(), residual.data_ptr(), weight.data_ptr(), kind, rows, width,
-                     x.stride(0), residual.stride(0), eps, residual_out.data_ptr(), residual_out.stride(0) if rows > 1 else width,
-                     codes.data_ptr(), pitch, scales.data_ptr())
+        residual_stride = 0 if residual is None else self._like(residual, x, index, "residual")
+        out_stride = 0 if residual is None else self._like(residual_out, x, index, "residual_out")
+        if residual is not None and rows <= 1:
+            out_stride = width
+        self._launch(self.lib.tri_rms_norm_rows, index, x.data_ptr(), _ptr(residual), weight.data_ptr(), kind, rows, width, stride,
+                     residual_stride, eps, _ptr(residual_out), out_stride, codes.data_ptr(), pitch, scales.data_ptr())
 
     def dequantize_rows(self, codes, scales, out):
         """out [T,H] = scale * code, rounded to out's type."""
-        kind, index = self._rows(out, "out")
+        kind, index, rows, width, stride = self._rows(out, "out")
         pitch = self._code_rows(codes, scales, index)
-        rows, width = out.shape
         if codes.shape != out.shape:
             raise RuntimeError("codes have the shape of out")
         self._launch(self.lib.tri_dequantize_rows, index, codes.data_ptr(), pitch, scales.data_ptr(), kind, rows, width,
-                     out.data_ptr(), out.stride(0) if rows > 1 else width)
+                     out.data_ptr(), stride if rows > 1 else width)
         return out
 
     def int8_linear(self, codes, scales, weight, weight_scales, out, bias=None, residual=None):
         """out [T,N] = (codes [T,K] . weight [N,K]^T) * weight_scales[n] * scales[t] + bias[n] + residual[t,n]."""
-        kind, index = self._rows(out, "out")
+        kind, index = ROW_TYPES.get(out.dtype), out.get_device()
+        if kind is None or index < 0 or out.dim() != 2 or (out.stride(1) != 1 and out.shape[1] != 1):
+            raise RuntimeError("out: rows [T,N] of bf16, fp16 or fp32 on a GPU with contiguous features")
         pitch, weight_pitch = self._code_rows(codes, scales, index), self._code_rows(weight, weight_scales, index, "weight")
         tokens, outputs = out.shape
         width = codes.shape[1]
         if codes.shape[0] != tokens or weight.shape != (outputs, width) or not 1 <= outputs <= MAX_OUTPUTS:
             raise RuntimeError("codes [T,K], weight [N,K], out [T,N]")
         if bias is not None:
-            self._bias(bias, out, outputs)
-        residual_stride = 0
-        if residual is not None:
-            self._like(residual, out, "residual")
-            residual_stride = residual.stride(0)
+            self._bias(bias, out.dtype, outputs, index)
+        residual_stride = 0 if residual is None else self._like(residual, out, index, "residual")
         self._launch(self.lib.tri_int8_linear, index, codes.data_ptr(), pitch, scales.data_ptr(), weight.data_ptr(), weight_pitch,
-                     weight_scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                     None if residual is None else residual.data_ptr(), residual_stride, out.data_ptr(),
+                     weight_scales.data_ptr(), _ptr(bias), _ptr(residual), residual_stride, out.data_ptr(),
                      out.stride(0) if tokens > 1 else outputs, kind, tokens, outputs, width, self._error_pointer(index))
         return out
 

@@ -49,18 +49,16 @@ class Int8Rows:
             raise RuntimeError("Int8Rows: codes and scales on one device")
 
     @classmethod
-    def _empty(cls, shape, rows, width, dtype, device, index):
-        """Uninitialised rows for a call to fill."""
-        if not 1 <= width <= MAX_WIDTH:
-            raise RuntimeError(f"rows of 1..{MAX_WIDTH} features")
+    def _empty(cls, like, rows, width, index):
+        """Uninitialised rows, of the shape and type of `like`, for a call to fill."""
         self = cls.__new__(cls)
         pitch = -(-width // CODE_ALIGN) * CODE_ALIGN
+        self.device = device = like.device
         self._buffer = buffer = torch.empty(rows * (pitch + 4), dtype=torch.int8, device=device)
-        self.shape, self.dtype, self.device, self.index = shape, dtype, device, index
-        self.rows, self.width, self.pitch = rows, width, pitch
-        self.codes_ptr = buffer.data_ptr()
-        self.scales_ptr = self.codes_ptr + rows * pitch
-        self._codes = self._scales = None
+        self.codes_ptr = pointer = buffer.data_ptr()
+        self.scales_ptr = pointer + rows * pitch
+        self.shape, self.dtype, self.index, self.rows, self.width, self.pitch = like.shape, like.dtype, index, rows, width, pitch
+        self._codes = None
         return self
 
     def _refuse(self, name):
@@ -94,7 +92,9 @@ class Int8Ops:
     inputs that ask for one are refused while gradients are being recorded."""
 
     def __init__(self, module):
-        self.module = module
+        self.module, lib = module, module.lib
+        self._launch, self._calls = module._launch, (lib.tri_quantize_rows, lib.tri_silu_mul_rows, lib.tri_rms_norm_rows,
+                                                     lib.tri_dequantize_rows, lib.tri_int8_linear)
 
     @staticmethod
     def _inference(*tensors):
@@ -107,12 +107,10 @@ class Int8Ops:
     def quantize_rows(self, x):
         """x [..., H] (bf16, fp16 or fp32) -> Int8Rows."""
         self._inference(x)
-        m, flat = self.module, _flat(x)
-        kind, index = m._rows(flat, "x")
-        rows, width = flat.shape
-        out = Int8Rows._empty(x.shape, rows, width, x.dtype, x.device, index)
-        m._launch(m.lib.tri_quantize_rows, index, flat.data_ptr(), kind, rows, width, flat.stride(0), out.codes_ptr, out.pitch,
-                  out.scales_ptr)
+        flat = x if x.dim() == 2 else _flat(x)
+        kind, index, rows, width, stride = self.module._rows(flat, "x")
+        out = Int8Rows._empty(x, rows, width, index)
+        self._launch(self._calls[0], index, flat.data_ptr(), kind, rows, width, stride, out.codes_ptr, out.pitch, out.scales_ptr)
         return out
 
     def silu_mul(self, gate, up):
@@ -120,13 +118,12 @@ class Int8Ops:
         self._inference(gate, up)
         if gate.shape != up.shape:
             raise RuntimeError("gate and up have one shape")
-        m, flat, other = self.module, _flat(gate), _flat(up)
-        kind, index = m._rows(flat, "gate")
-        m._like(other, flat, "up")
-        rows, width = flat.shape
-        out = Int8Rows._empty(gate.shape, rows, width, gate.dtype, gate.device, index)
-        m._launch(m.lib.tri_silu_mul_rows, index, flat.data_ptr(), other.data_ptr(), kind, rows, width, flat.stride(0),
-                  other.stride(0), out.codes_ptr, out.pitch, out.scales_ptr)
+        flat, other = (gate, up) if gate.dim() == 2 else (_flat(gate), _flat(up))
+        kind, index, rows, width, stride = self.module._rows(flat, "gate")
+        other_stride = self.module._like(other, flat, index, "up")
+        out = Int8Rows._empty(gate, rows, width, index)
+        self._launch(self._calls[1], index, flat.data_ptr(), other.data_ptr(), kind, rows, width, stride, other_stride, out.codes_ptr,
+                     out.pitch, out.scales_ptr)
         return out
 
     def rms_norm(self, x, weight, eps, residual=None):
@@ -135,33 +132,32 @@ class Int8Ops:
         self._inference(x, weight, residual)
         if residual is not None and residual.shape != x.shape:
             raise RuntimeError("x and residual have one shape")
-        m, flat = self.module, _flat(x)
-        kind, index = m._rows(flat, "x")
-        rows, width = flat.shape
-        m._norm_weight(weight, flat, width)
+        m, flat = self.module, x if x.dim() == 2 else _flat(x)
+        kind, index, rows, width, stride = m._rows(flat, "x")
+        m._norm_weight(weight, flat, width, index)
         if residual is None:
-            out = Int8Rows._empty(x.shape, rows, width, x.dtype, x.device, index)
-            m._launch(m.lib.tri_rms_norm_rows, index, flat.data_ptr(), None, weight.data_ptr(), kind, rows, width, flat.stride(0), 0,
-                      eps, None, 0, out.codes_ptr, out.pitch, out.scales_ptr)
+            out = Int8Rows._empty(x, rows, width, index)
+            self._launch(self._calls[2], index, flat.data_ptr(), None, weight.data_ptr(), kind, rows, width, stride, 0, eps, None, 0,
+                         out.codes_ptr, out.pitch, out.scales_ptr)
             return out
-        other = _flat(residual)
-        m._like(other, flat, "residual")
-        out = Int8Rows._empty(x.shape, rows, width, x.dtype, x.device, index)
+        other = residual if residual.dim() == 2 else _flat(residual)
+        other_stride = m._like(other, flat, index, "residual")
+        out = Int8Rows._empty(x, rows, width, index)
         total = torch.empty_like(x) if x.is_contiguous() else x.new_empty(*x.shape)
-        m._launch(m.lib.tri_rms_norm_rows, index, flat.data_ptr(), other.data_ptr(), weight.data_ptr(), kind, rows, width,
-                  flat.stride(0), other.stride(0), eps, total.data_ptr(), width, out.codes_ptr, out.pitch, out.scales_ptr)
+        self._launch(self._calls[2], index, flat.data_ptr(), other.data_ptr(), weight.data_ptr(), kind, rows, width, stride,
+                     other_stride, eps, total.data_ptr(), width, out.codes_ptr, out.pitch, out.scales_ptr)
         return out, total
 
     def dequantize(self, rows, dtype=None):
         """The values that rows of codes stand for, in `dtype` (default: the type they were made from)."""
         dtype = dtype or rows.dtype
-        m, out, kind = self.module, torch.empty(*rows.shape, dtype=dtype, device=rows.device), ROW_TYPES.get(dtype)
+        out, kind = torch.empty(*rows.shape, dtype=dtype, device=rows.device), ROW_TYPES.get(dtype)
         if rows.pitch < 0 or rows.index < 0:
             rows._refuse("dequantize")
         if kind is None:
             raise RuntimeError("dequantize: bf16, fp16 or fp32 values")
-        m._launch(m.lib.tri_dequantize_rows, rows.index, rows.codes_ptr, rows.pitch, rows.scales_ptr, kind, rows.rows, rows.width,
-                  out.data_ptr(), rows.width)
+        self._launch(self._calls[3], rows.index, rows.codes_ptr, rows.pitch, rows.scales_ptr, kind, rows.rows, rows.width,
+                     out.data_ptr(), rows.width)
         return out
 
     def linear(self, rows, weight, bias=None, residual=None, dtype=None):
@@ -181,7 +177,7 @@ class Int8Ops:
         if kind is None:
             raise RuntimeError("linear: bf16, fp16 or fp32 outputs")
         if bias is not None:
-            m._bias(bias, out, outputs)
+            m._bias(bias, dtype, outputs, index)
         residual_ptr, residual_stride = None, 0
         if residual is not None:
             if residual.shape != out.shape:
@@ -190,9 +186,9 @@ class Int8Ops:
             if residual.dtype != out.dtype or residual.get_device() != index or (residual.stride(1) != 1 and outputs != 1):
                 raise RuntimeError("residual of the output's type, on its device, with contiguous features")
             residual_ptr, residual_stride = residual.data_ptr(), residual.stride(0)
-        m._launch(m.lib.tri_int8_linear, index, rows.codes_ptr, rows.pitch, rows.scales_ptr, weight.codes_ptr, weight.pitch,
-                  weight.scales_ptr, None if bias is None else bias.data_ptr(), residual_ptr, residual_stride, out.data_ptr(),
-                  outputs, kind, rows.rows, outputs, rows.width, m._error_pointer(index))
+        self._launch(self._calls[4], index, rows.codes_ptr, rows.pitch, rows.scales_ptr, weight.codes_ptr, weight.pitch,
+                     weight.scales_ptr, None if bias is None else bias.data_ptr(), residual_ptr, residual_stride, out.data_ptr(),
+                     outputs, kind, rows.rows, outputs, rows.width, m._error_pointer(index))
         return out
 
 
