@@ -19,7 +19,7 @@
 
 namespace tri {
 
-constexpr int LinChannels = 128, LinDepth = 128;             // channels of a CTA's tile; bytes of width per stage
+constexpr int LinChannels = 128, LinDepth = 128;             // channels of a CTA's tile; bytes of width per step
 constexpr int LinWarps = 8, LinSmallWarps = 4;               // epilogue warps of a group, where a CTA has the SM to itself and where two
                                                              // share it; two groups take a CTA's tiles in turn
 __host__ __device__ constexpr int lin_threads(int warps) { return 64 + 2 * 32 * warps; }
@@ -269,8 +269,8 @@ __device__ __forceinline__ void lin_epilogue(const LinearArgs& p, uint32_t colum
   else lin_epilogue_as<T, C, Warps, false>(p, column, n0, t0, valid, token_scales, block, ready);
 }
 
-// One CTA per tile of 128 channels; Small: two of them per SM.  grid = CTAs (persistent) when splits is 1, otherwise tiles * splits with one tile per cluster.
-template <typename T, int C, bool Small> __global__ void __launch_bounds__(lin_threads(Small ? LinSmallWarps : LinWarps), Small ? 2 : 1) linear_kernel(const __grid_constant__ CUtensorMap map_w,
+// One CTA per tile of 128 channels; Small: two of them per SM; Deep: steps of 128 bytes of width that a stage holds.  grid = CTAs (persistent) when splits is 1, otherwise tiles * splits with one tile per cluster.
+template <typename T, int C, bool Small, int Deep> __global__ void __launch_bounds__(lin_threads(Small ? LinSmallWarps : LinWarps), Small ? 2 : 1) linear_kernel(const __grid_constant__ CUtensorMap map_w,
     const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearArgs p) {
   extern __shared__ uint8_t raw_smem[];
   __shared__ __align__(8) LinearBarriers bars;
@@ -281,7 +281,7 @@ template <typename T, int C, bool Small> __global__ void __launch_bounds__(lin_t
   __shared__ int abort_flag;
   uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int bt = p.token_tile, stage_bytes = LinWeightBytes + bt * LinDepth, splits = p.splits;
+  const int bt = p.token_tile, step_bytes = LinWeightBytes + bt * LinDepth, stage_bytes = Deep * step_bytes, splits = p.splits;
   const int rank = blockIdx.x % splits, first = blockIdx.x / splits, step = gridDim.x / splits;
   const int all_steps = (p.width + LinDepth - 1) / LinDepth;
   const int k0 = (int)((int64_t)all_steps * rank / splits), k1 = (int)((int64_t)all_steps * (rank + 1) / splits);
@@ -312,11 +312,16 @@ template <typename T, int C, bool Small> __global__ void __launch_bounds__(lin_t
       for (int tile = first; ok && tile < p.tiles; tile += step) {
         int n0, t0;
         lin_origin(p, tile, LinChannels, n0, t0);
-        for (int k = k0 * LinDepth; k < k1 * LinDepth; k += LinDepth) {
+        for (int k = k0; k < k1; k += Deep) {
           if (filled >= stages && !(ok = lin_wait(empty, phase, abortp))) break;
-          lin_expect(full, stage_bytes);
-          lin_copy(at, &map_w, k, n0, full);
-          lin_copy(at + LinWeightBytes, &map_x, k, t0, full);
+          const bool both = Deep > 1 && k + 1 < k1;
+          lin_expect(full, both ? stage_bytes : step_bytes);
+          lin_copy(at, &map_w, k * LinDepth, n0, full);
+          lin_copy(at + LinWeightBytes, &map_x, k * LinDepth, t0, full);
+          if (both) {
+            lin_copy(at + step_bytes, &map_w, (k + 1) * LinDepth, n0, full);
+            lin_copy(at + step_bytes + LinWeightBytes, &map_x, (k + 1) * LinDepth, t0, full);
+          }
           ++filled;
           at += stage_bytes; full += 8; empty += 8;
           if (++stage == stages) { stage = 0; at = smem_base; full = full_base; empty = empty_base; phase ^= 1u; }
@@ -329,7 +334,7 @@ template <typename T, int C, bool Small> __global__ void __launch_bounds__(lin_t
     if (lane == 0) {
       const uint32_t idesc = instr_desc(2, 1, 1, LinChannels, bt);
       const uint64_t desc = smem_desc(smem_base, 0, 1024, Layout128B);
-      const uint32_t stage_units = stage_bytes >> 4;          // descriptors address 16-byte units; a stage's all lie below 2^14 of them
+      const uint32_t stage_units = stage_bytes >> 4, step_units = step_bytes >> 4;   // descriptors address 16-byte units, all below 2^14
       uint32_t full = full_base, empty = empty_base, phase = 0;
       int stage = 0, n = 0;
       uint64_t dw = desc;
@@ -340,13 +345,17 @@ template <typename T, int C, bool Small> __global__ void __launch_bounds__(lin_t
         tc_fence_after();
         const uint32_t acc = tmem + b * buffer;
         uint32_t accumulate = 0;
-        for (int k = k0; k < k1; ++k) {
+        for (int k = k0; k < k1; k += Deep) {
           if (!(ok = lin_wait(full, phase, abortp))) break;
           tc_fence_after();
           const uint64_t dx = dw + (LinWeightBytes >> 4);
           umma_i8(acc, dw, dx, idesc, accumulate);            // 32 codes per MMA: 2 units of 16 bytes along the row
 #pragma unroll
           for (int kk = 1; kk < LinDepth / 32; ++kk) umma_i8(acc, dw + 2 * kk, dx + 2 * kk, idesc, 1u);
+          if (Deep > 1 && k + 1 < k1) {
+#pragma unroll
+            for (int kk = 0; kk < LinDepth / 32; ++kk) umma_i8(acc, dw + step_units + 2 * kk, dx + step_units + 2 * kk, idesc, 1u);
+          }
           lin_commit(empty);
           accumulate = 1;
           dw += stage_units; full += 8; empty += 8;
@@ -450,7 +459,8 @@ template <typename T, int C> __global__ void __launch_bounds__(lin_threads(LinWa
   __shared__ int abort_flag;
   uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int bt = p.token_tile, stage_bytes = LinWeightBytes + bt / 2 * LinDepth;
+  constexpr int Deep = 2;
+  const int bt = p.token_tile, step_bytes = LinWeightBytes + bt / 2 * LinDepth, stage_bytes = Deep * step_bytes;
   const int rank = blockIdx.x & 1, first = blockIdx.x / 2, step = gridDim.x / 2;
   const int steps = (p.width + LinDepth - 1) / LinDepth, stages = p.stages;
   if (tid == 0) {
@@ -479,11 +489,16 @@ template <typename T, int C> __global__ void __launch_bounds__(lin_threads(LinWa
         int n0, t0;
         lin_origin(p, tile, 2 * LinChannels, n0, t0);
         n0 += rank * LinChannels; t0 += rank * (bt / 2);
-        for (int k = 0; k < steps * LinDepth; k += LinDepth) {
+        for (int k = 0; k < steps; k += Deep) {
           if (filled >= stages && !(ok = lin_wait(empty, phase, abortp))) break;
-          if (rank == 0) lin_expect(full, 2 * stage_bytes);   // what both CTAs' copies bring
-          pair_copy(at, &map_w, k, n0, full);
-          pair_copy(at + LinWeightBytes, &map_x, k, t0, full);
+          const bool both = Deep > 1 && k + 1 < steps;
+          if (rank == 0) lin_expect(full, 2 * (both ? stage_bytes : step_bytes));   // what both CTAs' copies bring
+          pair_copy(at, &map_w, k * LinDepth, n0, full);
+          pair_copy(at + LinWeightBytes, &map_x, k * LinDepth, t0, full);
+          if (both) {
+            pair_copy(at + step_bytes, &map_w, (k + 1) * LinDepth, n0, full);
+            pair_copy(at + step_bytes + LinWeightBytes, &map_x, (k + 1) * LinDepth, t0, full);
+          }
           ++filled;
           at += stage_bytes; full += 8; empty += 8;
           if (++stage == stages) { stage = 0; at = smem_base; full = full_base; empty = empty_base; phase ^= 1u; }
@@ -496,7 +511,7 @@ template <typename T, int C> __global__ void __launch_bounds__(lin_threads(LinWa
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = instr_desc(2, 1, 1, 2 * LinChannels, bt);
       const uint64_t desc = smem_desc(smem_base, 0, 1024, Layout128B);
-      const uint32_t stage_units = stage_bytes >> 4;
+      const uint32_t stage_units = stage_bytes >> 4, step_units = step_bytes >> 4;
       uint32_t full = full_base, empty = empty_base, phase = 0;
       int stage = 0, n = 0;
       uint64_t dw = desc;
@@ -507,13 +522,17 @@ template <typename T, int C> __global__ void __launch_bounds__(lin_threads(LinWa
         tc_fence_after();
         const uint32_t acc = tmem + b * buffer;
         uint32_t accumulate = 0;
-        for (int k = 0; k < steps; ++k) {
+        for (int k = 0; k < steps; k += Deep) {
           if (!(ok = lin_wait(full, phase, abortp))) break;
           tc_fence_after();
           const uint64_t dx = dw + (LinWeightBytes >> 4);
           pair_umma(acc, dw, dx, idesc, accumulate);
 #pragma unroll
           for (int kk = 1; kk < LinDepth / 32; ++kk) pair_umma(acc, dw + 2 * kk, dx + 2 * kk, idesc, 1u);
+          if (Deep > 1 && k + 1 < steps) {
+#pragma unroll
+            for (int kk = 0; kk < LinDepth / 32; ++kk) pair_umma(acc, dw + step_units + 2 * kk, dx + step_units + 2 * kk, idesc, 1u);
+          }
           pair_commit(empty);
           accumulate = 1;
           dw += stage_units; full += 8; empty += 8;
@@ -561,11 +580,12 @@ static int make_code_map(CUtensorMap* map, const void* base, int64_t rows, int w
 }
 
 template <typename T, int C> static int launch_linear_as(const CUtensorMap& map_w, const CUtensorMap& map_x, const LinearArgs& p, int ctas,
-                                                         bool pair, cudaStream_t s) {
+                                                         bool pair, int deep, cudaStream_t s) {
   const bool small = !pair && p.shared == LinSharedSmall;
-  const auto kernel = pair ? linear_pair_kernel<T, C> : small ? linear_kernel<T, C, true> : linear_kernel<T, C, false>;
-  static TriPerDevice configured[3];
-  TriPerDevice& known = configured[pair ? 0 : small ? 1 : 2];
+  const auto kernel = pair ? linear_pair_kernel<T, C> : small ? linear_kernel<T, C, true, 1>
+                      : deep == 1 ? linear_kernel<T, C, false, 1> : linear_kernel<T, C, false, 2>;
+  static TriPerDevice configured[4];
+  TriPerDevice& known = configured[pair ? 0 : small ? 1 : 1 + deep];
   const int device = known.pending();
   TRI_CHECK(device != -2, "int8_linear: no current CUDA device");
   if (device >= 0) {
@@ -584,11 +604,11 @@ template <typename T, int C> static int launch_linear_as(const CUtensorMap& map_
   return tri_launch_status("int8_linear");
 }
 template <typename T> static int launch_linear(const CUtensorMap& map_w, const CUtensorMap& map_x, const LinearArgs& p, int ctas,
-                                               int channels, bool pair, cudaStream_t s) {
+                                               int channels, bool pair, int deep, cudaStream_t s) {
   constexpr int Widest = 16 / (int)sizeof(T);
-  if (channels == Widest) return launch_linear_as<T, Widest>(map_w, map_x, p, ctas, pair, s);
-  if (channels == 2) return launch_linear_as<T, 2>(map_w, map_x, p, ctas, pair, s);
-  return launch_linear_as<T, 1>(map_w, map_x, p, ctas, pair, s);
+  if (channels == Widest) return launch_linear_as<T, Widest>(map_w, map_x, p, ctas, pair, deep, s);
+  if (channels == 2) return launch_linear_as<T, 2>(map_w, map_x, p, ctas, pair, deep, s);
+  return launch_linear_as<T, 1>(map_w, map_x, p, ctas, pair, deep, s);
 }
 
 // ---- which tile, how many CTAs per tile --------------------------------------------------------------------------------
@@ -642,7 +662,7 @@ static const LinearDevice* linear_device() {
     if (known.pending() < 0) return &devices[device];         // another thread was first
     LinearDevice d{};
     cudaError_t e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device);
-    const auto large_tiles = linear_kernel<__nv_bfloat16, 8, false>, small_tiles = linear_kernel<__nv_bfloat16, 8, true>;
+    const auto large_tiles = linear_kernel<__nv_bfloat16, 8, false, 2>, small_tiles = linear_kernel<__nv_bfloat16, 8, true, 1>;
     if (e == cudaSuccess) e = cudaFuncSetAttribute(large_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, LinShared);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(small_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, LinSharedSmall);
     for (int small = 0; small < 2; ++small)
@@ -732,7 +752,11 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
   p.tiles = (int)tiles;
   p.group = 8;
   p.shared = !plan.pair && p.token_tile <= LinSmallTile ? LinSharedSmall : LinShared;
-  p.stages = (p.shared - 1024) / (LinWeightBytes + box * LinDepth);
+  // Two steps per stage where three stages of them fit: the issuing threads' work per stage is 0.1 us dearer than the MMAs of a
+  // narrow tile (128 steps of 16 tokens: 38 us, 29 with two per stage; 16384 x 14336 -> 4096 in pairs: 649 us, 602).
+  const int step_bytes = LinWeightBytes + box * LinDepth;
+  const int deep = plan.pair || (p.shared == LinShared && (p.shared - 1024) / (2 * step_bytes) >= 3) ? 2 : 1;
+  p.stages = (p.shared - 1024) / (deep * step_bytes);
   if (p.stages > LinMaxStages) p.stages = LinMaxStages;
   p.columns = 32;
   while (p.columns < 2 * p.token_tile) p.columns *= 2;
@@ -743,7 +767,7 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
   if (make_code_map(&map_w, weight, outputs, width, weight_stride, LinChannels) != TRI_OK) return TRI_ERR_CUDA;
   if (make_code_map(&map_x, codes, tokens, width, codes_stride, (unsigned)box) != TRI_OK) return TRI_ERR_CUDA;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, each, plan.pair, s);
-  if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, each, plan.pair, s);
-  return launch_linear<float>(map_w, map_x, p, ctas, each, plan.pair, s);
+  if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, each, plan.pair, deep, s);
+  if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, each, plan.pair, deep, s);
+  return launch_linear<float>(map_w, map_x, p, ctas, each, plan.pair, deep, s);
 }
