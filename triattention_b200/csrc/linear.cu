@@ -621,32 +621,32 @@ struct LinearDevice {                  // of one GPU, asked for once
   int clusters[2][9];                  // clusters of n CTAs that are resident at once, by shared memory (0: LinShared, 1: LinSharedSmall)
 };
 
-// Estimated time (us) of a plan, less what every plan takes.  The constants are a fit to measured times of 314 shapes (1 to 16384
-// tokens, 96 to 32768 channels, widths 96 to 16384) under every tile and split: the plan that the estimate picks takes 1.7 % more
-// than the best one on average, 22 % at worst.  A stage of 128 bytes of width costs what the issuing thread needs for it (0.3 us)
-// or what the SM's port to L2 does (0.12 MB/us); tiles run in rounds of as many as are resident, each no shorter than its epilogue;
-// a split adds a cluster barrier and the exchange of the partial sums; and all of it overlaps with the traffic to HBM.
+// Estimated time (us) of a plan, less what every plan takes.  The constants are a fit to measured times of 346 shapes (1 to 16384
+// tokens, 96 to 32768 channels, widths 96 to 16384) under every tile and split: the plan that the estimate picks takes 1 % more
+// than the best one on average, 16 % at worst.  A step of 128 bytes of width costs what the issuing threads need for it (0.3 us)
+// or what the SM's port to L2 does (0.1 MB/us); tiles run in rounds of as many as are resident, each no shorter than its epilogue;
+// a split adds a cluster barrier and the exchange of the partial sums; and part of it overlaps with the traffic to HBM.
 static float plan_time(const LinearPlan& plan, int64_t tokens, int outputs, int width, const LinearDevice& d) {
   const int steps = (width + LinDepth - 1) / LinDepth, bt = plan.token_tile;
   const int channels = plan.pair ? 2 * LinChannels : LinChannels;
   const int64_t tiles = (tokens + bt - 1) / bt * (int64_t)((outputs + channels - 1) / channels);
   float t;
   if (plan.pair) {
-    const float rounds = (float)((tiles + d.sms / 2 - 1) / (d.sms / 2)), epilogue = 0.035f + 0.0067f * bt;
-    const float stage = fmaxf(0.304f, (LinWeightBytes + bt / 2 * LinDepth) * (1.f / 116300.f));
-    t = rounds * fmaxf(stage * steps, epilogue) + epilogue;
+    const float rounds = (float)((tiles + d.sms / 2 - 1) / (d.sms / 2)), epilogue = 0.0054f + 0.009f * bt;
+    const float step = fmaxf(0.279f, (LinWeightBytes + bt / 2 * LinDepth) * (1.f / 98080.f));
+    t = rounds * fmaxf(step * steps, epilogue) + epilogue;
   } else {
     const bool small = bt <= LinSmallTile;
     const int64_t ctas = tiles * plan.splits, slots = (int64_t)d.clusters[small][plan.splits] * plan.splits;
     const float rounds = (float)((ctas + slots - 1) / slots), live = (float)(tokens < bt ? tokens : bt);
-    float stage = fmaxf(0.344f, (LinWeightBytes + bt * LinDepth) * (1.f / 116300.f));
-    if (small && ctas > d.sms) stage *= 1.83f;               // two CTAs per SM share its port and its tensor core
-    const float mine = (float)((steps + plan.splits - 1) / plan.splits) * stage, epilogue = 0.185f + 0.002f * live;
-    if (plan.splits > 1) t = rounds * (mine + 2.3f + 0.0118f * live);
+    float step = fmaxf(!small && bt <= 128 ? 0.297f : 0.31f, (LinWeightBytes + bt * LinDepth) * (1.f / 98080.f));
+    if (small && ctas > d.sms) step *= 1.96f;                // two CTAs per SM share its port and its tensor core
+    const float mine = (float)((steps + plan.splits - 1) / plan.splits) * step, epilogue = 0.091f + 0.0017f * live;
+    if (plan.splits > 1) t = rounds * (mine + 2.19f + 0.0061f * live);
     else t = rounds * fmaxf(mine, epilogue) + epilogue;
   }
   const float memory = (((float)outputs + (float)tokens) * (float)width + 2.f * (float)outputs * (float)tokens) * (1.f / 6.2e6f);
-  return fmaxf(t, memory) + 0.205f * fminf(t, memory);
+  return fmaxf(t, memory) + 0.58f * fminf(t, memory);
 }
 
 // The current GPU's figures; null after an error.
