@@ -279,6 +279,29 @@ def test_same_bits_every_time(ops):
         assert all(torch.equal(ops.linear(x, w), first) for _ in range(5))
 
 
+@pytest.mark.parametrize("outputs,width", [(4096, 4096), (1000, 14336), (333, 2051), (130, 500)])
+def test_a_row_has_the_same_bits_in_every_batch(ops, outputs, width):
+    """Whatever tile, split or pairing a batch gets, with bias and residual."""
+    x, w = codes_rows(1100, width, 60), codes_rows(outputs, width, 61)
+    bias, residual = randn(outputs, seed=62), randn(1100, outputs, seed=63)
+    whole = ops.linear(x, w, bias=bias, residual=residual)
+    for lo, hi in ((0, 1), (1, 17), (17, 81), (81, 281), (281, 700), (500, 1100)):
+        part = Int8Rows(x.codes[lo:hi], x.scales[lo:hi])
+        assert torch.equal(ops.linear(part, w, bias=bias, residual=residual[lo:hi]), whole[lo:hi]), (lo, hi)
+
+
+@pytest.mark.parametrize("width", (64, 500, 4096, 5001, 14336))
+def test_a_row_has_the_same_codes_in_every_batch(ops, width):
+    """Rows of one layout: whatever number of them a call gets."""
+    x, u, r, w = randn(900, width, seed=64, outliers=True), randn(900, width, seed=65), randn(900, width, seed=66), randn(width, seed=67)
+    for call in (lambda lo, hi: ops.quantize_rows(x[lo:hi]), lambda lo, hi: ops.silu_mul(x[lo:hi], u[lo:hi]),
+                 lambda lo, hi: ops.rms_norm(x[lo:hi], w, 1e-6, residual=r[lo:hi])[0]):
+        whole = call(0, 900)
+        for lo, hi in ((0, 1), (0, 37), (0, 400), (400, 900)):
+            part = call(lo, hi)
+            assert torch.equal(part.codes, whole.codes[lo:hi]) and torch.equal(part.scales, whole.scales[lo:hi])
+
+
 # ---- together, and as programs use them ------------------------------------------------------------------------------
 
 def layer(ops, state, x, residual):
@@ -342,6 +365,30 @@ def test_captured_replayed_and_on_other_streams(ops):
     xs[1].copy_(xs[1].flip(0)), rs[1].copy_(rs[1].flip(0))
     graphs[1].replay()
     assert torch.equal(outs[1], wants[1].flip(0))
+    ops.module.check_device_error()
+
+
+def test_many_calls_at_once(ops):
+    """Three streams with calls of every kind in flight at the same time (clusters that split the width, two CTAs per SM, pairs, rows):
+    each gives what it gives alone."""
+    jobs = []
+    for i, (tokens, outputs, width) in enumerate(((1, 4096, 4096), (40, 2000, 8192), (300, 1000, 4096), (900, 4096, 1024), (16, 20000, 512),
+                                                  (2500, 3000, 640))):
+        x, w = codes_rows(tokens, width, 70 + i), codes_rows(outputs, width, 80 + i)
+        jobs.append((x, w, ops.linear(x, w)))
+    acts = randn(700, 8192, seed=90)
+    want = ops.quantize_rows(acts)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for turn in range(20):
+        for i, (x, w, y) in enumerate(jobs):
+            with torch.cuda.stream(streams[(turn + i) % 3]):
+                got.append((ops.linear(x, w), y))
+        with torch.cuda.stream(streams[turn % 3]):
+            got.append((ops.quantize_rows(acts).codes, want.codes))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in got)
     ops.module.check_device_error()
 
 
