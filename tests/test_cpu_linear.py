@@ -190,6 +190,54 @@ def test_models_without_such_layers_are_refused():
         int8_projections(wrapped, ExactOps())   # once is enough
 
 
+@pytest.mark.parametrize("what", ["scaled residual", "norm in the block", "factor of the block", "scaled norm", "layer norm", "hook",
+                                  "pre-hook", "own forward", "hook on a projection", "parameter", "buffer"])
+def test_layers_with_something_more_are_refused(what):
+    """What the wrapped layer would drop: it computes the plain decoder layer and nothing else."""
+    from triattention_b200.models import int8_projections
+    model = toy("Llama")
+    for layer in model.model.layers:
+        norm = layer.input_layernorm
+        if what == "scaled residual":
+            layer.residual_multiplier = 0.5
+        elif what == "norm in the block":
+            layer.mlp.inner_norm = torch.nn.RMSNorm(8)
+        elif what == "factor of the block":
+            layer.mlp.multiplier = 2.0
+        elif what == "scaled norm":
+            norm.bias = torch.nn.Parameter(torch.zeros_like(norm.weight))
+        elif what == "layer norm":
+            layer.input_layernorm = torch.nn.LayerNorm(norm.weight.shape[0])
+            layer.input_layernorm.variance_epsilon = 1e-6
+        elif what == "hook":
+            layer.register_forward_hook(lambda *a: None)
+        elif what == "pre-hook":
+            layer.mlp.register_forward_pre_hook(lambda *a: None)
+        elif what == "own forward":
+            layer.forward = lambda *a, **k: None
+        elif what == "hook on a projection":
+            layer.self_attn.q_proj.register_forward_hook(lambda *a: None)
+        elif what == "parameter":
+            layer.gain = torch.nn.Parameter(torch.ones(1))
+        elif what == "buffer":
+            layer.mlp.register_buffer("gain", torch.ones(1))
+    with pytest.raises(RuntimeError, match="no decoder layer"):
+        int8_projections(model, ExactOps())
+    assert all(type(layer.self_attn.q_proj) is torch.nn.Linear for layer in model.model.layers)
+
+
+def test_wrapped_layers_keep_the_mode():
+    from triattention_b200.models import int8_projections
+    model = toy("Llama").eval()
+    int8_projections(model, ExactOps())
+    assert not any(m.training for m in model.modules())
+
+
+def test_rows_without_a_feature_axis_are_refused(lib):
+    with pytest.raises(RuntimeError, match="rows of 1"):
+        Int8Ops(Module(lib)).quantize_rows(torch.zeros(()))
+
+
 def test_a_layer_used_twice_stays_one_layer():
     from triattention_b200.models import int8_projections
     model = toy("Llama")

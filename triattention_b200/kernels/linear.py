@@ -83,7 +83,7 @@ class Int8Rows:
 
 def _flat(x):
     """[..., H] as [T, H] (a view wherever the rows lie one stride apart)."""
-    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    return x if x.dim() in (0, 2) else x.reshape(-1, x.shape[-1])
 
 
 class Int8Ops:
@@ -234,19 +234,24 @@ class Int8DecoderLayer(torch.nn.Module):
         for name, value in vars(layer).items():         # what the model looks up on its layers (attention_type and the like)
             if not name.startswith("_") and name not in self.__dict__:
                 setattr(self, name, value)
+        self.train(layer.training)
 
     @staticmethod
     def fits(layer):
-        """Whether `layer` is built like that."""
-        linear = lambda m: type(m) is torch.nn.Linear
-        norm = lambda m: hasattr(m, "variance_epsilon") and getattr(m, "weight", None) is not None
+        """Whether `layer` is built like that, with nothing in it that would be lost: no module or factor more (scaled residuals,
+        norms inside the block), no hooks and no forward of an object's own on what is replaced."""
+        bare = lambda m: not ("forward" in vars(m) or m._forward_hooks or m._forward_pre_hooks)
+        plain = lambda m: bare(m) and not any(isinstance(v, (float, torch.Tensor)) for v in vars(m).values()) and not m._parameters and not m._buffers
+        linear = lambda m: type(m) is torch.nn.Linear and bare(m)
+        norm = lambda m: ("RMSNorm" in type(m).__name__ and hasattr(m, "variance_epsilon") and bare(m) and
+                          [n for n, w in m.named_parameters() if w is not None] == ["weight"])
         attention, mlp = getattr(layer, "self_attn", None), getattr(layer, "mlp", None)
-        return (attention is not None and mlp is not None and
+        return (isinstance(attention, torch.nn.Module) and isinstance(mlp, torch.nn.Module) and
                 all(linear(getattr(attention, n, None)) for n in ("q_proj", "k_proj", "v_proj", "o_proj")) and
                 all(linear(getattr(mlp, n, None)) for n in ("gate_proj", "up_proj", "down_proj")) and
                 type(getattr(mlp, "act_fn", None)).__name__ in ("SiLU", "SiLUActivation") and
                 all(norm(getattr(layer, n, None)) for n in ("input_layernorm", "post_attention_layernorm")) and
-                sum(1 for _ in layer.children()) == 4)
+                plain(layer) and plain(mlp) and len(layer._modules) == 4 and len(mlp._modules) == 4)
 
     def forward(self, hidden_states, **kwargs):
         ops = self.ops
