@@ -20,6 +20,7 @@
 #include "tcgen05.cuh"
 #include "abi_internal.h"
 #include <mutex>
+#include <type_traits>
 
 namespace tri {
 
@@ -145,15 +146,35 @@ __device__ __forceinline__ void lin_origin(const LinearArgs& p, int tile, int ch
 template <typename T, int C> struct LinVector {
   T v[C];
 };
-template <typename T, int C> __device__ __forceinline__ LinVector<T, C> lin_load(const T* from) {
-  LinVector<T, C> x;
-  constexpr int B = C * sizeof(T);
-  if constexpr (B == 16) *reinterpret_cast<uint4*>(x.v) = __ldcs(reinterpret_cast<const uint4*>(from));
-  else if constexpr (B == 8) *reinterpret_cast<uint2*>(x.v) = __ldcs(reinterpret_cast<const uint2*>(from));
-  else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(x.v) = __ldcs(reinterpret_cast<const uint32_t*>(from));
-  else x.v[0] = *from;
-  return x;
-}
+// The same as it is read ahead: 32-bit words, taken apart only where they are used.  (With elements of 16 bits the compiler takes
+// them apart right behind the load, which waits for it: 16384 x 4096 outputs of width 128 with a residual took 120 us, now 74; of width 4096 210 and 190.)
+template <typename T, int C> struct LinWords {
+  uint32_t w[(C * sizeof(T) + 3) / 4];
+  __device__ __forceinline__ void load(const T* from) {
+    constexpr int B = C * sizeof(T);
+    if constexpr (B == 16) *reinterpret_cast<uint4*>(w) = __ldcs(reinterpret_cast<const uint4*>(from));
+    else if constexpr (B == 8) *reinterpret_cast<uint2*>(w) = __ldcs(reinterpret_cast<const uint2*>(from));
+    else if constexpr (B == 4) w[0] = __ldcs(reinterpret_cast<const uint32_t*>(from));
+    else w[0] = *reinterpret_cast<const unsigned short*>(from);
+  }
+  __device__ __forceinline__ void load_some(const T* from, int count) {
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      uint32_t bits = 0;
+      if (k < count) {
+        if constexpr (sizeof(T) == 4) bits = *reinterpret_cast<const uint32_t*>(from + k);
+        else bits = *reinterpret_cast<const unsigned short*>(from + k);
+      }
+      if constexpr (sizeof(T) == 4) w[k] = bits;
+      else w[k / 2] = k % 2 ? w[k / 2] | bits << 16 : bits;
+    }
+  }
+  __device__ __forceinline__ float value(int k) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[k]);
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(k % 2 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(w[k / 2] >> (16 * (k % 2)))));
+  }
+};
 template <typename T, int C> __device__ __forceinline__ void lin_store(T* to, const LinVector<T, C>& x) {
   constexpr int B = C * sizeof(T);
   if constexpr (B == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(x.v);
@@ -167,7 +188,7 @@ template <typename T, int C> __device__ __forceinline__ void lin_store(T* to, co
 // block goes, 8 tokens at a time, through the warp's own shared memory, out of which a lane takes C neighbouring channels of a
 // token (C: what the rows of output and residual allow, 16 bytes at most), so that the residual is read and the result written in
 // wide accesses.  Two groups, because most of a tile's epilogue is latency (scales, the accumulators' barrier, TMEM, the residual):
-// they overlap those of two tiles (with a residual, 16384 x 4096 outputs of width 4096: 210 us, 249 with one group of all warps).
+// they overlap those of two tiles (with a residual, 16384 x 4096 outputs of width 4096: 249 us with one group of all warps, 210 with two).
 // `ready` is called once, when everything that does not depend on the sums is under way.
 constexpr int LinPitch = 36, LinBlockTokens = 8, LinBlockFloats = LinBlockTokens * LinPitch;   // pitch: no two lanes on one bank either way
 template <typename T, int C, int Warps, bool Residual, typename Ready>
@@ -182,19 +203,15 @@ __device__ __forceinline__ void lin_epilogue_as(const LinearArgs& p, uint32_t co
   const bool all = count >= C;
   const int64_t out_step = C * p.out_stride, residual_step = C * p.residual_stride;      // from pass to pass
   // the residual is asked for two blocks ahead (the first two under the MMAs): one trip to HBM outlasts a block by far
-  using Ahead = LinVector<T, C>[Residual ? Passes : 1];
+  using Ahead = LinWords<T, C>[Residual ? Passes : 1];
   Ahead even, odd;
   auto fetch = [&](Ahead& ahead, int c) {
     const T* from = static_cast<const T*>(p.residual) + (int64_t)(t0 + c + my_token) * p.residual_stride + my_n;
 #pragma unroll
     for (int i = 0; i < (Residual ? Passes : 0); ++i, from += residual_step) {
       if (c + i * C + my_token < valid) {
-        if (all) {
-          ahead[i] = lin_load<T, C>(from);
-        } else {
-#pragma unroll
-          for (int k = 0; k < C; ++k) if (k < count) ahead[i].v[k] = from[k];
-        }
+        if (all) ahead[i].load(from);
+        else ahead[i].load_some(from, count);
       }
     }
   };
@@ -243,7 +260,7 @@ __device__ __forceinline__ void lin_epilogue_as(const LinearArgs& p, uint32_t co
         }
         LinVector<T, C> x;
 #pragma unroll
-        for (int k = 0; k < C; ++k) x.v[k] = lin_out<T>(Residual ? y[k] + lin_in(ahead[Residual ? pass : 0].v[k]) : y[k]);
+        for (int k = 0; k < C; ++k) x.v[k] = lin_out<T>(Residual ? y[k] + ahead[Residual ? pass : 0].value(k) : y[k]);
         if (c + pass * C + my_token < valid) {
           if (all) {
             lin_store<T, C>(to, x);
