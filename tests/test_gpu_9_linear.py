@@ -166,6 +166,53 @@ def test_dequantize(ops, rows, width, dtype):
     assert out.dtype == dtype and torch.equal(out, (got.codes.float() * got.scales[:, None]).to(dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (2, 3), (5, 9), (700, 31), (33, 250), (700, 257), (400, 1003), (9, 2049), (320, 8195), (4, 9001),
+                                        (310, 16391), (3, 20001), (2, 33333)])
+def test_rows_that_start_anywhere(ops, rows, width, dtype):
+    """Inputs between NaN, outputs between guards: nothing beside a row is used, nothing beside it is written; in place too."""
+    def room(seed, off, fill):
+        whole = torch.full((rows + 2, width + 11), fill, dtype=dtype, device="cuda")
+        view = whole[1:-1, off:off + width]
+        view.copy_(randn(rows, width, seed=seed, dtype=dtype))
+        return whole, view
+
+    def code_room():
+        whole = torch.full((rows + 2, -(-width // 16) * 16 + 32), 99, dtype=torch.int8, device="cuda")
+        return whole, whole[1:-1, 16:16 + width], torch.empty(rows, device="cuda")
+
+    def beside(whole, view, fill):
+        view.fill_(fill)
+        assert bool((whole == fill).all())
+
+    nan, m = float("nan"), ops.module
+    (_, x), (_, u), (_, r) = room(70, 3, nan), room(71, 6, nan), room(72, 1, nan)
+    w = randn(width + 1, seed=73, dtype=dtype)[1:]
+    whole, codes, scales = code_room()
+    m.quantize_rows(x, codes, scales)
+    check_codes(Int8Rows(codes, scales), x.double())
+    values_room, values = room(0, 5, 7.0)
+    m.dequantize_rows(codes, scales, values)
+    assert torch.equal(values, (codes.float() * scales[:, None]).to(dtype))
+    beside(values_room, values, 7.0), beside(whole, codes, 99)
+    whole, codes, scales = code_room()
+    m.silu_mul_rows(x, u, codes, scales)
+    g = x.double()
+    check_codes(Int8Rows(codes, scales), g * torch.sigmoid(g) * u.double(), slack=(2 + 1.173 * float(g.abs().max()) + 2 + 1) * 2 * U)
+    beside(whole, codes, 99)
+    h = (x.float() + r.float()).to(dtype)
+    y = h.double() / (h.double().square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+    whole, codes, scales = code_room()
+    total_room, total = room(0, 2, 7.0)
+    m.rms_norm_rows(x, w, 1e-5, codes, scales, r, total)
+    check_codes(Int8Rows(codes, scales), y, slack=(8 + width / 256 + 16) * U)
+    assert torch.equal(total, h)
+    again, again_scales = code_room()[1:]
+    m.rms_norm_rows(x, w, 1e-5, again, again_scales, r, r)
+    assert torch.equal(r, h) and torch.equal(again, codes) and torch.equal(again_scales, scales)
+    beside(total_room, total, 7.0), beside(whole, codes, 99)
+
+
 # ---- products --------------------------------------------------------------------------------------------------------
 
 def codes_rows(rows, width, seed, low=-127, high=128, extra=0):

@@ -174,7 +174,7 @@ constexpr float GatedNear = 3e-6f, GatedFar = 1.2e-5f, GateNear = -16.f;
 constexpr float PlainError = 5e-7f;     // y * (1/s) against y / s: 2^-23 for the reciprocal, 2^-24 for product and quotient each, 2^-22
 constexpr float Round = 12582912.f;     // 1.5 * 2^23: x + Round has rint(x) in its low bits
 
-enum RowLayout : int { RowCta = 0, RowFull = 1, RowWarp = 2, RowElements = 3 };
+enum RowLayout : int { RowCta = 0, RowFull = 1, RowWarp = 2, RowAnywhere = 3 };
 
 // max(|a|, |b|, |c|); NaN where any is.
 __device__ __forceinline__ float max_magnitude(float a, float b, float c) {
@@ -269,7 +269,91 @@ template <typename T> struct RowVector {
   }
 };
 
-// The same out of line, for the few elements that need it.
+// ---- rows that start anywhere ---------------------------------------------------------------------------------------------
+// Memory is read and written in aligned blocks of 16 bytes, and vectors are shifted out of two neighbouring ones.  Blocks that reach
+// over an end of the tensor (of the row, where something is written) are taken element by element.  8192 x 4095 in single
+// elements, 2 bytes an access, and like this: plain 62 and 37 us, gated 91 and 66, norm with residual 140 and 92, values 65 and 30.
+// 16 bytes from byte `shift` (0..15) on of lo, hi.
+__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint32_t shift) {
+  uint32_t w[7] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z};
+  if (shift & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = hi.w; }
+  if (shift & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
+  const uint32_t bits = 8 * (shift & 3);
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                    __funnelshift_r(w[3], w[4], bits));
+}
+template <typename T> __device__ __forceinline__ uint32_t element_bits(const T* from) {
+  if constexpr (sizeof(T) == 4) return *reinterpret_cast<const uint32_t*>(from);
+  else return *reinterpret_cast<const unsigned short*>(from);
+}
+// The vector-th vector of a row of `width` elements; zero past its end.
+template <typename T> __device__ __forceinline__ uint4 load_anywhere(const T* row, int vector, int width) {
+  constexpr int N = 16 / sizeof(T), S = sizeof(T);
+  const uint32_t shift = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
+  const int before = shift / S, e = vector * N;             // elements of the block in front of the vector's first
+  const uint4* block = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row) + (int64_t)vector * 16 - shift);
+  if (shift == 0 ? e + N <= width : e >= before && e - before + 2 * N <= width) {
+    const uint4 lo = block[0];
+    return shift == 0 ? lo : shifted(lo, block[1], shift);
+  }
+  uint32_t w[4] = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (e + i < width) w[i * S / 4] |= element_bits(row + e + i) << (8 * (i * S % 4));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The vector that begins `shift` bytes into the block at `from`, in shared memory; zero from its live-th element on.
+template <typename T> __device__ __forceinline__ uint4 shared_vector(uint32_t from, uint32_t shift, int live) {
+  constexpr int N = 16 / sizeof(T), S = sizeof(T);
+  if (live <= 0) return make_uint4(0, 0, 0, 0);
+  uint4 v = load_shared(from);
+  if (shift != 0) v = shifted(v, load_shared(from + 16), shift);
+  if (live < N) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i >= live) w[i * S / 4] &= S == 4 ? 0u : i % 2 ? 0x0000ffffu : 0xffff0000u;
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+// The elements of a block that lie in [low, high).
+template <typename T> __device__ __forceinline__ void copy_elements(uint32_t to, const char* block, const char* low, const char* high) {
+#pragma unroll 1
+  for (int i = 0; i < 16; i += sizeof(T))
+    if (block + i >= low && block + i < high) {
+      if constexpr (sizeof(T) == 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + i), "r"(element_bits(reinterpret_cast<const T*>(block + i))) : "memory");
+      else asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + i), "h"((unsigned short)element_bits(reinterpret_cast<const T*>(block + i))) : "memory");
+    }
+}
+// Stores the vectors that a whole warp holds, lane l the one after lane l - 1's.  A lane writes the block that its vector begins in.
+template <typename T> __device__ __forceinline__ void store_anywhere(T* row, int vector, int width, const uint4& v) {
+  constexpr int N = 16 / sizeof(T), S = sizeof(T);
+  const uint32_t shift = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
+  const int lane = threadIdx.x % 32, before = shift / S, e = vector * N;
+  const uint4 last = make_uint4(__shfl_up_sync(0xffffffffu, v.x, 1), __shfl_up_sync(0xffffffffu, v.y, 1),
+                                __shfl_up_sync(0xffffffffu, v.z, 1), __shfl_up_sync(0xffffffffu, v.w, 1));
+  const uint4 block = shift == 0 ? v : shifted(last, v, 16 - shift);
+  const auto put = [&](const uint4& from, int i, int at) {   // element i of a block
+    const uint32_t w[4] = {from.x, from.y, from.z, from.w}, bits = w[i * S / 4] >> (8 * (i * S % 4));
+    if constexpr (S == 4) reinterpret_cast<uint32_t*>(row)[at] = bits;
+    else reinterpret_cast<unsigned short*>(row)[at] = (unsigned short)bits;
+  };
+  if ((before == 0 || lane > 0) && e - before + N <= width) {
+    *reinterpret_cast<uint4*>(reinterpret_cast<char*>(row) + (int64_t)vector * 16 - shift) = block;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i >= before || lane > 0) && e - before + i < width) put(block, i, e - before + i);
+  }
+  if (lane == 31) {                                          // the next lane is another warp's
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i >= N - before && e + i < width) put(v, i, e + i);
+  }
+}
+
+// gated() out of line, for the few elements that need it.
 __device__ __noinline__ float gated_exact(float gate, float up) { return gated(gate, up); }
 template <typename T> __device__ __forceinline__ float load_shared_element(uint32_t from) {
   if constexpr (sizeof(T) == 4) {
@@ -285,37 +369,55 @@ template <typename T> __device__ __forceinline__ float load_shared_element(uint3
 
 // RowCta: inputs start on 16-byte boundaries and hold whole vectors; a CTA per row, gridDim.x rows at a time, `depth` rows in
 // shared memory.  RowFull: the same where every thread has all of its vectors.  RowWarp: for short rows, a warp per row, four
-// per CTA.  RowElements: any alignment and width, a CTA per row, single elements.
+// per CTA.  RowAnywhere: any alignment and width, a CTA per row.
 template <typename T, int Mode, int V, int Layout> __global__ void __launch_bounds__(Layout == RowWarp ? 128 : 1024)
     rows_kernel(const RowArgs p, int depth) {
   constexpr int N = RowVector<T>::N;
-  constexpr bool Ring = Layout == RowCta || Layout == RowFull, Full = Layout == RowFull;
-  extern __shared__ uint4 ring[];       // [depth][a, b][V][thread]
+  constexpr bool Ring = Layout != RowWarp, Full = Layout == RowFull, Anywhere = Layout == RowAnywhere;
+  extern __shared__ uint4 ring[];       // [depth][a, b][V][thread]; RowAnywhere: [depth][a, b][V][warp][33 blocks]
   __shared__ RowShare share;
   grid_launch_dependents();
   grid_dependency_wait();
   const int threads = Layout == RowWarp ? 32 : blockDim.x, me = Layout == RowWarp ? threadIdx.x % 32 : threadIdx.x;
   const int64_t first = Layout == RowWarp ? (int64_t)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
   const int64_t stride = Layout == RowWarp ? (int64_t)gridDim.x * 4 : gridDim.x;
-  const int vectors = p.width / N;      // (not RowElements)
+  const int vectors = (p.width + N - 1) / N;
   const bool two = Mode == RowGated || (Mode == RowNorm && p.b != nullptr);
-  const auto element = [&](int j, int i) { return Layout == RowElements ? (j * N + i) * threads + me : (j * threads + me) * N + i; };
+  const auto element = [&](int j, int i) { return (j * threads + me) * N + i; };
   const auto mine = [&](int j) { return Full || j * threads + me < vectors; };     // whether this thread has a j-th vector
   const auto row_a = [&](int64_t row) { return static_cast<const T*>(p.a) + row * p.a_stride; };
   const auto row_b = [&](int64_t row) { return static_cast<const T*>(p.b) + row * p.b_stride; };
 
   // Every address below is a start that advances by row plus j * `step` bytes, on both sides of the copies: with products worked
   // out per vector the address arithmetic was a third of all instructions.
-  const int step = threads * 16, slot_bytes = (two ? 2 : 1) * V * step;
-  const uint32_t ring_start = smem_u32(ring) + me * 16, ring_end = ring_start + depth * slot_bytes;
+  const int step = threads * 16, ring_step = Anywhere ? threads / 32 * 33 * 16 : step, slot_bytes = (two ? 2 : 1) * V * ring_step;
+  const uint32_t ring_start = smem_u32(ring) + (me + (Anywhere ? me / 32 : 0)) * 16, ring_end = ring_start + depth * slot_bytes;
   const char *next_a = reinterpret_cast<const char*>(row_a(first)) + me * 16, *next_b = two ? reinterpret_cast<const char*>(row_b(first)) + me * 16 : nullptr;
   const int64_t advance_a = stride * p.a_stride * (int64_t)sizeof(T), advance_b = stride * p.b_stride * (int64_t)sizeof(T);
   int64_t next_row = first;
+  // RowAnywhere: the blocks that a warp's 32 vectors begin in, and the one after them (lane 31's).  A block may reach over the
+  // row's ends into the rows beside it, but not out of the tensor.
+  const auto bytes_of = [&](const char* base, int64_t row_stride) { return base + ((p.rows - 1) * row_stride + p.width) * (int64_t)sizeof(T); };
+  const char* const low_a = static_cast<const char*>(p.a);
+  const char* const low_b = static_cast<const char*>(p.b);
+  const auto copy_anywhere = [&](uint32_t to, const char* from, int vector, const char* low, int64_t row_stride) {
+    const char *row_end = from + (p.width - vector * N) * (int64_t)sizeof(T), *high = bytes_of(low, row_stride);
+    const char* block = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(from) & ~(uintptr_t)15);
+#pragma unroll
+    for (int extra = 0; extra < 2; ++extra, block += 16, to += 16)
+      if (block < row_end && (extra == 0 || me % 32 == 31)) {
+        if (block >= low && block + 16 <= high) copy_async(to, block);
+        else copy_elements<T>(to, block, low, high);
+      }
+  };
   const auto prefetch = [&](uint32_t slot) {     // the next row that has not been asked for
     if (next_row < p.rows) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (mine(j)) {
+        if constexpr (Anywhere) {
+          copy_anywhere(slot + j * ring_step, next_a + j * step, j * threads + me, low_a, p.a_stride);
+          if (two) copy_anywhere(slot + (V + j) * ring_step, next_b + j * step, j * threads + me, low_b, p.b_stride);
+        } else if (mine(j)) {
           copy_async(slot + j * step, next_a + j * step);
           if (two) copy_async(slot + (V + j) * step, next_b + j * step);
         }
@@ -328,52 +430,35 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
   RowVector<T> vw[V];                   // norm: this thread's part of the weight, which every row needs
   if constexpr (Mode == RowNorm && Ring && V <= 2) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) vw[j].raw = mine(j) ? __ldg(reinterpret_cast<const uint4*>(p.weight) + j * threads + me) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < V; ++j) {
+      if constexpr (Anywhere) vw[j].raw = load_anywhere(static_cast<const T*>(p.weight), j * threads + me, p.width);
+      else vw[j].raw = mine(j) ? __ldg(reinterpret_cast<const uint4*>(p.weight) + j * threads + me) : make_uint4(0, 0, 0, 0);
+    }
   }
 
   uint32_t slot = ring_start, parity = 0;
-  int8_t* codes = p.codes + first * p.codes_stride + (Layout == RowElements ? me : me * N);
-  char* sum = Mode == RowNorm && two ? reinterpret_cast<char*>(static_cast<T*>(p.sum) + first * p.sum_stride) + (Layout == RowElements ? 0 : me * 16) : nullptr;
+  int8_t* codes = p.codes + first * p.codes_stride + me * N;
+  char* sum = Mode == RowNorm && two ? reinterpret_cast<char*>(static_cast<T*>(p.sum) + first * p.sum_stride) + (Layout == RowAnywhere ? 0 : me * 16) : nullptr;
   const int64_t advance_codes = stride * p.codes_stride, advance_sum = stride * p.sum_stride * (int64_t)sizeof(T);
   for (int64_t row = first; row < p.rows; row += stride, codes += advance_codes, sum += advance_sum, parity ^= 1) {
     float y[V][N], squares = 0.f, largest = 0.f, lowest = 0.f;   // lowest: of the gates
     if constexpr (Ring) copy_wait(depth - 1);
-    if constexpr (Layout == RowElements) {
-      float r[V][N], w[V][N];
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int e = min(element(j, i), p.width - 1);      // (unconditional, so that all loads are under way at once)
-          y[j][i] = row_to_float(row_a(row)[e]);
-          if (two) r[j][i] = row_to_float(row_b(row)[e]);
-          if (Mode == RowNorm) w[j][i] = row_to_float(static_cast<const T*>(p.weight)[e]);
-        }
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int e = element(j, i);
-          const bool live = e < p.width;
-          if (Mode == RowGated) { lowest = fminf(lowest, y[j][i]); y[j][i] = gated_fast(y[j][i], r[j][i]); }
-          if (Mode == RowNorm) {
-            if (two) {
-              const T h = row_from_float<T>(y[j][i] + r[j][i]);
-              if (live) reinterpret_cast<T*>(sum)[e] = h;
-              y[j][i] = row_to_float(h);
-            }
-            if (!live) y[j][i] = 0.f;
-            squares = fmaf(y[j][i], y[j][i], squares);
-            y[j][i] *= w[j][i];
-          }
-          if (!live) y[j][i] = 0.f;
-        }
-    } else {
+    uint32_t shift_a = 0, shift_b = 0;  // RowAnywhere: from a block's start to the vector's
+    if constexpr (Anywhere) {
+      __syncwarp();                     // a vector reaches into the next lane's block
+      shift_a = (uint32_t)reinterpret_cast<uintptr_t>(row_a(row)) & 15u;
+      if (two) shift_b = (uint32_t)reinterpret_cast<uintptr_t>(row_b(row)) & 15u;
+    }
+    RowVector<T> held[Layout == RowAnywhere && Mode == RowNorm ? V : 1];      // h, until the whole row has been read (h may replace it)
+    {
       RowVector<T> va[V], vb[V];
       float2 squares2 = both(0.f);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if constexpr (Ring) {
+        if constexpr (Anywhere) {
+          va[j].raw = shared_vector<T>(slot + j * ring_step, shift_a, p.width - element(j, 0));
+          if (two) vb[j].raw = shared_vector<T>(slot + (V + j) * ring_step, shift_b, p.width - element(j, 0));
+        } else if constexpr (Ring) {
           va[j].raw = mine(j) ? load_shared(slot + j * step) : make_uint4(0, 0, 0, 0);
           if (two) vb[j].raw = mine(j) ? load_shared(slot + (V + j) * step) : make_uint4(0, 0, 0, 0);
         } else {
@@ -403,11 +488,13 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
             RowVector<T> h;
             h.pack(y[j]);
             h.unpack(y[j]);
-            if (mine(j)) *reinterpret_cast<uint4*>(sum + j * step) = h.raw;
+            if constexpr (Layout == RowAnywhere) held[j] = h;
+            else if (mine(j)) *reinterpret_cast<uint4*>(sum + j * step) = h.raw;
           }
         }
         if constexpr (Mode == RowNorm) {
-          if constexpr (!Ring || V > 2) vw[j].raw = mine(j) ? __ldg(reinterpret_cast<const uint4*>(p.weight) + j * threads + me) : make_uint4(0, 0, 0, 0);
+          if constexpr (Anywhere && V > 2) vw[j].raw = load_anywhere(static_cast<const T*>(p.weight), j * threads + me, p.width);
+          else if constexpr (!Ring || V > 2) vw[j].raw = mine(j) ? __ldg(reinterpret_cast<const uint4*>(p.weight) + j * threads + me) : make_uint4(0, 0, 0, 0);
           float w[N];
           vw[j].unpack(w);
 #pragma unroll
@@ -439,8 +526,8 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
               if (fabsf(y[j][i]) >= bar) {
                 float g, u;
                 if constexpr (Ring) {
-                  g = load_shared_element<T>(slot + j * step + i * (int)sizeof(T));
-                  u = load_shared_element<T>(slot + (V + j) * step + i * (int)sizeof(T));
+                  g = load_shared_element<T>(slot + j * ring_step + shift_a + i * (int)sizeof(T));
+                  u = load_shared_element<T>(slot + (V + j) * ring_step + shift_b + i * (int)sizeof(T));
                 } else {
                   g = row_to_float(row_a(row)[element(j, i)]);
                   u = row_to_float(row_b(row)[element(j, i)]);
@@ -451,6 +538,7 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
         peak = exact;
       }
     }
+    if constexpr (Anywhere) __syncwarp();
     if constexpr (Ring) {               // the row's inputs are in registers: its slot takes the row `depth` turns ahead
       prefetch(slot);
       slot += slot_bytes;
@@ -458,8 +546,14 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
     }
     if constexpr (Layout == RowWarp) peak = __reduce_max_sync(0xffffffffu, peak);
     else row_reduce<Mode == RowNorm>(squares, peak, share, parity);
+    if constexpr (Layout == RowAnywhere && Mode == RowNorm) {
+      if (two)
+#pragma unroll
+        for (int j = 0; j < V; ++j) store_anywhere(reinterpret_cast<T*>(sum), j * threads + me, p.width, held[j].raw);
+    }
     if constexpr (Mode == RowNorm) {
       if (!squares_fit(squares) && !(squares == 0.f && peak == 0)) {      // (the same for the whole CTA)
+        if constexpr (Layout == RowAnywhere) __syncthreads();      // (h has just been written)
         row_general<T, Mode>(p, row, two, share);
         __syncthreads();                // (it leaves either half in use)
         continue;
@@ -493,9 +587,9 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
           }
         }
       }
-      if constexpr (Layout == RowElements) {
+      if (Layout == RowAnywhere && element(j, N) > p.width) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) if (element(j, i) < p.width) codes[(j * N + i) * threads] = r.live ? (int8_t)c[i] : (int8_t)0;
+        for (int i = 0; i < N; ++i) if (element(j, i) < p.width) codes[j * threads * N + i] = r.live ? (int8_t)c[i] : (int8_t)0;
       } else if (mine(j)) {
         uint32_t w[N / 4];
 #pragma unroll
@@ -509,8 +603,8 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
 }
 
 // out = scale * code.  blockDim.x threads per row, blockDim.y rows per CTA at a time; a thread takes the codes of 16 bytes of
-// output where the output rows allow that (neighbouring threads then write neighbouring 16 bytes; 32 bytes a thread were 7 %
-// slower), else single ones.  Bound by HBM (the writes): no index is divided, a row's scale is read once.
+// output (neighbouring threads then write neighbouring 16 bytes; 32 bytes a thread were 7 % slower), shifted into place where the
+// output rows start anywhere.  Bound by HBM (the writes): no index is divided, a row's scale is read once.
 template <typename T, bool Vector> __global__ void __launch_bounds__(256) dequantize_rows_kernel(const int8_t* codes, int64_t codes_stride,
     const float* scales, T* out, int64_t out_stride, int64_t rows, int width) {
   grid_launch_dependents();
@@ -519,11 +613,30 @@ template <typename T, bool Vector> __global__ void __launch_bounds__(256) dequan
     const float scale = scales[row];
     const int8_t* from = codes + row * codes_stride;
     T* to = out + row * out_stride;
+    constexpr int N = RowVector<T>::N;
     if constexpr (!Vector) {
-#pragma unroll 4
-      for (int e = threadIdx.x; e < width; e += blockDim.x) to[e] = row_from_float<T>((float)from[e] * scale);
+      for (int base = threadIdx.x & ~31; N * base < width; base += blockDim.x) {      // (the same turns for a whole warp)
+        const int vector = base + threadIdx.x % 32, e = N * vector;
+        float x[N];
+        if (e + N <= width) {
+          uint32_t w[N / 4];
+          if constexpr (N == 8) {
+            const uint2 c = __ldcs(reinterpret_cast<const uint2*>(from + e));
+            w[0] = c.x; w[1] = c.y;
+          } else {
+            w[0] = __ldcs(reinterpret_cast<const uint32_t*>(from + e));
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4))) * scale;
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[i] = e + i < width ? (float)from[e + i] * scale : 0.f;
+        }
+        RowVector<T> v;
+        v.pack(x);
+        store_anywhere(to, vector, width, v.raw);
+      }
     } else {
-      constexpr int N = RowVector<T>::N;
 #pragma unroll 4
       for (int e = N * threadIdx.x; e < width; e += N * blockDim.x) {
         uint32_t w[N / 4];
@@ -552,12 +665,7 @@ template <typename T, int Mode, int V, int Layout> static int launch_rows_kernel
     TRI_CUDA(launch_chained(kernel, dim3((unsigned)((p.rows + 3) / 4)), dim3(128), 0, s, p, 1), "rows");
     return tri_launch_status("rows");
   }
-  const int items = Layout == RowElements ? p.width : p.width / N, each = Layout == RowElements ? V * N : V;
-  const int threads = ((items + each - 1) / each + 31) / 32 * 32;
-  if (Layout == RowElements) {
-    TRI_CUDA(launch_chained(kernel, dim3((unsigned)p.rows), dim3(threads), 0, s, p, 1), "rows");
-    return tri_launch_status("rows");
-  }
+  const int vectors = (p.width + N - 1) / N, threads = ((vectors + V - 1) / V + 31) / 32 * 32;
   static TriPerDevice configured;
   static std::atomic<int> registers{0};
   const int device = configured.pending();
@@ -570,8 +678,8 @@ template <typename T, int Mode, int V, int Layout> static int launch_rows_kernel
     configured.mark(device);
   }
   // resident CTAs per SM by threads, registers and shared memory, then the depth that the rest of the shared memory gives
-  const int row_bytes = (Mode != RowPlain && p.b != nullptr ? 2 : 1) * V * threads * 16;
-  int resident = 2048 / threads;
+  const int row_bytes = (Mode != RowPlain && p.b != nullptr ? 2 : 1) * V * (Layout == RowAnywhere ? threads / 32 * 33 : threads) * 16;
+  int resident = 2048 / threads < 32 ? 2048 / threads : 32;
   const int by_registers = 65536 / ((registers.load(std::memory_order_relaxed) + 7) / 8 * 8 * threads);
   if (by_registers < resident) resident = by_registers;
   if (RowShared / row_bytes < resident) resident = RowShared / row_bytes;
@@ -593,23 +701,27 @@ template <typename T, int Mode> static int launch_rows_type(const RowArgs& p, in
   constexpr int N = RowVector<T>::N;
   const auto vector_rows = [](const void* base, int64_t stride) { return aligned16(base) && stride % N == 0; };
   const int vectors = p.width / N;
+  // Vectors per thread.  One while there are few rows (a trip to memory and a reduction bound the call); for long batches as
+  // many as pay for what a thread does once a row, as few as keep warps on the SM.  Measured (us, 1 / 2 / 4 vectors): norm
+  // 16384 x 3584 with residual 73 / 76 / 81, 16384 x 8192 142 / 167 / 163; gated 8192 x 4096 51 / 43 / 39, 8192 x 8192
+  // 97 / 83 / 72, 8192 x 14336 146 / 147 / 129; plain 16384 x 4096 58 / 44 / 45, 16384 x 8192 116 / 83 / 79.
+  const int want = p.rows <= 2 * sms || Mode == RowNorm ? 1 : Mode == RowGated || vectors > 512 ? 4 : 2;
   if (p.width % N == 0 && vector_rows(p.a, p.a_stride) && vector_rows(p.b, p.b_stride) && vector_rows(p.weight, 0) &&
       vector_rows(p.sum, p.sum_stride) && vectors <= 4096) {
     if constexpr (Mode != RowNorm) {
       if (vectors <= 32) return launch_rows_kernel<T, Mode, 1, RowWarp>(p, sms, s);
       if (vectors <= 64) return launch_rows_kernel<T, Mode, 2, RowWarp>(p, sms, s);
     }
-    // Vectors per thread.  One while there are few rows (a trip to memory and a reduction bound the call); for long batches as
-    // many as pay for what a thread does once a row, as few as keep warps on the SM.  Measured (us, 1 / 2 / 4 vectors): norm
-    // 16384 x 3584 with residual 73 / 76 / 81, 16384 x 8192 142 / 167 / 163; gated 8192 x 4096 51 / 43 / 39, 8192 x 8192
-    // 97 / 83 / 72, 8192 x 14336 146 / 147 / 129; plain 16384 x 4096 58 / 44 / 45, 16384 x 8192 116 / 83 / 79.
-    const int want = p.rows <= 2 * sms || Mode == RowNorm ? 1 : Mode == RowGated || vectors > 512 ? 4 : 2;
     if (want == 1 && vectors <= 1024) return launch_rows_ring<T, Mode, 1>(p, sms, s);
     if (want <= 2 && vectors <= 2048) return launch_rows_ring<T, Mode, 2>(p, sms, s);
     return launch_rows_ring<T, Mode, 4>(p, sms, s);
   }
-  if (p.width <= 8192 / 8 * N) return launch_rows_kernel<T, Mode, 1, RowElements>(p, sms, s);
-  if (p.width <= 16384 / 8 * N) return launch_rows_kernel<T, Mode, 2, RowElements>(p, sms, s);
+  // Rows that start anywhere: four vectors do not fit into the registers beside the shifts.  1 / 2 / 4 vectors: plain 8192 x 4095
+  // 40 / 37 / 40, 16384 x 101 8.1 / 9.8 / 16; gated 8192 x 4095 75 / 66 / 95, 16384 x 101 12 / 19 / 39; norm with residual
+  // 8192 x 4095 92 / 111 / 141.
+  if ((want == 1 || vectors <= 32) && vectors < 1024) return launch_rows_kernel<T, Mode, 1, RowAnywhere>(p, sms, s);
+  if (vectors < 2048) return launch_rows_kernel<T, Mode, 2, RowAnywhere>(p, sms, s);
+  if (vectors < 4096) return launch_rows_kernel<T, Mode, 4, RowAnywhere>(p, sms, s);
   TRI_CUDA(launch_chained(rows_general_kernel<T, Mode>, dim3((unsigned)p.rows), dim3(1024), 0, s, p), "rows");
   return tri_launch_status("rows");
 }
@@ -638,7 +750,7 @@ template <int Mode> static int launch_rows(int type, const RowArgs& p, cudaStrea
 template <typename T> static int launch_values(const void* codes, int64_t codes_stride, const float* scales, int64_t rows, int width,
                                                void* out, int64_t out_stride, cudaStream_t s) {
   const bool vector = width % RowVector<T>::N == 0 && aligned16(out) && out_stride * sizeof(T) % 16 == 0;
-  const int items = vector ? width / RowVector<T>::N : width;
+  const int items = (width + RowVector<T>::N - 1) / RowVector<T>::N;
   int across = 32;
   while (across < 256 && across < items) across *= 2;
   const dim3 block((unsigned)across, (unsigned)(256 / across));
