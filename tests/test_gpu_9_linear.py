@@ -213,6 +213,20 @@ def test_rows_that_start_anywhere(ops, rows, width, dtype):
     beside(total_room, total, 7.0), beside(whole, codes, 99)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("stride", (0, 1, 3, 5, 9))
+def test_rows_that_overlap(ops, stride, dtype):
+    """One row for many, and windows of a sequence: rows less than 16 bytes apart."""
+    for width in (37, 515):
+        x = randn(9 * stride + width, seed=74, dtype=dtype).as_strided((10, width), (stride, 1))
+        u = randn(9 * stride + width, seed=75, dtype=dtype).as_strided((10, width), (stride, 1))
+        w = randn(width, seed=76, dtype=dtype)
+        for call in (lambda x, u: ops.quantize_rows(x), lambda x, u: ops.silu_mul(x, u), lambda x, u: ops.rms_norm(x, w, 1e-6, residual=u)[0]):
+            got, want = call(x, u), call(x.contiguous(), u.contiguous())
+            assert torch.equal(got.codes, want.codes)
+            torch.testing.assert_close(got.scales, want.scales, rtol=46 * U, atol=0)
+
+
 # ---- products --------------------------------------------------------------------------------------------------------
 
 def codes_rows(rows, width, seed, low=-127, high=128, extra=0):

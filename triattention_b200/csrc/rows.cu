@@ -272,15 +272,20 @@ template <typename T> struct RowVector {
 // ---- rows that start anywhere ---------------------------------------------------------------------------------------------
 // Memory is read and written in aligned blocks of 16 bytes, and vectors are shifted out of two neighbouring ones.  Blocks that reach
 // over an end of the tensor (of the row, where something is written) are taken element by element.  8192 x 4095 in single
-// elements, 2 bytes an access, and like this: plain 62 and 37 us, gated 91 and 66, norm with residual 140 and 92, values 65 and 30.
-// 16 bytes from byte `shift` (0..15) on of lo, hi.
+// elements, 2 bytes an access, and like this: plain 62 and 35 us, gated 91 and 59, norm with residual 140 and 87, values 65 and 30.
+// 16 bytes from byte `shift` (0..15) on of lo, hi.  (Four branches, one of which a whole row takes: 59 us for the gated rows above,
+// 65 with selects.)
 __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint32_t shift) {
-  uint32_t w[7] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z};
-  if (shift & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = hi.w; }
-  if (shift & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
   const uint32_t bits = 8 * (shift & 3);
-  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
-                    __funnelshift_r(w[3], w[4], bits));
+  const auto join = [bits](uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e) {
+    return make_uint4(__funnelshift_r(a, b, bits), __funnelshift_r(b, c, bits), __funnelshift_r(c, d, bits), __funnelshift_r(d, e, bits));
+  };
+  switch (shift >> 2) {
+    case 0: return join(lo.x, lo.y, lo.z, lo.w, hi.x);
+    case 1: return join(lo.y, lo.z, lo.w, hi.x, hi.y);
+    case 2: return join(lo.z, lo.w, hi.x, hi.y, hi.z);
+    default: return join(lo.w, hi.x, hi.y, hi.z, hi.w);
+  }
 }
 template <typename T> __device__ __forceinline__ uint32_t element_bits(const T* from) {
   if constexpr (sizeof(T) == 4) return *reinterpret_cast<const uint32_t*>(from);
@@ -317,8 +322,9 @@ template <typename T> __device__ __forceinline__ uint4 shared_vector(uint32_t fr
   }
   return v;
 }
-// The elements of a block that lie in [low, high).
-template <typename T> __device__ __forceinline__ void copy_elements(uint32_t to, const char* block, const char* low, const char* high) {
+// A block's elements that lie in [low, high).
+template <typename T> __device__ __noinline__ void copy_elements(uint32_t to, const char* block, const char* low, const char* high) {
+  if (block >= low && block + 16 <= high) { copy_async(to, block); return; }
 #pragma unroll 1
   for (int i = 0; i < 16; i += sizeof(T))
     if (block + i >= low && block + i < high) {
@@ -396,27 +402,28 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
   const int64_t advance_a = stride * p.a_stride * (int64_t)sizeof(T), advance_b = stride * p.b_stride * (int64_t)sizeof(T);
   int64_t next_row = first;
   // RowAnywhere: the blocks that a warp's 32 vectors begin in, and the one after them (lane 31's).  A block may reach over the
-  // row's ends into the rows beside it, but not out of the tensor.
-  const auto bytes_of = [&](const char* base, int64_t row_stride) { return base + ((p.rows - 1) * row_stride + p.width) * (int64_t)sizeof(T); };
-  const char* const low_a = static_cast<const char*>(p.a);
-  const char* const low_b = static_cast<const char*>(p.b);
-  const auto copy_anywhere = [&](uint32_t to, const char* from, int vector, const char* low, int64_t row_stride) {
-    const char *row_end = from + (p.width - vector * N) * (int64_t)sizeof(T), *high = bytes_of(low, row_stride);
-    const char* block = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(from) & ~(uintptr_t)15);
-#pragma unroll
-    for (int extra = 0; extra < 2; ++extra, block += 16, to += 16)
-      if (block < row_end && (extra == 0 || me % 32 == 31)) {
-        if (block >= low && block + 16 <= high) copy_async(to, block);
-        else copy_elements<T>(to, block, low, high);
-      }
+  // row's ends into the rows beside it, but not out of the tensor: the first and the last row are copied with care.
+  const auto copy_anywhere = [&](uint32_t to, const char* from, int vector, const void* base, int64_t row_stride) {
+    const int shift = (int)reinterpret_cast<uintptr_t>(from) & 15, past = vector * 16 - p.width * (int)sizeof(T);    // (of the row's end)
+    const char* block = from - shift;
+    const bool first_block = past < shift, extra_block = me % 32 == 31 && past + 16 < shift;
+    // Between two other rows neither block leaves the tensor.
+    if (next_row > 0 && next_row + 1 < p.rows && row_stride >= N) {
+      if (first_block) copy_async(to, block);
+      if (extra_block) copy_async(to + 16, block + 16);
+    } else {
+      const char *low = static_cast<const char*>(base), *high = low + ((p.rows - 1) * row_stride + p.width) * (int64_t)sizeof(T);
+      if (first_block) copy_elements<T>(to, block, low, high);
+      if (extra_block) copy_elements<T>(to + 16, block + 16, low, high);
+    }
   };
   const auto prefetch = [&](uint32_t slot) {     // the next row that has not been asked for
     if (next_row < p.rows) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if constexpr (Anywhere) {
-          copy_anywhere(slot + j * ring_step, next_a + j * step, j * threads + me, low_a, p.a_stride);
-          if (two) copy_anywhere(slot + (V + j) * ring_step, next_b + j * step, j * threads + me, low_b, p.b_stride);
+          copy_anywhere(slot + j * ring_step, next_a + j * step, j * threads + me, p.a, p.a_stride);
+          if (two) copy_anywhere(slot + (V + j) * ring_step, next_b + j * step, j * threads + me, p.b, p.b_stride);
         } else if (mine(j)) {
           copy_async(slot + j * step, next_a + j * step);
           if (two) copy_async(slot + (V + j) * step, next_b + j * step);
