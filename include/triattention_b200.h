@@ -314,7 +314,8 @@ int tri_qk_accumulators(const int32_t* requests, int num_requests, const void* q
 /* ---- INT8 projections: the matrix products around the attention (no counterpart in the reference, whose models run theirs
  * in bf16 through torch) -----------------------------------------------------------------------------------------------
  * Rows of codes: int8, symmetric, one f32 scale per row; a row stands for scale * code.  Code rows start on 16-byte
- * boundaries (base pointer and codes_stride, in bytes).  Element types of the other tensors: */
+ * boundaries (base pointer and codes_stride, in bytes); on 128-byte boundaries products are fastest.  Element types of the
+ * other tensors: */
 enum { TRI_BF16 = 0, TRI_FP16 = 1, TRI_FP32 = 2 };
 /* Strides are in elements, features contiguous; width 1..131071 (128 * 128 * width < 2^31); rows = 0 is a no-op.
  * scale = max|y| / 127, code = rint(y / scale).  A row whose largest magnitude is below 2^-119 gets scale 0 and codes 0; a row

@@ -4,7 +4,7 @@ import torch
 
 from triattention_b200.kernels import extension
 from triattention_b200.kernels.extension import MAX_WIDTH, Module, load_library
-from triattention_b200.kernels.linear import Int8Ops, Int8Rows
+from triattention_b200.kernels.linear import Int8Ops, Int8Rows, code_pitch
 
 P = 4096            # a 16-byte aligned address that a refused call never touches
 
@@ -115,6 +115,14 @@ def test_rows_of_codes_are_checked():
     for bad in ((codes.float(), torch.ones(2, 3)), (codes, torch.ones(2, 3).double()), (codes, torch.ones(6)), (codes, torch.ones(2, 3, 1))):
         with pytest.raises(RuntimeError, match="Int8Rows"):
             Int8Rows(*bad)
+
+
+def test_rows_that_calls_make_start_on_cache_lines():
+    for width, pitch in ((1, 16), (65, 80), (512, 512), (513, 640), (4096, 4096), (4099, 4224), (MAX_WIDTH, 131072)):
+        assert code_pitch(width) == pitch
+        rows = Int8Rows._empty(torch.zeros(3, width), 3, width, -1)
+        assert rows.pitch == pitch and rows.codes.shape == (3, width) and rows.codes.stride() == (pitch, 1)
+        assert rows.scales.shape == (3,) and rows.scales.data_ptr() == rows.codes_ptr + 3 * pitch == rows.scales_ptr
 
 
 def test_a_library_without_an_entry_point_asks_to_be_rebuilt(monkeypatch):

@@ -44,6 +44,7 @@ struct LinearArgs {
   int channel_tiles, tiles, group;                           // group: token tiles that share a sweep over the channels
   int splits;                                                // CTAs of a cluster that share a tile's width
   int shared;                                                // dynamic shared memory
+  int ahead;                                                 // steps whose weights are asked for before the kernel before this one has ended
   int* error;
 };
 
@@ -101,6 +102,9 @@ __device__ __forceinline__ void lin_commit(uint32_t bar) {
 }
 __device__ __forceinline__ void lin_prefetch(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+__device__ __forceinline__ void lin_prefetch_box(const CUtensorMap* map, int column, int row) {      // into L2
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(column), "r"(row) : "memory");
 }
 
 // The forms for a pair of CTAs.  Barrier addresses with the peer bit cleared name the even CTA's barrier at the same place.
@@ -314,7 +318,14 @@ __global__ void __launch_bounds__(lin_threads(Small ? LinSmallWarps : LinWarps),
     mbar_fence_init();
     abort_flag = 0;
   }
-  if (tid == 32) { lin_prefetch(&map_w); lin_prefetch(&map_x); }
+  if (tid == 32) {
+    lin_prefetch(&map_w); lin_prefetch(&map_x);
+    if (p.ahead > 0 && first < p.tiles) {
+      int n0, t0;
+      lin_origin(p, first, LinChannels, n0, t0);
+      for (int k = k0; k < min(k1, k0 + p.ahead); ++k) lin_prefetch_box(&map_w, k * LinDepth, n0);
+    }
+  }
   if (warp == 0) { tmem_alloc(&tmem_slot, p.columns); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
@@ -774,6 +785,12 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
   TRI_CHECK(tiles <= 0x7fffffff / 8, "int8_linear: tokens * outputs");
   p.tiles = (int)tiles;
   p.group = 8;
+  // Where a CTA's share of the weights is short, its first stages start on their way into L2 while the kernel that makes the
+  // tokens' codes still runs (L2 only, so whatever that kernel writes is what is read afterwards).
+  // quantize_rows and product, DRAM-cold weights: 1 x 4096 -> 4096 9.3 us, 8.5 like this; 64 tokens 12.0, 11.3.  With longer
+  // shares it is no gain (16 x 14336 -> 4096 17.4, 18.2).
+  const int share = ((width + LinDepth - 1) / LinDepth + plan.splits - 1) / plan.splits;
+  p.ahead = !plan.pair && tokens <= p.token_tile && share <= 8 ? (share < 5 ? share : 5) : 0;
   p.shared = !plan.pair && p.token_tile <= LinSmallTile ? LinSharedSmall : LinShared;
   // Two steps per stage where three stages of them fit: the issuing threads' work per stage is 0.1 us dearer than the MMAs of a
   // narrow tile (128 steps of 16 tokens: 38 us, 29 with two per stage; 16384 x 14336 -> 4096 in pairs: 649 us, 602).
