@@ -257,6 +257,7 @@ SHAPES = [(1, 1, 1), (1, 17, 33), (2, 8, 16), (3, 128, 64), (7, 130, 127), (1, 4
           (16, 1000, 4099), (17, 129, 160), (31, 384, 8192), (32, 4608, 3584), (33, 96, 96), (64, 300, 1000), (65, 127, 2000),
           (100, 2000, 500), (127, 640, 2048), (128, 128, 128), (129, 257, 2051), (200, 1111, 777), (255, 256, 512), (256, 4096, 1024),
           (257, 513, 130), (300, 1000, 100), (511, 384, 384), (512, 512, 512), (777, 1003, 1051), (1000, 640, 512), (1500, 2048, 256),
+          (1, 9001, 4099), (1, 5000, 2047), (1, 30001, 31), (1, 40, 131071), (1, 3, 2), (1, 700, 14336),
           (2049, 1025, 129), (4096, 512, 640), (3, 20000, 48), (5000, 3, 48), (700, 5000, 17), (2, 2, 30000), (24, 24, 131071)]
 
 

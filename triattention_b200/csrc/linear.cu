@@ -4,8 +4,8 @@
 // depend on the order of the additions (nor on how the width is split).  The rest is fp32, rounded once.
 //
 // tcgen05 kind::i8 with the WEIGHTS as the 128-row operand and the tokens as the N of the MMA: N goes from 16 to 256 in steps of
-// 16, so a decode step of one to 256 tokens is one tile of tokens that fits it, and the weights (what such a step is bound by)
-// are read once.  TMEM lane = channel, TMEM column = token.
+// 16, so a decode step of two to 256 tokens is one tile of tokens that fits it, and the weights (what such a step is bound by)
+// are read once (a single token has a kernel of its own, linear_row_kernel).  TMEM lane = channel, TMEM column = token.
 //   warp 0      producer: TMA copies of the weights' and tokens' 128-byte columns (128-byte swizzle, edges zero-filled)
 //   warp 1      issues the MMAs (one elected thread), accumulators alternate between two TMEM buffers
 //   warps 2-    epilogue: TMEM -> scales, bias, residual -> global, while the next tiles' MMAs run
@@ -14,8 +14,8 @@
 // the result has the same bits whatever else is in the batch: only the exact sums depend on tile and split.
 // Every wait on a barrier is bounded; after one has run out the CTA runs through, reports it and its output is void.
 //
-// Measured on one B200 (device time; DRAM-cold weights): 16 x 4096 -> 128256 fp32 84 us = 6.3 TB/s, bound by HBM; 1 x 4096 -> 6144
-// 8.5-9.7 us depending on the GPU, bound by latencies (launch, first bytes, cluster exchange; a 1 x 128 -> 128 product takes 2.7);
+// Measured on one B200 (device time; DRAM-cold weights): 16 x 4096 -> 128256 fp32 84 us = 6.3 TB/s, bound by HBM; 32 x 3584 -> 4608
+// 8.2-9.0 us depending on the GPU, bound by latencies (launch, first bytes, cluster exchange; 2.7 for the smallest product);
 // 16384 x 14336 -> 4096 with residual 602-632 us = 3.0-3.2 POP/s in bursts, bound by the 1000 W limit when it runs for seconds.
 #include "tcgen05.cuh"
 #include "abi_internal.h"
@@ -600,6 +600,83 @@ __global__ void __launch_bounds__(lin_threads(LinWarps), 1)
   if (warp == 0) pair_dealloc(tmem, p.columns);
 }
 
+// One token: a warp per channel, whose codes it reads once, 16 bytes a lane, four products an instruction.  No tensor core, no TMEM,
+// no cluster: a call is the trip to memory and one reduction across the warp.  `Ahead` loads of a lane are under way at a time, twice
+// as many in the Deep form, which takes registers that more than 32 warps an SM do not have.  Measured (us, DRAM-cold weights, with
+// the quantisation before it; tensor cores / this / this, Deep): 4096 -> 6144 11.3 / 7.7 / 8.0, 4096 -> 4096 8.5 / 6.1 / 5.9,
+// 14336 -> 4096 17.4 / 15.3 / 13.7, 14336 -> 256 10.2 / 11.9 / 9.9, 4096 -> 28672 24.0 / 22.3 / 23.0, 4096 -> 128256 84 / 79 / 90.
+// Alone 4096 -> 6144 takes 4.6 us (5.4 TB/s), 9.6 on the tensor cores.  Two tokens are faster there already (4096 -> 28672: 24.0 us,
+// 28.6 like this).
+constexpr int LinRowWarps = 4, LinRowDeep = 32;               // LinRowDeep: warps an SM up to which the Deep form is taken
+__device__ __forceinline__ uint4 row_end_codes(const int8_t* from, int count) {     // the last 1..15 codes of a row, then zeros
+  uint32_t w[4] = {};
+#pragma unroll
+  for (int i = 0; i < 15; ++i) if (i < count) w[i / 4] |= (uint32_t)(uint8_t)from[i] << (8 * (i % 4));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int sum) {
+  sum = __dp4a((int)a.x, (int)b.x, sum);
+  sum = __dp4a((int)a.y, (int)b.y, sum);
+  sum = __dp4a((int)a.z, (int)b.z, sum);
+  return __dp4a((int)a.w, (int)b.w, sum);
+}
+template <typename T, bool Deep> __global__ void __launch_bounds__(32 * LinRowWarps)
+    linear_row_kernel(const int8_t* codes, const int8_t* weight, int64_t weight_stride, const __grid_constant__ LinearArgs p) {
+  constexpr int Ahead = 4, Step = 512, Chunk = Ahead * Step;  // Step: bytes that a warp reads at a time
+  const int lane = threadIdx.x % 32, whole = p.width & ~15;
+  const int64_t step = (int64_t)gridDim.x * LinRowWarps;
+  int64_t n = (int64_t)blockIdx.x * LinRowWarps + threadIdx.x / 32;
+  grid_launch_dependents();
+  if (n < p.outputs)                                          // into L2 only, under the kernel that makes the codes
+    for (int e = lane * 128; e < min(p.width, 4096); e += 4096)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(weight + n * weight_stride + e));
+  grid_dependency_wait();
+  const float st = p.scales[0];
+  for (; n < p.outputs; n += step) {
+    const int8_t* row = weight + n * weight_stride;
+    const auto fetch = [&](uint4 (&w)[Ahead], int e) {
+#pragma unroll
+      for (int a = 0; a < Ahead; ++a) {
+        w[a] = make_uint4(0, 0, 0, 0);
+        if (e + a * Step < whole) w[a] = __ldcs(reinterpret_cast<const uint4*>(row + e + a * Step));
+      }
+    };
+    int sum = 0;
+    const auto work = [&](const uint4 (&w)[Ahead], int e) {
+      uint4 c[Ahead];
+#pragma unroll
+      for (int a = 0; a < Ahead; ++a) {
+        c[a] = make_uint4(0, 0, 0, 0);
+        if (e + a * Step < whole) c[a] = *reinterpret_cast<const uint4*>(codes + e + a * Step);
+      }
+#pragma unroll
+      for (int a = 0; a < Ahead; ++a) sum = dot16(c[a], w[a], sum);
+    };
+    const float sw = p.weight_scales[n], bias = p.bias != nullptr ? lin_in(static_cast<const T*>(p.bias)[n]) : 0.f;
+    const float r = p.residual != nullptr ? lin_in(static_cast<const T*>(p.residual)[n]) : 0.f;
+    uint4 even[Ahead], odd[Ahead];
+    if constexpr (Deep) {
+      fetch(even, lane * 16);
+      for (int e = lane * 16; e < whole; e += 2 * Chunk) {
+        fetch(odd, e + Chunk);
+        work(even, e);
+        fetch(even, e + 2 * Chunk);
+        work(odd, e + Chunk);
+      }
+    } else {
+      for (int e = lane * 16; e < whole; e += Chunk) {
+        fetch(even, e);
+        work(even, e);
+      }
+    }
+    if (whole < p.width && lane == 31) sum = dot16(row_end_codes(codes + whole, p.width - whole), row_end_codes(row + whole, p.width - whole), sum);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    float y = fmaf(__fmul_rn((float)sum, sw), st, bias);      // (the other kernels' arithmetic)
+    if (p.residual != nullptr) y += r;
+    if (lane == 0) static_cast<T*>(p.out)[n] = lin_out<T>(y);
+  }
+}
+
 // int8 rows: box = `box` rows x 128 bytes, 128-byte swizzle; what lies past the last row or the width reads as zero.
 static int make_code_map(CUtensorMap* map, const void* base, int64_t rows, int width, int64_t stride, unsigned box) {
   EncodeTiled enc = encode_fn();
@@ -643,6 +720,15 @@ template <typename T> static int launch_linear(const CUtensorMap& map_w, const C
   if (channels == Widest) return launch_linear_as<T, Widest>(map_w, map_x, p, ctas, pair, deep, s);
   if (channels == 2) return launch_linear_as<T, 2>(map_w, map_x, p, ctas, pair, deep, s);
   return launch_linear_as<T, 1>(map_w, map_x, p, ctas, pair, deep, s);
+}
+
+template <typename T> static int launch_row(const void* codes, const void* weight, int64_t weight_stride, const LinearArgs& p, int sms, cudaStream_t s) {
+  const bool deep = p.outputs <= LinRowDeep * sms;
+  const int ctas = (p.outputs + LinRowWarps - 1) / LinRowWarps, most = sms * (48 / LinRowWarps);
+  TRI_CUDA(launch_chained(deep ? linear_row_kernel<T, true> : linear_row_kernel<T, false>, dim3((unsigned)(ctas < most ? ctas : most)),
+                          dim3(32 * LinRowWarps), 0, s, static_cast<const int8_t*>(codes), static_cast<const int8_t*>(weight), weight_stride, p),
+           "int8_linear");
+  return tri_launch_status("int8_linear");
 }
 
 // ---- which tile, how many CTAs per tile --------------------------------------------------------------------------------
@@ -767,11 +853,16 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
   TRI_CHECK(out_stride >= outputs && (residual == nullptr || residual_stride >= 0), "int8_linear: output and residual rows");
   const LinearDevice* gpu = linear_device();
   if (gpu == nullptr) return TRI_ERR_CUDA;
-  const LinearPlan plan = choose_plan(tokens, outputs, width, *gpu);
-
   LinearArgs p{};
   p.residual_stride = residual_stride; p.out_stride = out_stride; p.scales = scales; p.weight_scales = weight_scales;
   p.bias = bias; p.residual = residual; p.out = out; p.tokens = (int)tokens; p.outputs = outputs; p.width = width; p.error = device_error;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (tokens == 1) {
+    if (type == TRI_BF16) return launch_row<__nv_bfloat16>(codes, weight, weight_stride, p, gpu->sms, s);
+    if (type == TRI_FP16) return launch_row<__half>(codes, weight, weight_stride, p, gpu->sms, s);
+    return launch_row<float>(codes, weight, weight_stride, p, gpu->sms, s);
+  }
+  const LinearPlan plan = choose_plan(tokens, outputs, width, *gpu);
   p.token_tile = plan.token_tile; p.splits = plan.splits;
   const auto rows_allow = [&](int channels) {                // accesses of so many channels to the rows of output and residual
     const int64_t bytes = channels * (int64_t)cell;
@@ -806,7 +897,6 @@ extern "C" int tri_int8_linear(const void* codes, int64_t codes_stride, const fl
   CUtensorMap map_w, map_x;
   if (make_code_map(&map_w, weight, outputs, width, weight_stride, LinChannels) != TRI_OK) return TRI_ERR_CUDA;
   if (make_code_map(&map_x, codes, tokens, width, codes_stride, (unsigned)box) != TRI_OK) return TRI_ERR_CUDA;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (type == TRI_BF16) return launch_linear<__nv_bfloat16>(map_w, map_x, p, ctas, each, plan.pair, deep, s);
   if (type == TRI_FP16) return launch_linear<__half>(map_w, map_x, p, ctas, each, plan.pair, deep, s);
   return launch_linear<float>(map_w, map_x, p, ctas, each, plan.pair, deep, s);
