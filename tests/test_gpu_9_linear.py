@@ -587,3 +587,35 @@ def test_on_another_device_than_the_current_one(ops):
         return Int8Rows(codes.copy_(rows.codes), rows.scales.to("cuda:1"))
 
     assert torch.equal(ops.linear(move(x), move(w)).cpu(), ops.linear(x, w).cpu())
+
+
+# ---- the norm's second try -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", (BF16, FP32))
+@pytest.mark.parametrize("rows,width", [(5, 8), (700, 24), (300, 128), (300, 256), (5, 1024), (300, 4096), (3, 8704), (3, 16384), (2, 40000)])
+@pytest.mark.parametrize("size", (1e30, 1e19, 1e-15, 1e-30))
+def test_norm_of_aligned_rows_whose_squares_leave_fp32(ops, rows, width, size, dtype):
+    """Rows of one warp and of many, with a residual: the second try reads the new residual that other threads have just written.
+    Between rows that fit, beside rows that hold a NaN or an infinity, and in place."""
+    x, r = ((randn(rows, width, seed=s, dtype=FP32) * size).to(dtype) for s in (110, 111))
+    x[1::4], r[1::4] = randn(rows, width, seed=112, dtype=dtype)[1::4], randn(rows, width, seed=113, dtype=dtype)[1::4]
+    w = (1 + 0.1 * randn(width, seed=114, dtype=FP32)).to(dtype)
+    if rows > 3:
+        x[2, width // 3], r[3, width - 1] = float("nan"), float("-inf")
+    h = (x.float() + r.float()).to(dtype)
+    good = torch.isfinite(h).all(1)
+    wide = h.double()[good]
+    y = wide / (wide.square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+
+    def check(rows_of_codes, total):
+        assert torch.equal(total.view(torch.int16 if dtype == BF16 else torch.int32)[good], h.view(torch.int16 if dtype == BF16 else torch.int32)[good])
+        assert torch.isnan(rows_of_codes.scales[~good]).all() and not rows_of_codes.codes[~good].any()
+        check_codes(Int8Rows(rows_of_codes.codes[good], rows_of_codes.scales[good]), y, slack=(8 + width / 256 + 16) * U)
+
+    got, total = ops.rms_norm(x, w, 1e-6, residual=r)
+    check(got, total)
+    for place in ("residual", "x"):             # the new residual over the old one, or over x
+        x2, r2 = x.clone(), r.clone()
+        codes, scales = torch.empty(rows, -(-width // 16) * 16, dtype=torch.int8, device="cuda")[:, :width], torch.empty(rows, device="cuda")
+        ops.module.rms_norm_rows(x2, w, 1e-6, codes, scales, r2, r2 if place == "residual" else x2)
+        check(Int8Rows(codes, scales), r2 if place == "residual" else x2)

@@ -560,7 +560,8 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
     }
     if constexpr (Mode == RowNorm) {
       if (!squares_fit(squares) && !(squares == 0.f && peak == 0)) {      // (the same for the whole CTA)
-        if constexpr (Layout == RowAnywhere) __syncthreads();      // (h has just been written)
+        __syncthreads();                // other threads' h has just been written; the reduction's own barrier comes before it
+                                        // (RowAnywhere) or is left out (a row of one warp: shuffles order no memory)
         row_general<T, Mode>(p, row, two, share);
         __syncthreads();                // (it leaves either half in use)
         continue;
