@@ -619,3 +619,90 @@ def test_norm_of_aligned_rows_whose_squares_leave_fp32(ops, rows, width, size, d
         codes, scales = torch.empty(rows, -(-width // 16) * 16, dtype=torch.int8, device="cuda")[:, :width], torch.empty(rows, device="cuda")
         ops.module.rms_norm_rows(x2, w, 1e-6, codes, scales, r2, r2 if place == "residual" else x2)
         check(Int8Rows(codes, scales), r2 if place == "residual" else x2)
+
+
+# ---- codes next to a tie -------------------------------------------------------------------------------------------------
+
+# Every way through the row kernels: a warp a row, one warp a row with a ring, several warps (whole and with a remainder), two and
+# four vectors a thread, rows that start anywhere, rows too wide for registers; a few rows and long batches.
+TIE_SHAPES = [(5, 8), (3, 24), (700, 256), (900, 512), (5, 777), (400, 1000), (3, 4096), (500, 4096), (700, 4095), (2, 9000),
+              (400, 8704), (2, 14336), (310, 14336), (310, 16391), (2, 40000)]
+
+
+def rows_of_ties(rows, width, seed):
+    """Whole numbers of which the largest is 254, so that every odd one's quotient, y / 2, lies on a tie."""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    y = torch.randint(-253, 254, (rows, width), generator=gen, device="cuda").float()
+    y[torch.arange(rows), torch.randint(0, width, (rows,), generator=gen, device="cuda")] = 254
+    return y
+
+
+def fp32_codes(y):
+    """Scales and codes of y as the formulas have them, each operation in IEEE fp32: s = max|y| * fl(1/127), rint(y / s)."""
+    assert y.dtype == FP32
+    scales = y.abs().amax(1) * torch.tensor(1 / 127, device="cuda")
+    return scales, torch.round(y / scales[:, None]).to(torch.int8)
+
+
+def silu_mul_fp32(gate, up):
+    """gate / (1 + e^-gate) * up in IEEE fp32; zero where the sum passes 2^126, as the kernels have it."""
+    g, u = gate.float(), up.float()
+    d = 1 + torch.exp(-g)
+    return torch.where(d > 2.0 ** 126, 0 * g * u, g / d * u)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", TIE_SHAPES)
+def test_plain_codes_are_those_of_fp32(ops, rows, width, dtype):
+    """Bit for bit: on rows full of ties (where s = fl(fl(1/127) * 254) decides the side), and on rows as they come."""
+    for y in (rows_of_ties(rows, width, 90), 1.4140625 * rows_of_ties(rows, width, 91), randn(rows, width, seed=92, dtype=FP32, outliers=True)):
+        x = y.to(dtype)
+        got, (scales, codes) = ops.quantize_rows(x), fp32_codes(x.float())
+        assert torch.equal(got.scales, scales) and torch.equal(got.codes, codes)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", TIE_SHAPES)
+def test_gated_codes_are_those_of_fp32(ops, rows, width, dtype):
+    """Bit for bit, although most elements go by a fast exponential.  From a gate of 18 on 1 + e^-gate is 1 in fp32, so gates of 32 give
+    y = 32 up: rows full of ties.  Then gates as they come, gates below -16 (where the exponential's error is largest) and beyond
+    -87.3 (where the product counts as zero), and rows of nothing else."""
+    gen = torch.Generator("cuda").manual_seed(93)
+    ties = rows_of_ties(rows, width, 94) / 32
+    spread = 90 * torch.rand(rows, width, generator=gen, device="cuda") * torch.where(torch.rand(rows, width, generator=gen, device="cuda") < 0.7, -1, 1)
+    far = -14 - 70 * torch.rand(rows, width, generator=gen, device="cuda")
+    for gate, up in ((torch.full_like(ties, 32), ties), (torch.full_like(ties, 32), 1.4140625 * ties),
+                     (3 * randn(rows, width, seed=95, dtype=FP32), randn(rows, width, seed=96, dtype=FP32, outliers=True)),
+                     (spread, randn(rows, width, seed=97, dtype=FP32)), (far, randn(rows, width, seed=98, dtype=FP32) * 1e20 if dtype != FP16 else ties)):
+        gate, up = gate.to(dtype), up.to(dtype)
+        y = silu_mul_fp32(gate, up)
+        got, (scales, codes) = ops.silu_mul(gate, up), fp32_codes(y)
+        live = y.abs().amax(1) >= 2.0 ** -119
+        assert bool(live.any()) and torch.equal(got.scales, torch.where(live, scales, 0.0))
+        assert torch.equal(got.codes, torch.where(live[:, None], codes, 0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", TIE_SHAPES)
+@pytest.mark.parametrize("residual", (False, True))
+def test_norm_codes_next_to_ties(ops, rows, width, dtype, residual):
+    """A norm's code is the nearest to q = 127 y / max|y|, y = fl(h * weight), up to the fp32 roundings between them, in steps of 2^-24:
+    fl(1/127) and its product half a step each (1 + 1 of 2^-24), the approximate reciprocal one step (2), the product (1).  On a tie
+    either neighbour is as near.  Every row of ties, powers of two in front of it that send its squares out of fp32's range, rows
+    as they come."""
+    y = rows_of_ties(rows, width, 99)
+    gen = torch.Generator("cuda").manual_seed(100)
+    w = 2.0 ** torch.randint(-1, 2, (width,), generator=gen, device="cuda")
+    cases = [(y / w * 2.0 ** power, factor * w, torch.round(y / w) * 2.0 ** power)    # h - r is a half at most: exact in every type
+             for power, factor in (((0, 1), (-30, 1.4140625), (66, 1.0078125), (-66, 1.7265625)) if dtype != FP16 else ((0, 1), (5, 1.4140625)))]
+    cases.append((randn(rows, width, seed=101, dtype=FP32, outliers=True), 1 + 0.1 * randn(width, seed=102, dtype=FP32), 3 * randn(rows, width, seed=103, dtype=FP32)))
+    for h, weight, r in cases:
+        x, weight, r = (h - r if residual else h).to(dtype), weight.to(dtype), r.to(dtype)
+        got = ops.rms_norm(x, weight, 1e-6, residual=r if residual else None)
+        if residual:
+            x = (x.float() + r.float()).to(dtype)
+            assert torch.equal(got[1], x)
+            got = got[0]
+        z = (x.float() * weight.float()).double()
+        q = z * 127 / z.abs().amax(1, keepdim=True)
+        assert float(((got.codes.double() - q).abs() - q.abs() * 5 * U).max()) <= 0.5

@@ -7,11 +7,16 @@
 //
 // A row of zeros has scale 0 and codes 0; so has one whose largest magnitude is below 2^-119, where max/127 would leave the
 // range of normal floats.  A row that holds a NaN or an infinity, or whose y overflows, has scale NaN and codes 0: every product
-// that reads it is NaN, and no other row is touched by it.
-// All arithmetic is IEEE fp32 (this file is compiled without --use_fast_math): the codes of plain and gated rows are, bit for
-// bit, rint(y / s) of the formulas above with s = max|y| * fl(1/127) and CUDA's expf.  A row's largest element can be eighty
-// times its root mean square, so a code that is off by one step where y / s is next to a tie would be off by more than half
-// of that.  h is rounded to the stream's type before it is normed, because that is what later layers read.
+// that reads it is NaN, and no other row is touched by it.  (Of a norm, |y| here is |h * w|, before the root divides it.)
+// Plain and gated rows: codes and scales are, bit for bit, rint(y / s) and s = max|y| * fl(1/127) of the formulas above in IEEE fp32
+// with CUDA's expf (the file is compiled without --use_fast_math).  Approximate instructions are used on the way, but every
+// element whose code they might change is worked out again.  A row's largest element can be eighty times its root mean square, so a
+// code that is off by one step where y / s is next to a tie would be off by more than half of that.
+// Normed rows: the code is rint of h * w times the approximate reciprocal of max|h * w| / 127.  It is the nearest code up to the
+// roundings in between, 5 * 2^-24 of the quotient (|code - quotient| <= 1/2 + 3.8e-5); on a tie, which exact products of 16-bit
+// numbers do meet, it may be either neighbour, both of which are as far from y.  Deciding ties as exact arithmetic does changed 183
+// of 58.7 million codes of 16384 x 3584 and took 80 us for 74 (71 for 53 without a residual).  The scale's root is approximate too
+// (2^-22.9).  h is rounded to the stream's type before it is normed, because that is what later layers read.
 #include "common.cuh"
 #include "abi_internal.h"
 #include <type_traits>
