@@ -299,3 +299,50 @@ def test_infer_flag(monkeypatch):
         monkeypatch.setattr(sys, "argv", ["infer", "--model", "m", "--prompt", "p", *flags])
         infer.main()
         assert done == want
+
+
+# ---- copies --------------------------------------------------------------------------------------------------------------
+
+def copies(rows):
+    import copy
+    import io
+    import pickle
+    saved = io.BytesIO()
+    torch.save(rows, saved)
+    saved.seek(0)
+    yield "deepcopy", copy.deepcopy(rows)
+    yield "pickle", pickle.loads(pickle.dumps(rows))
+    yield "save", torch.load(saved, weights_only=False)
+    yield "copy", copy.copy(rows)
+
+
+def test_copied_and_saved_rows_hold_their_own_memory():
+    """Calls read rows by address: a copy's addresses are those of the copy's tensors, and its pitch theirs."""
+    made = Int8Rows._empty(torch.zeros(2, 3, 600, dtype=torch.float16), 6, 600, -1)      # as a call makes them, 640 bytes apart
+    made._buffer.copy_(torch.arange(made._buffer.numel()) % 61)
+    pitched = torch.arange(5 * 64).reshape(5, 64).to(torch.int8)
+    for rows in (made, Int8Rows(pitched[:, :50], torch.arange(5.0)), Int8Rows(pitched[2], torch.tensor(3.0), torch.float32),
+                 Int8Rows(pitched[:, :50].view(5, 1, 50), torch.ones(5, 1)), Int8Rows(pitched[:0], torch.ones(0)),
+                 Int8Rows(pitched[:, 1:50], torch.ones(5)),                              # (this one is refused by the calls)
+                 Int8Rows(made.codes[:1], made.scales[:1])):                             # one allocation, two types
+        codes, scales = rows.codes.clone(), rows.scales.clone()
+        for how, other in copies(rows):
+            assert type(other) is Int8Rows and (other.shape, other.dtype, other.index, other.rows, other.width, other.pitch) == (
+                rows.shape, rows.dtype, rows.index, rows.rows, rows.width, rows.pitch), how
+            assert torch.equal(other.codes, codes) and torch.equal(other.scales, scales), how
+            assert other.codes_ptr == other.codes.data_ptr() and other.scales_ptr == other.scales.data_ptr(), how
+            assert how == "copy" or not rows.rows or other.codes_ptr != rows.codes_ptr, how
+    import copy
+    other = copy.deepcopy(made)
+    made._buffer.fill_(9)
+    assert not torch.equal(other.codes, made.codes)
+
+
+def test_copies_of_the_executor(lib):
+    """It holds the loaded library and no data: copies of a model share it, and saving it is refused in words."""
+    import copy
+    import pickle
+    ops = Int8Ops(Module(lib))
+    assert copy.deepcopy(ops) is ops and copy.deepcopy([ops])[0] is ops
+    with pytest.raises(RuntimeError, match="Int8Rows"):
+        pickle.dumps(ops)

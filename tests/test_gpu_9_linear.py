@@ -706,3 +706,33 @@ def test_norm_codes_next_to_ties(ops, rows, width, dtype, residual):
         z = (x.float() * weight.float()).double()
         q = z * 127 / z.abs().amax(1, keepdim=True)
         assert float(((got.codes.double() - q).abs() - q.abs() * 5 * U).max()) <= 0.5
+
+
+# ---- copies --------------------------------------------------------------------------------------------------------------
+
+def test_products_of_copied_and_saved_rows(ops):
+    """A copy is read where it lies: what becomes of the original's memory does not show."""
+    import copy
+    import io
+    w, x = ops.quantize_rows(randn(300, 1000, seed=120)), ops.quantize_rows(randn(5, 1000, seed=121))
+    want = ops.linear(x, w)
+    saved = io.BytesIO()
+    torch.save(w, saved)
+    saved.seek(0)
+    others = [copy.deepcopy(w), torch.load(saved, weights_only=False)]
+    w.codes.zero_(), w.scales.fill_(float("nan"))
+    for other in others:
+        assert torch.equal(ops.linear(x, other), want)
+
+
+@torch.inference_mode()
+def test_a_copied_model_runs_on_its_own_weights(ops):
+    import copy
+    from triattention_b200.models import int8_projections
+    ids = torch.arange(40).cuda()[None]
+    model = int8_projections(toy_llama(), ops)
+    want = model(input_ids=ids, use_cache=False).logits
+    other = copy.deepcopy(model)
+    for layer in model.model.layers:
+        layer.down.rows.codes.zero_()
+    assert torch.equal(other(input_ids=ids, use_cache=False).logits, want)

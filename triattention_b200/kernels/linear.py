@@ -71,6 +71,22 @@ class Int8Rows:
         self._codes = None
         return self
 
+    @classmethod
+    def _of_buffer(cls, buffer, shape, dtype):
+        """Rows as a call makes them, in memory that holds them already."""
+        self = cls.__new__(cls)
+        self.shape, self.dtype, self.device, self.index = shape, dtype, buffer.device, buffer.get_device()
+        self.rows, self.width, self.pitch = shape[:-1].numel(), shape[-1], code_pitch(shape[-1])
+        self.codes_ptr, self._buffer, self._codes = buffer.data_ptr(), buffer, None
+        self.scales_ptr = self.codes_ptr + self.rows * self.pitch
+        return self
+
+    def __reduce__(self):               # copies and saved rows are made anew from their tensors: addresses do not travel
+        if self._buffer is not None:    # (one tensor: torch.save takes no two types of one allocation)
+            return self._of_buffer, (self._buffer, self.shape, self.dtype)
+        shared = self._codes.untyped_storage().data_ptr() == self._scales.untyped_storage().data_ptr()
+        return type(self), (self.codes, self.scales.clone() if shared else self.scales, self.dtype)
+
     def _refuse(self, name):
         raise RuntimeError(f"{name}: rows of 1..{MAX_WIDTH} codes that start on 16-byte boundaries, with contiguous features and "
                            "scales, on a GPU")
@@ -105,6 +121,12 @@ class Int8Ops:
         self.module, lib = module, module.lib
         self._launch, self._calls = module._launch, (lib.tri_quantize_rows, lib.tri_silu_mul_rows, lib.tri_rms_norm_rows,
                                                      lib.tri_dequantize_rows, lib.tri_int8_linear)
+
+    def __deepcopy__(self, memo):       # (the loaded library, and no data)
+        return self
+
+    def __reduce__(self):
+        raise RuntimeError("Int8Ops holds the loaded library and cannot be saved, nor can layers that hold it: save their Int8Rows")
 
     @staticmethod
     def _inference(*tensors):
