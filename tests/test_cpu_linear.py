@@ -346,3 +346,32 @@ def test_copies_of_the_executor(lib):
     assert copy.deepcopy(ops) is ops and copy.deepcopy([ops])[0] is ops
     with pytest.raises(RuntimeError, match="Int8Rows"):
         pickle.dumps(ops)
+
+
+def test_rows_shown_to_two_threads_at_once():
+    """The tensors of rows that a call made are made when first asked for: a second thread that asks meanwhile gets them too."""
+    import threading
+    rows = Int8Rows._empty(torch.zeros(3, 40), 3, 40, -1)
+    inside, go_on = threading.Event(), threading.Event()
+
+    class Slow:             # the first thread that comes to the scales stops there
+        def __init__(self, buffer):
+            self.buffer = buffer
+
+        def __getitem__(self, part):
+            if part.start is not None and not inside.is_set():
+                inside.set()
+                go_on.wait(20)
+            return self.buffer[part]
+
+    rows._buffer = Slow(rows._buffer)
+    first = []
+    thread = threading.Thread(target=lambda: first.append(rows.scales))
+    thread.start()
+    try:
+        assert inside.wait(20)
+        assert rows.scales.shape == (3,) and rows.codes.shape == (3, 40)
+    finally:
+        go_on.set()
+        thread.join()
+    assert first[0].data_ptr() == rows.scales.data_ptr() == rows.scales_ptr

@@ -94,8 +94,8 @@ class Int8Rows:
     def _views(self):
         if self._codes is None:
             end = self.rows * self.pitch
+            self._scales = self._buffer[end:].view(torch.float32)      # (first: who finds codes takes the scales for made)
             self._codes = self._buffer[:end].view(self.rows, self.pitch)[:, :self.width]
-            self._scales = self._buffer[end:].view(torch.float32)
         return self._codes, self._scales
 
     @property
