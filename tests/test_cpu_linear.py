@@ -375,3 +375,130 @@ def test_rows_shown_to_two_threads_at_once():
         go_on.set()
         thread.join()
     assert first[0].data_ptr() == rows.scales.data_ptr() == rows.scales_ptr
+
+
+# ---- which layers are taken: by what they compute ----------------------------------------------------------------------------
+
+def behaving(kind):
+    """A toy model whose layers have the names, modules and settings of the Llama kind, and one thing that they compute otherwise."""
+    from transformers.models.llama.modeling_llama import LlamaAttention, LlamaDecoderLayer, LlamaMLP, LlamaRMSNorm
+    model = toy("Llama")
+
+    class Scaled(LlamaDecoderLayer):            # an integer factor: no float among the settings
+        def forward(self, hidden_states, **kwargs):
+            hidden_states = hidden_states + self.times * self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
+            return hidden_states + self.mlp(self.post_attention_layernorm(hidden_states))
+
+    class Behind(LlamaDecoderLayer):            # norms behind the blocks
+        def forward(self, hidden_states, **kwargs):
+            hidden_states = hidden_states + self.input_layernorm(self.self_attn(hidden_states=hidden_states, **kwargs)[0])
+            return hidden_states + self.post_attention_layernorm(self.mlp(hidden_states))
+
+    class Beside(LlamaDecoderLayer):            # both blocks on the layer's input
+        def forward(self, hidden_states, **kwargs):
+            attended = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
+            return hidden_states + attended + self.mlp(self.post_attention_layernorm(hidden_states))
+
+    class Tuple(LlamaDecoderLayer):
+        def forward(self, hidden_states, **kwargs):
+            return (super().forward(hidden_states, **kwargs),)
+
+    class Clamped(LlamaMLP):
+        def forward(self, x):
+            return self.down_proj(self.act_fn(self.gate_proj(x).clamp(max=7)) * self.up_proj(x))
+
+    class Swapped(LlamaMLP):
+        def forward(self, x):
+            return self.down_proj(self.gate_proj(x) * self.act_fn(self.up_proj(x)))
+
+    class OneMoreRMSNorm(LlamaRMSNorm):         # weights around zero
+        def forward(self, x):
+            return x * (x.square().mean(-1, keepdim=True) + self.variance_epsilon).rsqrt() * (1 + self.weight)
+
+    class Gate(LlamaAttention):                 # values of its own made of what it is given
+        def forward(self, hidden_states, **kwargs):
+            out, weights = super().forward(hidden_states, **kwargs)
+            return out * hidden_states.mean(-1, keepdim=True), weights
+
+    for layer in model.model.layers:
+        layer.times = 2
+        if kind in ("Scaled", "Behind", "Beside", "Tuple"):
+            layer.__class__ = locals()[kind]
+        elif kind in ("Clamped", "Swapped"):
+            layer.mlp.__class__ = locals()[kind]
+        elif kind == "OneMore":
+            layer.post_attention_layernorm.__class__ = OneMoreRMSNorm
+        elif kind == "Gate":
+            layer.self_attn.__class__ = Gate
+        elif kind == "hook":
+            layer.self_attn.register_forward_hook(lambda *a: None)
+        elif kind == "pre-hook":
+            layer.self_attn.register_forward_pre_hook(lambda *a: None)
+        elif kind == "own forward":
+            layer.self_attn.forward = layer.self_attn.forward
+    return model
+
+
+@pytest.mark.parametrize("kind", ["Scaled", "Behind", "Beside", "Tuple", "Clamped", "Swapped", "OneMore", "Gate", "hook", "pre-hook", "own forward"])
+def test_layers_that_compute_something_else_are_refused(kind):
+    from triattention_b200.models import int8_projections
+    model = behaving(kind)
+    before = [(n, type(m)) for n, m in model.named_modules()]
+    with pytest.raises(RuntimeError, match="no decoder layer"):
+        int8_projections(model, ExactOps())
+    assert [(n, type(m)) for n, m in model.named_modules()] == before
+    assert all("forward" not in vars(m) for m in model.modules()) or kind == "own forward"
+
+
+def test_models_whose_attention_wants_values_are_refused_whole():
+    """DiffLlama, the text model of Qwen2.5-VL, Mllama's and Chameleon's layers ask the hidden states for their size (and Chameleon's norms
+    stand behind, its results are tuples): refused before anything is replaced, and they run as before."""
+    import transformers
+    from transformers.models.chameleon import modeling_chameleon as chameleon
+    from transformers.models.mllama import modeling_mllama as mllama
+    from triattention_b200.kernels.linear import Int8DecoderLayer
+    from triattention_b200.models import int8_projections
+    small = dict(hidden_size=96, intermediate_size=160, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, vocab_size=200)
+    ids = torch.arange(7)[None]
+    for model in (toy("DiffLlama"), transformers.Qwen2_5_VLTextModel(transformers.Qwen2_5_VLTextModel.config_class(
+            **small, rope_parameters=dict(rope_type="default", rope_theta=1e4, mrope_section=[2, 4, 6]))).eval()):
+        with torch.no_grad():
+            want = model(input_ids=ids, use_cache=False)[0]
+            with pytest.raises(RuntimeError, match="no decoder layer"):
+                int8_projections(model, ExactOps())
+            assert torch.equal(model(input_ids=ids, use_cache=False)[0], want)
+    config = transformers.ChameleonConfig(**small)
+    for layer in (chameleon.ChameleonDecoderLayer(config, 0), chameleon.ChameleonSwinDecoderLayer(config, 0)):
+        assert not Int8DecoderLayer.fits(layer)
+    config = mllama.MllamaTextConfig(**small)
+    config._attn_implementation = "eager"
+    assert not Int8DecoderLayer.fits(mllama.MllamaSelfAttentionDecoderLayer(config, 0))
+
+
+@pytest.mark.parametrize("kind", ["Ministral", "SmolLM3", "Cwm", "Ernie4_5"])
+def test_other_models_of_the_kind_are_taken(kind):
+    from triattention_b200.models import int8_projections
+    model, ids = toy(kind, pad_token_id=0, bos_token_id=1, eos_token_id=2), torch.arange(3, 15)[None]
+    with torch.no_grad():
+        want = model(input_ids=ids, use_cache=False).logits
+        got = int8_projections(model, ExactOps())(input_ids=ids, use_cache=False).logits
+    torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-4 * float(want.abs().max()))
+
+
+def test_trying_a_layer_leaves_the_model_alone():
+    """Whatever attention the model is set to is not called, and no setting of the model changes."""
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+    from triattention_b200.models import int8_projections
+    calls = []
+    ALL_ATTENTION_FUNCTIONS["counted"] = lambda module, query, *a, **k: (calls.append(1), (query.transpose(1, 2).contiguous(), None))[1]
+    model = toy("Llama").train()
+    model.set_attn_implementation("counted")
+    settings, weights = repr(model.config), [(n, p.data_ptr()) for n, p in model.named_parameters()]
+    from triattention_b200.kernels.linear import Int8DecoderLayer
+    assert all(Int8DecoderLayer.fits(layer) for layer in model.model.layers)
+    assert not calls and repr(model.config) == settings and [(n, p.data_ptr()) for n, p in model.named_parameters()] == weights
+    assert model.config._attn_implementation == "counted" and all(m.training for m in model.modules())
+    int8_projections(model, ExactOps())
+    assert not calls
+    model(input_ids=torch.arange(4)[None], use_cache=False)
+    assert len(calls) == 3

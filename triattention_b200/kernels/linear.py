@@ -11,6 +11,9 @@ activation, or plain rows.
 """
 from __future__ import annotations
 
+import copy
+import inspect
+
 import torch
 
 from triattention_b200.kernels.extension import MAX_OUTPUTS, MAX_WIDTH, ROW_TYPES
@@ -247,6 +250,88 @@ class Int8Linear(torch.nn.Module):
         return self.ops.linear(rows, self.rows, bias=self.bias_row, residual=residual)
 
 
+def _stand_in(module, **children):
+    """An object of the module's class with its settings, but other children: its forward can be run without touching the model."""
+    made = type(module).__new__(type(module))
+    made.__dict__.update(vars(module), training=False, _modules={**module._modules, **children})
+    return made
+
+
+def _run(module, values, **more):
+    """The class's forward on `values`, as a decoder layer's modules are called; arguments that it cannot do without are None."""
+    names = inspect.signature(type(module).forward).parameters.values()
+    given = [p.name for p in names if p.kind is p.POSITIONAL_OR_KEYWORD][2:]
+    anything = any(p.kind is p.VAR_KEYWORD for p in names)
+    missing = {p.name: None for p in list(names)[2:] if p.default is p.empty and p.kind in (p.POSITIONAL_OR_KEYWORD, p.KEYWORD_ONLY)}
+    return type(module).forward(module, values, **{**missing, **{n: v for n, v in more.items() if anything or n in given or n in missing}})
+
+
+def _same(got, want):
+    return type(got) is torch.Tensor and got.shape == want.shape and torch.allclose(got, want, rtol=1e-9, atol=1e-9)
+
+
+def _trial():
+    """What forwards are tried on: small and large numbers of both signs (a clamp or a factor shows), in float64."""
+    even = dict(dtype=torch.float64, device="cpu")
+    return (torch.linspace(-1, 1, 24, **even) * 10.0 ** torch.arange(-3, 5, **even).repeat(3)).reshape(2, 3, 4)
+
+
+def _layer_adds_up(layer):
+    """x + attention(norm(x)), and the feed-forward block of its norm added to that; a tensor, not a tuple."""
+    def attention(hidden_states, *args, **kwargs):
+        return torch.sin(hidden_states), None
+    norm, other, block = lambda x: 2 * x + 1, lambda x: x / 3 - 2, lambda x: 5 * torch.cos(x)
+    x = _trial()
+    h = x + torch.sin(norm(x))
+    got = _run(_stand_in(layer, self_attn=attention, input_layernorm=norm, post_attention_layernorm=other, mlp=block), x)
+    return _same(got, h + block(other(h)))
+
+
+def _block_is_gated(mlp):
+    """down(act(gate(x)) * up(x))."""
+    x, gate, up, down, act = _trial(), lambda x: 2 * x + 1, lambda x: x / 3 - 2, lambda x: 5 * x - 7, torch.atan
+    return _same(_run(_stand_in(mlp, gate_proj=gate, up_proj=up, down_proj=down, act_fn=act), x), down(act(gate(x)) * up(x)))
+
+
+def _norm_is_rms(norm):
+    """weight * x / sqrt(mean x^2 + eps), on the norm's own width in fp32."""
+    width, at = norm.weight.shape[0], dict(dtype=torch.float32, device="cpu")
+    x, weight = torch.cos(torch.arange(2 * width, **at)).reshape(2, width) * 0.01, torch.sin(torch.arange(width, **at))
+    made = _stand_in(norm)
+    made.__dict__["_parameters"] = {**norm._parameters, "weight": weight}
+    want = x / (x.square().mean(1, keepdim=True) + norm.variance_epsilon).sqrt() * weight
+    got = _run(made, x)
+    return type(got) is torch.Tensor and torch.allclose(got, want, rtol=1e-4, atol=1e-6)
+
+
+def _attention_takes_rows(attention):
+    """Whether its forward gets by on rows of codes, which have a shape, a type and a device and are otherwise there for the three
+    projections.  Run on two tokens with the model's plain attention (whichever is set keeps what it holds)."""
+    like, width = attention.o_proj.weight, attention.q_proj.in_features
+    rows = Int8Rows(torch.zeros(1, 2, width, dtype=torch.int8, device="cpu"), torch.zeros(1, 2, dtype=torch.float32, device="cpu"), like.dtype)
+    rows.device = like.device
+
+    def projection(linear):
+        def project(x):
+            if x is not rows:
+                raise TypeError("not the rows")
+            return like.new_zeros(1, 2, linear.out_features)
+        return project
+
+    def output(x):
+        if type(x) is not torch.Tensor or x.shape != (1, 2, attention.o_proj.in_features):
+            raise TypeError("not the heads' outputs")
+        return x.new_zeros(1, 2, attention.o_proj.out_features)
+
+    made = _stand_in(attention, o_proj=output, **{n: projection(getattr(attention, n)) for n in ("q_proj", "k_proj", "v_proj")})
+    if hasattr(attention, "config"):
+        made.config = copy.deepcopy(attention.config)
+        made.config._attn_implementation = "eager"
+    turn, places = like.new_zeros(1, 2, attention.head_dim), torch.arange(2, device=like.device)
+    out = _run(made, rows, position_embeddings=(turn, turn), attention_mask=None, position_ids=places[None], cache_position=places)
+    return isinstance(out, tuple) and type(out[0]) is torch.Tensor and out[0].shape == (1, 2, attention.o_proj.out_features)
+
+
 class Int8DecoderLayer(torch.nn.Module):
     """A decoder layer of the Llama kind (two RMS norms, q / k / v / o projections, a gated SiLU feed-forward block) whose
     projections run on INT8 codes.  Both norms, the addition of the attention's output to the residual stream and the gated
@@ -271,19 +356,29 @@ class Int8DecoderLayer(torch.nn.Module):
     @staticmethod
     def fits(layer):
         """Whether `layer` is built like that, with nothing in it that would be lost: no module or factor more (scaled residuals,
-        norms inside the block), no hooks and no forward of an object's own on what is replaced."""
+        norms inside the block), no hooks and no forward of an object's own on what is replaced or is handed rows of codes in place
+        of values; and whether it computes that, which its forwards show by what they make of stand-ins for the modules (names
+        alone say little: norms behind the blocks, factors, clamped activations and tuples as results go by the same ones)."""
         bare = lambda m: not ("forward" in vars(m) or m._forward_hooks or m._forward_pre_hooks)
         plain = lambda m: bare(m) and not any(isinstance(v, (float, torch.Tensor)) for v in vars(m).values()) and not m._parameters and not m._buffers
         linear = lambda m: type(m) is torch.nn.Linear and bare(m)
         norm = lambda m: ("RMSNorm" in type(m).__name__ and hasattr(m, "variance_epsilon") and bare(m) and
                           [n for n, w in m.named_parameters() if w is not None] == ["weight"])
         attention, mlp = getattr(layer, "self_attn", None), getattr(layer, "mlp", None)
-        return (isinstance(attention, torch.nn.Module) and isinstance(mlp, torch.nn.Module) and
+        if not (isinstance(attention, torch.nn.Module) and isinstance(mlp, torch.nn.Module) and bare(attention) and
                 all(linear(getattr(attention, n, None)) for n in ("q_proj", "k_proj", "v_proj", "o_proj")) and
                 all(linear(getattr(mlp, n, None)) for n in ("gate_proj", "up_proj", "down_proj")) and
                 type(getattr(mlp, "act_fn", None)).__name__ in ("SiLU", "SiLUActivation") and
                 all(norm(getattr(layer, n, None)) for n in ("input_layernorm", "post_attention_layernorm")) and
-                plain(layer) and plain(mlp) and len(layer._modules) == 4 and len(mlp._modules) == 4)
+                plain(layer) and plain(mlp) and len(layer._modules) == 4 and len(mlp._modules) == 4):
+            return False
+        try:
+            return (_layer_adds_up(layer) and _block_is_gated(mlp) and _attention_takes_rows(attention) and
+                    all(_norm_is_rms(n) for n in (layer.input_layernorm, layer.post_attention_layernorm)))
+        except torch.OutOfMemoryError:
+            raise
+        except Exception:       # a forward that wants something else
+            return False
 
     def forward(self, hidden_states, **kwargs):
         ops = self.ops
