@@ -502,3 +502,44 @@ def test_trying_a_layer_leaves_the_model_alone():
     assert not calls
     model(input_ids=torch.arange(4)[None], use_cache=False)
     assert len(calls) == 3
+
+
+# ---- all of the model or nothing of it ---------------------------------------------------------------------------------------
+
+def unchanged_by(model, ops, match):
+    """int8_projections(model, ops) fails, and the model is what it was."""
+    from triattention_b200.models import int8_projections
+    before, ids = [(n, id(m)) for n, m in model.named_modules()], torch.arange(9)[None]
+    with torch.no_grad():
+        want = model(input_ids=ids, use_cache=False).logits
+        with pytest.raises(RuntimeError, match=match):
+            int8_projections(model, ops)
+        assert [(n, id(m)) for n, m in model.named_modules()] == before
+        assert torch.equal(model(input_ids=ids, use_cache=False).logits, want)
+
+
+@pytest.mark.parametrize("at", [0, 1, 4, 5, 6, 11, 17])
+def test_a_conversion_that_fails_leaves_the_model_whole(at):
+    class Failing(ExactOps):
+        calls = 0
+
+        def quantize_rows(self, x):
+            if self.calls == at:
+                raise RuntimeError("no memory")
+            self.calls += 1
+            return super().quantize_rows(x)
+
+    unchanged_by(toy("Llama", attention_bias=True), Failing(), "no memory")
+
+
+def test_weights_of_several_types_are_refused():
+    """Calls want the norm's weight and a bias in the type of the rows: said before anything is replaced, not by the first forward."""
+    model = toy("Llama")
+    model.model.layers[2].post_attention_layernorm.bfloat16()
+    unchanged_by(model, ExactOps(), "one type")
+
+
+def test_layers_that_share_an_attention_are_refused():
+    model = toy("Llama")
+    model.model.layers[1].self_attn = model.model.layers[0].self_attn
+    unchanged_by(model, ExactOps(), "torch.nn.Linear")

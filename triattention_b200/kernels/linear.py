@@ -18,6 +18,7 @@ import torch
 
 from triattention_b200.kernels.extension import MAX_OUTPUTS, MAX_WIDTH, ROW_TYPES
 
+ATTENTION_PROJECTIONS = ("q_proj", "k_proj", "v_proj", "o_proj")
 CODE_ALIGN = 16     # code rows start on 16-byte boundaries
 # Rows that the calls make start on 128-byte boundaries, one cache line, where that is little memory: products read codes 128 bytes
 # a row at a time, and rows that straddle lines cost up to a third (16384 x 4099 -> 4096: 262 us 16 bytes apart, 188 with 64, 179
@@ -238,6 +239,8 @@ class Int8Linear(torch.nn.Module):
     @classmethod
     def of(cls, ops, *linears):
         """One projection of torch.nn.Linear layers that read the same rows; their outputs come side by side."""
+        if any(type(l) is not torch.nn.Linear for l in linears):
+            raise RuntimeError("Int8Linear: torch.nn.Linear layers (one of these is something else, or shared and replaced already)")
         biases = [l.bias for l in linears]
         if any(b is None for b in biases) and any(b is not None for b in biases):
             biases = [torch.zeros_like(l.weight[:, 0]) if b is None else b for l, b in zip(linears, biases)]
@@ -341,13 +344,16 @@ class Int8DecoderLayer(torch.nn.Module):
 
     def __init__(self, ops, layer):
         super().__init__()
-        attention, mlp = layer.self_attn, layer.mlp
-        self.ops, self.self_attn = ops, attention
-        for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
-            setattr(attention, name, Int8Linear.of(ops, getattr(attention, name)))
+        attention, mlp, norms = layer.self_attn, layer.mlp, (layer.input_layernorm, layer.post_attention_layernorm)
+        projections = [getattr(attention, n) for n in ATTENTION_PROJECTIONS]
+        if len({(w.dtype, w.device) for m in (*projections, *norms, mlp.gate_proj, mlp.up_proj, mlp.down_proj) for w in m.parameters()}) > 1:
+            raise RuntimeError("Int8DecoderLayer: the projections' and norms' weights and biases have one type and lie on one device")
+        made = [Int8Linear.of(ops, p) for p in projections]
         self.gate_up, self.down = Int8Linear.of(ops, mlp.gate_proj, mlp.up_proj), Int8Linear.of(ops, mlp.down_proj)
-        norms = layer.input_layernorm, layer.post_attention_layernorm
         self.norm_weights, self.eps = [n.weight.detach() for n in norms], [n.variance_epsilon for n in norms]
+        for name, projection in zip(ATTENTION_PROJECTIONS, made):       # (nothing is replaced before all is made)
+            setattr(attention, name, projection)
+        self.ops, self.self_attn = ops, attention
         for name, value in vars(layer).items():         # what the model looks up on its layers (attention_type and the like)
             if not name.startswith("_") and name not in self.__dict__:
                 setattr(self, name, value)
@@ -366,7 +372,7 @@ class Int8DecoderLayer(torch.nn.Module):
                           [n for n, w in m.named_parameters() if w is not None] == ["weight"])
         attention, mlp = getattr(layer, "self_attn", None), getattr(layer, "mlp", None)
         if not (isinstance(attention, torch.nn.Module) and isinstance(mlp, torch.nn.Module) and bare(attention) and
-                all(linear(getattr(attention, n, None)) for n in ("q_proj", "k_proj", "v_proj", "o_proj")) and
+                all(linear(getattr(attention, n, None)) for n in ATTENTION_PROJECTIONS) and
                 all(linear(getattr(mlp, n, None)) for n in ("gate_proj", "up_proj", "down_proj")) and
                 type(getattr(mlp, "act_fn", None)).__name__ in ("SiLU", "SiLUActivation") and
                 all(norm(getattr(layer, n, None)) for n in ("input_layernorm", "post_attention_layernorm")) and

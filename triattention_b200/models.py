@@ -15,7 +15,7 @@ from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
 from triattention_b200.kernels.decode import DecodeCache
 from triattention_b200.kernels.extension import LONG_TAIL_ROWS, load_extension
-from triattention_b200.kernels.linear import Int8DecoderLayer, Int8Ops
+from triattention_b200.kernels.linear import ATTENTION_PROJECTIONS, Int8DecoderLayer, Int8Ops
 from triattention_b200.kernels.prefill import Prefill
 from triattention_b200.maps import load_map, preset
 
@@ -65,17 +65,26 @@ def int8_projections(model, ops=None):
     """Run the projections of every decoder layer on INT8 codes (kernels/linear.py): weights quantised in place, one scale per
     output channel; activations per token.  Changes numerics, so it is off unless asked for; independent of the attention
     implementation, before or after ``TriAttention(model, ...)``.  Embeddings, the final norm and the vocabulary projection stay
-    as they are, and so does what a model records of its own layer classes (output_hidden_states finds none).  Returns the
-    model; a model without a layer of the Llama kind (RMS norms, q / k / v / o, gated SiLU) is refused."""
+    as they are, and so do layers of another kind and what a model records of its own layer classes (output_hidden_states finds none).
+    Returns the model; a model without a layer of the Llama kind (RMS norms, q / k / v / o, gated SiLU) is refused, and one whose
+    conversion fails (types, memory: the codes are made beside the weights) stays as it was."""
     ops = Int8Ops(load_extension()) if ops is None else ops
     found = [(parent, name, child) for parent in model.modules() for name, child in parent._modules.items()
              if child is not None and Int8DecoderLayer.fits(child)]
     if not found:
         raise RuntimeError("int8_projections: no decoder layer with RMS norms, q / k / v / o projections and a gated SiLU block")
-    made = {}       # a layer that the model uses in several places stays one layer
+    made, kept = {}, []       # a layer that the model uses in several places stays one layer
+    try:
+        for _, _, child in found:
+            if id(child) not in made:
+                kept.append((child.self_attn, {n: getattr(child.self_attn, n) for n in ATTENTION_PROJECTIONS}))
+                made[id(child)] = Int8DecoderLayer(ops, child)
+    except BaseException:
+        for attention, projections in reversed(kept):
+            for name, projection in projections.items():
+                setattr(attention, name, projection)
+        raise
     for parent, name, child in found:
-        if id(child) not in made:
-            made[id(child)] = Int8DecoderLayer(ops, child)
         parent._modules[name] = made[id(child)]
     return model
 
