@@ -543,3 +543,26 @@ def test_layers_that_share_an_attention_are_refused():
     model = toy("Llama")
     model.model.layers[1].self_attn = model.model.layers[0].self_attn
     unchanged_by(model, ExactOps(), "torch.nn.Linear")
+
+
+def test_two_threads_get_one_error_word(lib, monkeypatch):
+    """A word that nothing holds any more would be written to by kernels under way, and read by nobody."""
+    import threading
+    module, both, zeros = Module(lib), threading.Barrier(2, timeout=5), torch.zeros
+    module._errors = {}
+
+    def slow(*args, device=None, **kwargs):
+        try:
+            both.wait()
+        except threading.BrokenBarrierError:        # (one thread alone)
+            pass
+        return zeros(*args, **kwargs)
+
+    monkeypatch.setattr(extension.torch, "zeros", slow)
+    words = []
+    threads = [threading.Thread(target=lambda: words.append(module.error_word("cuda:0"))) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert words[0] is words[1] is module.error_word(torch.device("cuda", 0))

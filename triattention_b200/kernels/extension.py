@@ -110,9 +110,10 @@ class Module:
     def error_word(self, device):
         """The int32 word on `device` that kernels with bounded waits write their error code to (one per GPU)."""
         key = self._device_index(device)
-        if key not in self._errors:
-            self._errors[key] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
-        return self._errors[key]
+        word = self._errors.get(key)
+        if word is None:        # (setdefault: two threads that come here at once both get the word that is kept)
+            word = self._errors.setdefault(key, torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key)))
+        return word
 
     def check_device_error(self, device=None):
         """Synchronise and raise if a kernel reported an error (a bounded wait that ran out, a bad table entry).
@@ -564,9 +565,12 @@ class Module:
         return out
 
     def _error_pointer(self, index):
-        if index not in self._errors and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the first call on a GPU belongs outside of a stream capture (it allocates the error word)")
-        return self.error_word(index).data_ptr() if index not in self._errors else self._errors[index].data_ptr()
+        word = self._errors.get(index)
+        if word is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first call on a GPU belongs outside of a stream capture (it allocates the error word)")
+            word = self.error_word(index)
+        return word.data_ptr()
 
     # -- parity helpers --------------------------------------------------------------------------
     def qk_accumulators(self, requests, q8, q4x, k8, k4x, batch, heads_q, heads_kv, tokens):
