@@ -566,3 +566,13 @@ def test_two_threads_get_one_error_word(lib, monkeypatch):
     for t in threads:
         t.join()
     assert words[0] is words[1] is module.error_word(torch.device("cuda", 0))
+
+
+def test_error_words_are_the_process_s(lib, monkeypatch):
+    """The projections of a model and the engine around it each loaded the library for themselves: what one's kernels report, the
+    other's check (generate's, or any) must see."""
+    one, other = Module(lib), Module(lib)
+    monkeypatch.setitem(one._errors, 5, torch.tensor([1], dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="device error 1 on cuda:5"):
+        other.check_device_error()
+    other.check_device_error()                  # reported once

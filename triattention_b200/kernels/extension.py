@@ -88,12 +88,15 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+ERROR_WORDS = {}        # of each GPU that this process has launched on, whichever Module did
+
+
 class Module:
     """The five reference method names (batched), plus the cache-store and parity helpers."""
 
     def __init__(self, lib):
         self.lib = lib
-        self._errors = {}
+        self._errors = ERROR_WORDS
 
     # -- plumbing ------------------------------------------------------------------------------
     def _check(self, status):

@@ -119,7 +119,11 @@ def _flat(x):
 class Int8Ops:
     """Calls that end in rows of codes, and the product that starts from them.  Every call allocates its results and runs on the
     current stream of the inputs' device; nothing synchronises with the host.  Inference only: codes carry no gradient, and
-    inputs that ask for one are refused while gradients are being recorded."""
+    inputs that ask for one are refused while gradients are being recorded.
+
+    A product whose bounded waits ran out (a GPU that others hold up for seconds) returns all the same, with void results, and says so
+    in the GPU's error word: call ``ops.module.check_device_error()``, which synchronises and raises, before results are relied
+    on.  ``TriAttention.generate`` does."""
 
     def __init__(self, module):
         self.module, lib = module, module.lib

@@ -67,7 +67,8 @@ def int8_projections(model, ops=None):
     implementation, before or after ``TriAttention(model, ...)``.  Embeddings, the final norm and the vocabulary projection stay
     as they are, and so do layers of another kind and what a model records of its own layer classes (output_hidden_states finds none).
     Returns the model; a model without a layer of the Llama kind (RMS norms, q / k / v / o, gated SiLU) is refused, and one whose
-    conversion fails (types, memory: the codes are made beside the weights) stays as it was."""
+    conversion fails (types, memory: the codes are made beside the weights) stays as it was.  ``TriAttention.generate`` checks the
+    GPU's error word; where the model runs otherwise, ``load_extension().check_device_error()`` belongs behind its passes."""
     ops = Int8Ops(load_extension()) if ops is None else ops
     found = [(parent, name, child) for parent in model.modules() for name, child in parent._modules.items()
              if child is not None and Int8DecoderLayer.fits(child)]
