@@ -576,3 +576,12 @@ def test_error_words_are_the_process_s(lib, monkeypatch):
     with pytest.raises(RuntimeError, match="device error 1 on cuda:5"):
         other.check_device_error()
     other.check_device_error()                  # reported once
+
+
+def test_an_error_word_made_in_inference_mode_is_reported_outside(lib):
+    module = Module(lib)
+    with torch.inference_mode():
+        module._errors = {5: torch.tensor([1], dtype=torch.int32), 6: torch.zeros(1, dtype=torch.int32)}
+    with pytest.raises(RuntimeError, match="device error 1 on cuda:5"):
+        module.check_device_error()
+    module.check_device_error()

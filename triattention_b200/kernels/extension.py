@@ -127,7 +127,8 @@ class Module:
                 continue
             word = int(self._errors[key].item())
             if word:
-                self._errors[key].zero_()
+                with torch.inference_mode():        # (whichever mode the word was made in)
+                    self._errors[key].zero_()
                 where = f", wait site {(word >> 8) & 0xff} at step {word >> 16} of the prefill kernel" if word >> 8 else ""
                 raise RuntimeError(f"TriAttention kernel reported device error {word & 0xff} on cuda:{key}{where} (1 = "
                                    "barrier wait ran out, 3 = tile number outside the prompt in a task table, 4 = partial "
