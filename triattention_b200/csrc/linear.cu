@@ -107,7 +107,8 @@ __device__ __forceinline__ void lin_prefetch_box(const CUtensorMap* map, int col
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(column), "r"(row) : "memory");
 }
 
-// The forms for a pair of CTAs.  Barrier addresses with the peer bit cleared name the even CTA's barrier at the same place.
+// The forms for a pair of CTAs.  In a shared::cluster address of a pair bit 24 tells the two CTAs apart: barrier addresses with it
+// cleared name the even CTA's barrier at the same place.
 constexpr uint32_t PairEven = 0xfeffffffu;
 __device__ __forceinline__ void pair_alloc(uint32_t* slot, uint32_t columns) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns) : "memory");
@@ -148,12 +149,12 @@ __device__ __forceinline__ void lin_origin(const LinearArgs& p, int tile, int ch
 
 // C neighbouring channels of one token as one access.
 template <typename T, int C> struct LinVector {
-  T v[C];
+  alignas(C * sizeof(T)) T v[C];
 };
 // The same as it is read ahead: 32-bit words, taken apart only where they are used.  (With elements of 16 bits the compiler takes
 // them apart right behind the load, which waits for it: 16384 x 4096 outputs of width 128 with a residual took 120 us, now 74; of width 4096 210 and 190.)
 template <typename T, int C> struct LinWords {
-  uint32_t w[(C * sizeof(T) + 3) / 4];
+  alignas(C * sizeof(T) < 4 ? 4 : C * sizeof(T)) uint32_t w[(C * sizeof(T) + 3) / 4];
   __device__ __forceinline__ void load(const T* from) {
     constexpr int B = C * sizeof(T);
     if constexpr (B == 16) *reinterpret_cast<uint4*>(w) = __ldcs(reinterpret_cast<const uint4*>(from));
@@ -253,7 +254,7 @@ __device__ __forceinline__ void lin_epilogue_as(const LinearArgs& p, uint32_t co
       for (int i = 0; i < LinBlockTokens / C; ++i, to += out_step) {
         constexpr int Skip = C * LinPitch;
         const int pass = part / C + i;
-        float y[C];
+        alignas(16) float y[C];
         if constexpr (C >= 4) {
 #pragma unroll
           for (int k = 0; k < C; k += 4) *reinterpret_cast<float4*>(y + k) = *reinterpret_cast<const float4*>(from + i * Skip + k);
