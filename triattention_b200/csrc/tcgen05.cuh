@@ -4,6 +4,7 @@
 #pragma once
 #include "common.cuh"
 #include <cuda.h>
+#include <atomic>
 
 namespace tri {
 
@@ -101,14 +102,18 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// (Atomic: host threads may make their first calls at once.  A failure is not kept.)
 inline EncodeTiled encode_fn() {
-  static EncodeTiled fn = nullptr;
+  static std::atomic<EncodeTiled> known{nullptr};
+  EncodeTiled fn = known.load(std::memory_order_relaxed);
   if (fn == nullptr) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
+        q == cudaDriverEntryPointSuccess) {
       fn = reinterpret_cast<EncodeTiled>(p);
+      known.store(fn, std::memory_order_relaxed);
+    }
   }
   return fn;
 }
