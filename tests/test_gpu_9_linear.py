@@ -736,3 +736,21 @@ def test_a_copied_model_runs_on_its_own_weights(ops):
     for layer in model.model.layers:
         layer.down.rows.codes.zero_()
     assert torch.equal(other(input_ids=ids, use_cache=False).logits, want)
+
+
+# ---- subnormal numbers -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,outputs,width", [(1, 200, 512), (2, 640, 4096), (40, 200, 512), (300, 640, 300), (5000, 4096, 256)])
+def test_linear_keeps_subnormal_numbers(ops, tokens, outputs, width, dtype):
+    """IEEE arithmetic down to the smallest numbers of each type: products of powers of two, residuals and biases come out as they are."""
+    least = torch.finfo(dtype).smallest_normal / 2 ** 4
+    x, w = codes_rows(tokens, width, 130), codes_rows(outputs, width, 131)
+    x.codes.zero_(), w.codes.fill_(1)
+    residual, bias = (randn(*shape, seed=s, dtype=FP32).mul(least).to(dtype) for shape, s in (((tokens, outputs), 132), ((outputs,), 133)))
+    assert bool(residual.any()) and float(residual.abs().max()) < torch.finfo(dtype).smallest_normal
+    assert torch.equal(ops.linear(x, w, residual=residual, dtype=dtype), residual)
+    assert torch.equal(ops.linear(x, w, bias=bias, dtype=dtype), bias.expand(tokens, outputs))
+    x.codes[:, 0] = 3
+    x.scales.fill_(2.0 ** -60), w.scales.fill_(least * 2.0 ** 60)        # (2^-60 each way: 3 * 2^60 * 2^-60 * least)
+    assert torch.equal(ops.linear(x, w, dtype=dtype), torch.full((tokens, outputs), 3 * least, dtype=FP32, device="cuda").to(dtype))

@@ -19,7 +19,9 @@ ROOT = Path(__file__).resolve().parent
 CSRC = ROOT / "csrc"
 LIBRARY = ROOT / "libtriattn_sm100a.so"
 SOURCES = ("abi.cu", "kv_write.cu", "decode.cu", "prefill.cu", "tasks.cu", "rows.cu", "linear.cu")
-IEEE = ("rows.cu",)     # compiled without --use_fast_math: their codes are those of IEEE fp32 arithmetic
+# Compiled without --use_fast_math: rows.cu's codes are those of IEEE fp32 arithmetic, linear.cu keeps subnormal numbers (it has no
+# division and no function that would be faster with it).
+IEEE = ("rows.cu", "linear.cu")
 FLAGS = ("-O3", "-std=c++17", "--use_fast_math", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
          "-Xcompiler", "-fPIC")
 

@@ -1,7 +1,8 @@
 // Product of INT8 code rows with one scale per token and one per channel:
 //   out[t][n] = round( (sum_k c[t][k] d[n][k]) * sd[n] * sc[t] + bias[n] + residual[t][n] )
 // The sum over k is an exact 32-bit integer: |c d| <= 128 * 128, so width <= 131071 cannot overflow, and its value does not
-// depend on the order of the additions (nor on how the width is split).  The rest is fp32, rounded once.
+// depend on the order of the additions (nor on how the width is split).  The rest is IEEE fp32 (subnormal numbers too: this file is
+// compiled without --use_fast_math), rounded once.
 //
 // tcgen05 kind::i8 with the WEIGHTS as the 128-row operand and the tokens as the N of the MMA: N goes from 16 to 256 in steps of
 // 16, so a decode step of two to 256 tokens is one tile of tokens that fits it, and the weights (what such a step is bound by)
