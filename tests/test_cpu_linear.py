@@ -585,3 +585,20 @@ def test_an_error_word_made_in_inference_mode_is_reported_outside(lib):
     with pytest.raises(RuntimeError, match="device error 1 on cuda:5"):
         module.check_device_error()
     module.check_device_error()
+
+
+def test_forward_mode_tangents_are_refused(lib):
+    """Codes carry no tangent either: it would be dropped without a word, under no_grad as well (which is about the other mode)."""
+    import torch.autograd.forward_ad as forward
+    ops, x = Int8Ops(Module(lib)), torch.zeros(4, 64)
+    weight, rows = torch.ones(64), Int8Rows(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4))
+    with forward.dual_level(), torch.no_grad():
+        dual = forward.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.quantize_rows(dual), lambda: ops.silu_mul(x, dual), lambda: ops.rms_norm(x, weight, 1e-6, residual=dual),
+                     lambda: ops.linear(rows, rows, residual=dual)):
+            with pytest.raises(RuntimeError, match="no forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="on a GPU"):     # (one without a tangent goes on to the next check)
+            ops.quantize_rows(x)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: ops.quantize_rows(x).scales, (x,), (torch.ones_like(x),))

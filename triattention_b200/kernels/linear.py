@@ -15,6 +15,7 @@ import copy
 import inspect
 
 import torch
+from torch.autograd import forward_ad
 
 from triattention_b200.kernels.extension import MAX_OUTPUTS, MAX_WIDTH, ROW_TYPES
 
@@ -119,7 +120,7 @@ def _flat(x):
 class Int8Ops:
     """Calls that end in rows of codes, and the product that starts from them.  Every call allocates its results and runs on the
     current stream of the inputs' device; nothing synchronises with the host.  Inference only: codes carry no gradient, and
-    inputs that ask for one are refused while gradients are being recorded.
+    inputs that ask for one are refused while gradients are being recorded, and inputs with a forward-mode tangent always.
 
     A product whose bounded waits ran out (a GPU that others hold up for seconds) returns all the same, with void results, and says so
     in the GPU's error word: call ``ops.module.check_device_error()``, which synchronises and raises, before results are relied
@@ -143,6 +144,10 @@ class Int8Ops:
                 if t is not None and t.requires_grad:
                     raise RuntimeError("the INT8 projections have no backward pass: call them under torch.no_grad() or "
                                        "inference_mode()")
+        if forward_ad._current_level >= 0:
+            for t in tensors:
+                if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                    raise RuntimeError("the INT8 projections have no forward-mode derivative")
 
     def quantize_rows(self, x):
         """x [..., H] (bf16, fp16 or fp32) -> Int8Rows."""
