@@ -218,7 +218,6 @@ __device__ __forceinline__ float2 gated_fast2(float2 g, float2 u) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
   return mul2(mul2(g, r), u);
 }
-__device__ __forceinline__ float gated_fast(float g, float u) { return gated_fast2(both(g), both(u)).x; }
 __device__ __forceinline__ void copy_async(uint32_t to, const char* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
@@ -771,7 +770,10 @@ template <typename T> static int launch_values(const void* codes, int64_t codes_
   while (across < most && across < items) across *= 2;
   const dim3 block((unsigned)across, (unsigned)(256 / across));
   const int64_t blocks = (rows + block.y - 1) / block.y;
-  const dim3 grid((unsigned)(blocks < 148 * 32 ? blocks : 148 * 32));
+  const int sms = row_sms();
+  if (sms < 0) return TRI_ERR_CUDA;
+  const int64_t most_blocks = (int64_t)sms * 32;            // (8 are resident; the rest evens out the last turn)
+  const dim3 grid((unsigned)(blocks < most_blocks ? blocks : most_blocks));
   const int8_t* c = static_cast<const int8_t*>(codes);
   if (vector) TRI_CUDA(launch_chained(dequantize_rows_kernel<T, true>, grid, block, 0, s, c, codes_stride, scales, static_cast<T*>(out), out_stride, rows, width), "values");
   else TRI_CUDA(launch_chained(dequantize_rows_kernel<T, false>, grid, block, 0, s, c, codes_stride, scales, static_cast<T*>(out), out_stride, rows, width), "values");
