@@ -318,9 +318,9 @@ int tri_qk_accumulators(const int32_t* requests, int num_requests, const void* q
  * other tensors: */
 enum { TRI_BF16 = 0, TRI_FP16 = 1, TRI_FP32 = 2 };
 /* Strides are in elements, features contiguous; width 1..131071 (128 * 128 * width < 2^31); rows = 0 is a no-op.
- * scale = max|y| / 127, code = rint(y / scale) (of a norm the nearest code up to fp32 roundings: on a tie either).  A row whose largest magnitude is below 2^-119 gets scale 0 and codes 0; a row
- * with a NaN, an infinity or an overflow in it gets scale NaN and codes 0.  Output buffers must not overlap inputs, except
- * residual_out, which may be residual or x itself (same stride). */
+ * scale = max|y| / 127, code = rint(y / scale).  A row whose largest magnitude (of a norm that of h * weight, before the root divides
+ * it) is below 2^-119 gets scale 0 and codes 0; a row with a NaN, an infinity or an overflow in it gets scale NaN and codes 0.
+ * Output buffers must not overlap inputs, except residual_out, which may be residual or x itself (same stride). */
 
 /* y = x. */
 int tri_quantize_rows(const void* x, int type, int64_t rows, int width, int64_t x_stride, void* codes, int64_t codes_stride,

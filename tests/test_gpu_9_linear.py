@@ -686,10 +686,9 @@ def test_gated_codes_are_those_of_fp32(ops, rows, width, dtype):
 @pytest.mark.parametrize("rows,width", TIE_SHAPES)
 @pytest.mark.parametrize("residual", (False, True))
 def test_norm_codes_next_to_ties(ops, rows, width, dtype, residual):
-    """A norm's code is the nearest to q = 127 y / max|y|, y = fl(h * weight), up to the fp32 roundings between them, in steps of 2^-24:
-    fl(1/127) and its product half a step each (1 + 1 of 2^-24), the approximate reciprocal one step (2), the product (1).  On a tie
-    either neighbour is as near.  Every row of ties, powers of two in front of it that send its squares out of fp32's range, rows
-    as they come."""
+    """A norm's code is rint(q), q = 127 y / max|y| rounded to fp32 once (2^-24 of q), y = fl(h * weight), ties to even: as exact arithmetic
+    has it on rows of ties (multiples of half a weight), with powers of two in front that send the squares out of fp32's range,
+    and on the ties among rows as they come."""
     y = rows_of_ties(rows, width, 99)
     gen = torch.Generator("cuda").manual_seed(100)
     w = 2.0 ** torch.randint(-1, 2, (width,), generator=gen, device="cuda")
@@ -704,8 +703,11 @@ def test_norm_codes_next_to_ties(ops, rows, width, dtype, residual):
             assert torch.equal(got[1], x)
             got = got[0]
         z = (x.float() * weight.float()).double()
-        q = z * 127 / z.abs().amax(1, keepdim=True)
-        assert float(((got.codes.double() - q).abs() - q.abs() * 5 * U).max()) <= 0.5
+        q = z * 127 / z.abs().amax(1, keepdim=True)       # 127 z has 31 bits: a tie in float64 where the exact quotient is one, else 2^-32 away
+        code = got.codes.double()
+        assert float(((code - q).abs() - q.abs() * U).max()) <= 0.5
+        tie = (q - q.floor()) == 0.5
+        assert torch.equal(code[tie], torch.round(q[tie])) and (h is cases[-1][0] or bool(tie.any()))
 
 
 # ---- copies --------------------------------------------------------------------------------------------------------------

@@ -12,11 +12,11 @@
 // with CUDA's expf (the file is compiled without --use_fast_math).  Approximate instructions are used on the way, but every
 // element whose code they might change is worked out again.  A row's largest element can be eighty times its root mean square, so a
 // code that is off by one step where y / s is next to a tie would be off by more than half of that.
-// Normed rows: the code is rint of h * w times the approximate reciprocal of max|h * w| / 127.  It is the nearest code up to the
-// roundings in between, 5 * 2^-24 of the quotient (|code - quotient| <= 1/2 + 3.8e-5); on a tie, which exact products of 16-bit
-// numbers do meet, it may be either neighbour, both of which are as far from y.  Deciding ties as exact arithmetic does changed 183
-// of 58.7 million codes of 16384 x 3584 and took 80 us for 74 (71 for 53 without a residual).  The scale's root is approximate too
-// (2^-22.9).  h is rounded to the stream's type before it is normed, because that is what later layers read.
+// Normed rows: the code is rint(127 y / max|y|) of y = h * w in fp32 (exact for 16-bit types), the quotient rounded to fp32 once: on
+// a tie, which products of 16-bit numbers do meet, the even code as exact arithmetic has it.  (The quotient comes from the reciprocal
+// in two terms.  With one, 1273 of 58.7 million codes of 16384 x 3584 in bf16 fell on a tie's other side; 54 us without a residual,
+// 57 like this, 73 and 69 with one; deciding near ties by a branch took 71 and 80.)  The scale's root is approximate (2^-22.9).  h is
+// rounded to the stream's type before it is normed, because that is what later layers read.
 #include "common.cuh"
 #include "abi_internal.h"
 #include <type_traits>
@@ -88,6 +88,7 @@ __device__ __forceinline__ bool squares_fit(float squares) { return squares < 3e
 
 struct RowScale {
   float scale, inverse;                 // inverse: of max|y| / 127, before the norm's common factor
+  float rest;                           // norm: what `inverse` lacks of 127 / max|y| (inverse + rest: to 2^-45)
   bool live;                            // codes are not all zero
 };
 // (Every thread of a row works this out, and it weighs as much as eight elements: approximate reciprocal and root, 2^-22.9.)
@@ -107,6 +108,7 @@ template <int Mode> __device__ __forceinline__ RowScale row_scale(uint32_t peak,
   r.live = finite && !zero;
   r.scale = !finite ? CUDART_NAN_F : zero ? 0.f : fminf(r.scale, RowLargestScale);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inverse) : "f"(r.live ? step : 1.f));
+  if (Mode == RowNorm) r.rest = fmaf(-r.inverse, __uint_as_float(peak), 127.f) * (r.inverse * (1.f / 127.f));
   return r;
 }
 
@@ -153,7 +155,7 @@ template <typename T, int Mode> __device__ __noinline__ void row_general(const R
   int8_t* codes = p.codes + row * p.codes_stride;
   for (int e = threadIdx.x; e < p.width; e += threads) {
     const float y = row_element<T, Mode>(p, a, b, sum, e, shift, squares);
-    codes[e] = !r.live ? (int8_t)0 : (int8_t)__float2int_rn(Mode == RowNorm ? y * r.inverse : y / r.scale);
+    codes[e] = !r.live ? (int8_t)0 : (int8_t)__float2int_rn(Mode == RowNorm ? fmaf(y, r.inverse, y * r.rest) : y / r.scale);
   }
 }
 
@@ -580,7 +582,8 @@ template <typename T, int Mode, int V, int Layout> __global__ void __launch_boun
       float off = 0.f, size = 0.f;      // largest distance from the next code, largest quotient
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
-        const float2 q = mul2(make_float2(y[j][i], y[j][i + 1]), both(inverse)), up = add2(q, both(Round));
+        const float2 two_y = make_float2(y[j][i], y[j][i + 1]);
+        const float2 q = Mode == RowNorm ? fma2(two_y, both(inverse), mul2(two_y, both(r.rest))) : mul2(two_y, both(inverse)), up = add2(q, both(Round));
         c[i] = __float_as_uint(up.x); c[i + 1] = __float_as_uint(up.y);
         if (Mode != RowNorm) {
           const float2 back = add2(up, both(-Round)), from = fma2(back, both(-1.f), q);
