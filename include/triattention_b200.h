@@ -341,10 +341,11 @@ int tri_dequantize_rows(const void* codes, int64_t codes_stride, const float* sc
                         void* out, int64_t out_stride, void* stream);
 
 /* out[t][n] = (sum_k codes[t][k] weight[n][k]) * weight_scales[n] * scales[t] + bias[n] + residual[t][n]: the sum is an exact
- * 32-bit integer, the rest f32 (channel scale; token scale and bias fused; residual), rounded once to the type.  Any sizes and
- * output strides; output and residual rows on 16-byte boundaries are accessed 16 bytes at a time.  No workspace.  codes int8 [tokens,width], weight int8 [outputs,width] (both code
- * rows), scales f32 [tokens], weight_scales f32 [outputs]; bias [outputs] and residual [tokens,outputs] of the output's type
- * or NULL.  out must not overlap any input except residual itself (same stride). */
+ * 32-bit integer, the rest IEEE f32 (channel scale; token scale and bias fused; residual), rounded once to the type.  Any sizes and
+ * output strides; output and residual rows on 16-byte boundaries are accessed 16 bytes at a time.  No workspace.  codes int8
+ * [tokens,width], weight int8 [outputs,width] (both code rows), scales f32 [tokens], weight_scales f32 [outputs]; bias [outputs]
+ * and residual [tokens,outputs] of the output's type or NULL.  out must not overlap any input except residual itself (same
+ * stride).  A bounded wait that runs out leaves void results and sets device_error. */
 int tri_int8_linear(const void* codes, int64_t codes_stride, const float* scales, const void* weight, int64_t weight_stride,
                     const float* weight_scales, const void* bias, const void* residual, int64_t residual_stride, void* out,
                     int64_t out_stride, int type, int64_t tokens, int outputs, int width, int* device_error, void* stream);

@@ -278,7 +278,7 @@ template <typename T> struct RowVector {
 // ---- rows that start anywhere ---------------------------------------------------------------------------------------------
 // Memory is read and written in aligned blocks of 16 bytes, and vectors are shifted out of two neighbouring ones.  Blocks that reach
 // over an end of the tensor (of the row, where something is written) are taken element by element.  8192 x 4095 in single
-// elements, 2 bytes an access, and like this: plain 62 and 35 us, gated 91 and 59, norm with residual 140 and 87, values 65 and 30.
+// elements, 2 bytes an access, and like this: plain 62 and 35 us, gated 91 and 59, norm with residual 140 and 85, values 65 and 30.
 // 16 bytes from byte `shift` (0..15) on of lo, hi.  (Four branches, one of which a whole row takes: 59 us for the gated rows above,
 // 65 with selects.)
 __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint32_t shift) {
@@ -718,8 +718,10 @@ template <typename T, int Mode> static int launch_rows_type(const RowArgs& p, in
   const int vectors = p.width / N;
   // Vectors per thread.  One while there are few rows (a trip to memory and a reduction bound the call); for long batches as
   // many as pay for what a thread does once a row, as few as keep warps on the SM.  Measured (us, 1 / 2 / 4 vectors): norm
-  // 16384 x 3584 with residual 73 / 76 / 81, 16384 x 8192 142 / 167 / 163; gated 8192 x 4096 51 / 43 / 39, 8192 x 8192
-  // 97 / 83 / 72, 8192 x 14336 146 / 147 / 129; plain 16384 x 4096 58 / 44 / 45, 16384 x 8192 116 / 83 / 79.
+  // 16384 x 3584 with residual 69 / 78 / 82, without 57 / 54 / 67, 16384 x 8192 146 / 172 / 162 and 122 / 115 / 120; gated
+  // 8192 x 4096 51 / 43 / 39, 8192 x 8192 97 / 83 / 72, 8192 x 14336 146 / 146 / 129; plain 16384 x 4096 58 / 43 / 44, 16384 x 8192
+  // 117 / 83 / 80.  (A norm keeps one without a residual too: the sum of squares takes another order with two, and a row's scale has
+  // the same bits whatever batch it is in.)
   const int want = p.rows <= 2 * sms || Mode == RowNorm ? 1 : Mode == RowGated || vectors > 512 ? 4 : 2;
   if (p.width % N == 0 && vector_rows(p.a, p.a_stride) && vector_rows(p.b, p.b_stride) && vector_rows(p.weight, 0) &&
       vector_rows(p.sum, p.sum_stride) && vectors <= 4096) {
@@ -732,8 +734,8 @@ template <typename T, int Mode> static int launch_rows_type(const RowArgs& p, in
     return launch_rows_ring<T, Mode, 4>(p, sms, s);
   }
   // Rows that start anywhere: four vectors do not fit into the registers beside the shifts.  1 / 2 / 4 vectors: plain 8192 x 4095
-  // 40 / 37 / 40, 16384 x 101 8.1 / 9.8 / 16; gated 8192 x 4095 75 / 66 / 95, 16384 x 101 12 / 19 / 39; norm with residual
-  // 8192 x 4095 92 / 111 / 141.
+  // 38 / 35 / 36, 16384 x 101 8.1 / 9.8 / 16; gated 8192 x 4095 68 / 59 / 78, 16384 x 101 12 / 19 / 39; norm with residual
+  // 8192 x 4095 85 / 111 / 142, without 52 / 54 / 66.
   if ((want == 1 || vectors <= 32) && vectors < 1024) return launch_rows_kernel<T, Mode, 1, RowAnywhere>(p, sms, s);
   if (vectors < 2048) return launch_rows_kernel<T, Mode, 2, RowAnywhere>(p, sms, s);
   if (vectors < 4096) return launch_rows_kernel<T, Mode, 4, RowAnywhere>(p, sms, s);
