@@ -756,3 +756,63 @@ def test_linear_keeps_subnormal_numbers(ops, tokens, outputs, width, dtype):
     x.codes[:, 0] = 3
     x.scales.fill_(2.0 ** -60), w.scales.fill_(least * 2.0 ** 60)        # (2^-60 each way: 3 * 2^60 * 2^-60 * least)
     assert torch.equal(ops.linear(x, w, dtype=dtype), torch.full((tokens, outputs), 3 * least, dtype=FP32, device="cuda").to(dtype))
+
+
+# ---- the largest tensors, broadcast residuals --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("width", (32768, 32765))
+def test_rows_past_32_bits(ops, width):
+    """2.3e9 elements, 4.6 GB an operand: the last rows are what they are alone."""
+    rows = 70001
+    x, u = (torch.empty(rows, width, dtype=BF16, device="cuda") for _ in range(2))
+    for t, seed in ((x, 140), (u, 141)):
+        t.copy_(randn(1, width, seed=seed).expand(rows, width))
+        t[-3:] = randn(3, width, seed=seed + 2)
+    w = (1 + 0.1 * randn(width, seed=144, dtype=FP32)).to(BF16)
+    last = slice(rows - 3, rows)
+    for call in (lambda p: ops.quantize_rows(x[p]), lambda p: ops.silu_mul(x[p], u[p]), lambda p: ops.rms_norm(x[p], w, 1e-6, residual=u[p])):
+        got, want = call(slice(None)), call(last)
+        if isinstance(got, tuple):
+            assert torch.equal(got[1][last], want[1])
+            got, want = got[0], want[0]
+        assert torch.equal(got.codes[last], want.codes) and torch.equal(got.codes[1], got.codes[rows - 4])
+        if width % 8 == 0:                      # (rows that lie alike)
+            assert torch.equal(got.scales[last], want.scales)
+        else:
+            torch.testing.assert_close(got.scales[last], want.scales, rtol=46 * U, atol=0)
+        part = Int8Rows(got.codes[last], got.scales[last])
+        assert torch.equal(ops.dequantize(got)[last], ops.dequantize(part))
+        del got, want, part
+
+
+@pytest.mark.parametrize("tokens,outputs,width", [(40001, 65536, 48), (40001, 65533, 48)])
+def test_linear_results_past_32_bits(ops, tokens, outputs, width):
+    x, w = codes_rows(tokens, width, 150), codes_rows(outputs, width, 151)
+    bias, residual = randn(outputs, seed=152), randn(1, outputs, seed=153).expand(tokens, outputs)
+    got = ops.linear(x, w, bias=bias, residual=residual)
+    for lo in (0, 32760, tokens - 5):
+        part = slice(lo, lo + 5)
+        assert torch.equal(got[part], ops.linear(Int8Rows(x.codes[part], x.scales[part]), w, bias=bias, residual=residual[part]))
+    ops.module.check_device_error()
+
+
+def test_linear_weights_past_32_bits(ops):
+    outputs, width = 200003, 16384
+    w = codes_rows(outputs, width, 154)
+    last = Int8Rows(w.codes[-300:], w.scales[-300:])
+    for tokens in (1, 7, 300):
+        x = codes_rows(tokens, width, 155 + tokens)
+        assert torch.equal(ops.linear(x, w)[:, -300:], ops.linear(x, last))
+        check_linear(ops, x, last)
+
+
+@pytest.mark.parametrize("tokens", (1, 3, 40, 300, 2500))
+def test_linear_residuals_that_lie_otherwise(ops, tokens):
+    """One row for all tokens, rows further apart, odd offsets, a transposed batch: the values count."""
+    x, w = codes_rows(tokens, 260, 160), codes_rows(520, 260, 161)
+    for residual in (randn(1, 520, seed=162).expand(tokens, 520), randn(tokens, 1100, seed=163)[:, 5:525], randn(tokens, 528, seed=164)[:, 8:]):
+        assert torch.equal(ops.linear(x, w, residual=residual), ops.linear(x, w, residual=residual.contiguous()))
+    if tokens % 4 == 0:
+        cube = Int8Rows(x.codes.view(4, tokens // 4, 260), x.scales.view(4, tokens // 4))
+        turned = randn(tokens // 4, 4, 520, seed=165).transpose(0, 1)
+        assert torch.equal(ops.linear(cube, w, residual=turned).view(tokens, 520), ops.linear(x, w, residual=turned.reshape(tokens, 520)))
