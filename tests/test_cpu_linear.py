@@ -343,7 +343,7 @@ def test_copies_of_the_executor(lib):
     import copy
     import pickle
     ops = Int8Ops(Module(lib))
-    assert copy.deepcopy(ops) is ops and copy.deepcopy([ops])[0] is ops
+    assert copy.deepcopy(ops) is ops and copy.deepcopy([ops])[0] is ops and copy.copy(ops) is ops
     with pytest.raises(RuntimeError, match="Int8Rows"):
         pickle.dumps(ops)
 

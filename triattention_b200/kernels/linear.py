@@ -131,7 +131,10 @@ class Int8Ops:
         self._launch, self._calls = module._launch, (lib.tri_quantize_rows, lib.tri_silu_mul_rows, lib.tri_rms_norm_rows,
                                                      lib.tri_dequantize_rows, lib.tri_int8_linear)
 
-    def __deepcopy__(self, memo):       # (the loaded library, and no data)
+    def __copy__(self):                 # (the loaded library, and no data)
+        return self
+
+    def __deepcopy__(self, memo):
         return self
 
     def __reduce__(self):
