@@ -17,8 +17,8 @@
 //
 // Measured on one B200 (device time; DRAM-cold weights): 16 x 4096 -> 128256 fp32 84 us = 6.3 TB/s, bound by HBM; 32 x 3584 -> 4608
 // 8.2-9.0 us depending on the GPU, bound by latencies (launch, first bytes, cluster exchange: of width 128 3.0, of 1024 5.1, the
-// smallest product 2.7);
-// 16384 x 14336 -> 4096 with residual 602-632 us = 3.0-3.2 POP/s in bursts, bound by the 1000 W limit when it runs for seconds.
+// smallest product 2.7); 16384 x 14336 -> 4096 with residual 602-632 us = 3.0-3.2 POP/s in bursts, bound by the 1000 W limit when it
+// runs for seconds.
 #include "tcgen05.cuh"
 #include "abi_internal.h"
 #include <mutex>

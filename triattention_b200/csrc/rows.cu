@@ -14,9 +14,10 @@
 // code that is off by one step where y / s is next to a tie would be off by more than half of that.
 // Normed rows: the code is rint(127 y / max|y|) of y = h * w in fp32 (exact for 16-bit types), the quotient rounded to fp32 once: on
 // a tie, which products of 16-bit numbers do meet, the even code as exact arithmetic has it.  (The quotient comes from the reciprocal
-// in two terms.  With one, 1273 of 58.7 million codes of 16384 x 3584 in bf16 fell on a tie's other side; 54 us without a residual,
-// 57 like this; 73 and 68 with one in a replayed graph, 71 and 73 called one by one; deciding near ties by a branch took 71 and 80.)  The scale's root is approximate (2^-22.9).  h is
-// rounded to the stream's type before it is normed, because that is what later layers read.
+// in two terms.  With one, 1273 of 58.7 million codes of 16384 x 3584 in bf16 fell on a tie's other side.  Times of that size: 54 us
+// without a residual, 57 like this; with one 73 and 68 in a replayed graph, 71 and 73 called one by one; deciding near ties by a
+// branch took 71 and 80.)  The scale's root is approximate (2^-22.9).  h is rounded to the stream's type before it is normed,
+// because that is what later layers read.
 #include "common.cuh"
 #include "abi_internal.h"
 #include <type_traits>

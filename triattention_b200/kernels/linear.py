@@ -123,8 +123,8 @@ class Int8Ops:
     inputs that ask for one are refused while gradients are being recorded, and inputs with a forward-mode tangent always.
 
     A product whose bounded waits ran out (a GPU that others hold up for seconds) returns all the same, with void results, and says so
-    in the GPU's error word: call ``ops.module.check_device_error()``, which synchronises and raises, before results are relied
-    on.  ``TriAttention.generate`` does."""
+    in the GPU's error word: call ``ops.module.check_device_error()``, which waits for the current stream and raises, before results
+    are relied on.  ``TriAttention.generate`` does."""
 
     def __init__(self, module):
         self.module, lib = module, module.lib
